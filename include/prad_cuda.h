@@ -528,6 +528,70 @@ prad_status prad_rmsnorm_forward(prad_ctx* ctx, prad_dtype dt, const void* x, co
 prad_status prad_rmsnorm_backward(prad_ctx* ctx, prad_dtype dt, const void* x, const void* g,
                                   const void* dy, void* dx, void* dg, int64_t rows, int cols);
 
+/* ---------------------------------------------------------------- state space layers
+ * Not in the reference, whose sequence models are the LSTM examples and attention: the operators of a layer that keeps a
+ * state per channel instead.  Tokens of all sequences are the rows of one matrix, channels its columns; `offsets` (device,
+ * sequences + 1 ascending row numbers) says which rows are whose, and NULL means tokens / sequences rows each.  A sequence may
+ * have no row.  Rows in front of offsets[0] and from offsets[sequences] on belong to none: results there stay as they
+ * were.  Offsets that do not ascend give wrong results, but no access outside the matrices.  A pitch (ld_*) of 0 is a dense
+ * matrix; u and z, say, may be column ranges of one product.  Results may not overlap inputs unless it says so.
+ * `swish` != 0 applies x * sigmoid(x).  All of these can be recorded into launch sequences.
+ *
+ * Group normalisation, channels last: x is [samples x positions x channels]; a group is channels / groups neighbouring channels
+ * of all positions of a sample (positions == 1: one norm per row).  xhat = (x - mean) * rstd with rstd = 1 / sqrt(variance + eps)
+ * (population variance); y = xhat * gamma + beta, then swish.  gamma, beta: [channels], NULL for 1 and 0.  mean, rstd: [samples x
+ * groups], the op's state.  The backward is the whole Jacobian; dgamma, dbeta may be NULL; dx may be dy. */
+prad_status prad_group_norm_forward(prad_ctx* ctx, prad_dtype dt, const void* x, const void* gamma, const void* beta, void* y,
+                                    void* mean, void* rstd, int64_t samples, int64_t positions, int channels, int groups,
+                                    double eps, int swish);
+prad_status prad_group_norm_backward(prad_ctx* ctx, prad_dtype dt, const void* x, const void* gamma, const void* beta,
+                                     const void* mean, const void* rstd, const void* dy, void* dx, void* dgamma, void* dbeta,
+                                     int64_t samples, int64_t positions, int channels, int groups, int swish);
+/* Dropout without a stored mask: y[i] = x[i] / (1 - p) where word i mod 4 of Philox4x32-10 with the counter (i / 4, offset) and
+ * the key `seed` is below (1 - p) * 2^32, else 0; plus residual[i] if residual is not NULL.  Backward is the same call on dy,
+ * without a residual, with the same seed and offset.  `step`: NULL, or a device uint64 that is added to offset when the
+ * kernel runs, so that each replay of a recorded sequence can draw a mask of its own.  y may be x or residual. */
+prad_status prad_dropout(prad_ctx* ctx, prad_dtype dt, const void* x, const void* residual, void* y, int64_t n, double p,
+                         uint64_t seed, uint64_t offset, const uint64_t* step);
+/* Causal convolution per channel: y_t = swish(bias + sum_k w[c][k] * x_(t - (width - 1) + k)), w [dim x width], width at most
+ * PRAD_CONV_MAX_WIDTH.  state [sequences x (width - 1) x dim]: the rows in front of each sequence, oldest first (NULL: zero);
+ * state_out: the same after its last token (NULL: not wanted).  The backward does not differentiate state_out; dw, dbias and
+ * dstate may be NULL.  prad_causal_conv_step takes one new row of each of `batch` sequences; state_out may be state. */
+#define PRAD_CONV_MAX_WIDTH 8
+prad_status prad_causal_conv_forward(prad_ctx* ctx, prad_dtype dt, const void* x, int64_t ld_x, const void* w, const void* bias,
+                                     const void* state, const int32_t* offsets, void* y, int64_t ld_y, void* state_out, int sequences,
+                                     int64_t tokens, int dim, int width, int swish);
+prad_status prad_causal_conv_backward(prad_ctx* ctx, prad_dtype dt, const void* x, int64_t ld_x, const void* w, const void* bias,
+                                      const void* state, const int32_t* offsets, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx,
+                                      void* dw, void* dbias, void* dstate, int sequences, int64_t tokens, int dim, int width, int swish);
+prad_status prad_causal_conv_step(prad_ctx* ctx, prad_dtype dt, const void* x, int64_t ld_x, const void* w, const void* bias,
+                                  const void* state, void* y, int64_t ld_y, void* state_out, int64_t batch, int dim, int width, int swish);
+/* Selective scan.  Channel d belongs to group d / (dim / groups) and has `state` states (at most 128):
+ *   dt = delta + delta_bias[d], softplus of it if delta_softplus;  h_n <- exp(dt * A[d][n]) * h_n + dt * u * B[group][n];
+ *   r = sum_n C[group][n] * h_n + D[d] * u;  y = r, or r * swish(z) with a z.
+ * u, delta, z, y: [tokens x dim]; A: [dim x state]; B, C: [tokens x groups * state]; D, delta_bias: [dim]; h0, h_last: [sequences
+ * x dim * state].  z, D, delta_bias and h0 may be NULL (none, 0, 0, 0), h_last as well.  `saved` (prad_selective_scan_saved_bytes
+ * of the same scan) keeps what the backward needs; NULL where none follows.  The backward does not differentiate h_last; of its
+ * results dA, dD, ddelta_bias and dh0 may be NULL, and dz where there is no z. */
+typedef struct {
+  int64_t tokens;
+  int32_t sequences, dim, state, groups, delta_softplus;
+  const int32_t *offsets;
+  const void *u, *delta, *z, *A, *B, *C, *D, *delta_bias, *h0;
+  int64_t ld_u, ld_delta, ld_z, ld_B, ld_C;
+} prad_scan_t;
+typedef struct {
+  void *du, *ddelta, *dz, *dA, *dB, *dC, *dD, *ddelta_bias, *dh0;
+  int64_t ld_du, ld_ddelta, ld_dz, ld_dB, ld_dC;
+} prad_scan_gradients_t;
+prad_status prad_selective_scan_saved_bytes(prad_dtype dt, const prad_scan_t* scan, size_t* out_bytes);
+prad_status prad_selective_scan_forward(prad_ctx* ctx, prad_dtype dt, const prad_scan_t* scan, void* y, int64_t ld_y, void* h_last,
+                                        void* saved);
+prad_status prad_selective_scan_backward(prad_ctx* ctx, prad_dtype dt, const prad_scan_t* scan, const void* saved, const void* dy,
+                                         int64_t ld_dy, const prad_scan_gradients_t* gradients);
+/* One new token for each of `sequences` == tokens sequences: h0 is the state, h_out (which may be h0) the new one. */
+prad_status prad_selective_scan_step(prad_ctx* ctx, prad_dtype dt, const prad_scan_t* scan, void* y, int64_t ld_y, void* h_out);
+
 /* ---------------------------------------------------------------- losses
  * Loss/MeanSquaredErrorLossOperation.cs:37-84 and
  * Loss/CategoricalCrossEntropyLossOperation.cs:37-87.  loss_out is one device scalar.

@@ -88,6 +88,7 @@ namespace ParallelReverseAutoDiff.RMAD.Cuda
         }
 
         public const int StaticColsumMaxCols = 32768;
+        public const int ConvMaxWidth = 8;
         public const int DpMarks = 256;
 
         [StructLayout(LayoutKind.Sequential, CharSet = CharSet.Ansi)]
@@ -104,6 +105,23 @@ namespace ParallelReverseAutoDiff.RMAD.Cuda
             [MarshalAs(UnmanagedType.ByValTStr, SizeConst = 48)] public string Label;
             public double Milliseconds;
             public long Launches;
+        }
+
+        [StructLayout(LayoutKind.Sequential)]
+        public struct Scan
+        {
+            public long Tokens;
+            public int Sequences, Dim, State, Groups, DeltaSoftplus;
+            public IntPtr Offsets;
+            public IntPtr U, Delta, Z, A, B, C, D, DeltaBias, H0;
+            public long LdU, LdDelta, LdZ, LdB, LdC;
+        }
+
+        [StructLayout(LayoutKind.Sequential)]
+        public struct ScanGradients
+        {
+            public IntPtr Du, Ddelta, Dz, DA, DB, DC, DD, DdeltaBias, Dh0;
+            public long LdDu, LdDdelta, LdDz, LdDB, LdDC;
         }
 
         [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
@@ -381,6 +399,36 @@ namespace ParallelReverseAutoDiff.RMAD.Cuda
 
         [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
         public static extern int prad_rmsnorm_backward(IntPtr ctx, DType dt, IntPtr x, IntPtr g, IntPtr dy, IntPtr dx, IntPtr dg, long rows, int cols);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_group_norm_forward(IntPtr ctx, DType dt, IntPtr x, IntPtr gamma, IntPtr beta, IntPtr y, IntPtr mean, IntPtr rstd, long samples, long positions, int channels, int groups, double eps, int swish);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_group_norm_backward(IntPtr ctx, DType dt, IntPtr x, IntPtr gamma, IntPtr beta, IntPtr mean, IntPtr rstd, IntPtr dy, IntPtr dx, IntPtr dgamma, IntPtr dbeta, long samples, long positions, int channels, int groups, int swish);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_dropout(IntPtr ctx, DType dt, IntPtr x, IntPtr residual, IntPtr y, long n, double p, ulong seed, ulong offset, IntPtr step);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_causal_conv_forward(IntPtr ctx, DType dt, IntPtr x, long ld_x, IntPtr w, IntPtr bias, IntPtr state, IntPtr offsets, IntPtr y, long ld_y, IntPtr state_out, int sequences, long tokens, int dim, int width, int swish);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_causal_conv_backward(IntPtr ctx, DType dt, IntPtr x, long ld_x, IntPtr w, IntPtr bias, IntPtr state, IntPtr offsets, IntPtr dy, long ld_dy, IntPtr dx, long ld_dx, IntPtr dw, IntPtr dbias, IntPtr dstate, int sequences, long tokens, int dim, int width, int swish);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_causal_conv_step(IntPtr ctx, DType dt, IntPtr x, long ld_x, IntPtr w, IntPtr bias, IntPtr state, IntPtr y, long ld_y, IntPtr state_out, long batch, int dim, int width, int swish);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_selective_scan_saved_bytes(DType dt, ref Scan scan, out UIntPtr out_bytes);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_selective_scan_forward(IntPtr ctx, DType dt, ref Scan scan, IntPtr y, long ld_y, IntPtr h_last, IntPtr saved);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_selective_scan_backward(IntPtr ctx, DType dt, ref Scan scan, IntPtr saved, IntPtr dy, long ld_dy, ref ScanGradients gradients);
+
+        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
+        public static extern int prad_selective_scan_step(IntPtr ctx, DType dt, ref Scan scan, IntPtr y, long ld_y, IntPtr h_out);
 
         [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]
         public static extern int prad_mse_forward(IntPtr ctx, DType dt, IntPtr @out, IntPtr target, IntPtr loss_out, long rows, int cols);

@@ -22,10 +22,12 @@ OUT = os.path.join(HERE, "PradCuda.cs")
 ENUM_NAMES = {"prad_dtype": "DType", "prad_act": "Act", "prad_adam_form": "AdamForm", "prad_op": "Op",
               "prad_tensor_op": "TensorOp"}
 STRUCTS = {"prad_device_info_t": "DeviceInfo", "prad_timing_t": "Timing"}
+# structs of plain numbers and pointers that a call reads, emitted from the header
+IN_STRUCTS = {"prad_scan_t": "Scan", "prad_scan_gradients_t": "ScanGradients"}
 # C type -> C# type of a parameter
 SCALARS = {"int": "int", "int32_t": "int", "int64_t": "long", "double": "double", "size_t": "UIntPtr", "float": "float",
            "prad_status": "int", "uint64_t": "ulong"}
-OUT_SCALARS = {"int*": "out int", "int64_t*": "out long", "double*": "out double"}
+OUT_SCALARS = {"int*": "out int", "int64_t*": "out long", "double*": "out double", "size_t*": "out UIntPtr"}
 
 
 def strip_comments(text: str) -> str:
@@ -58,6 +60,24 @@ def parse_functions(text: str):
     return fns
 
 
+def cs_struct(text: str, cname: str):
+    """The fields of a plain struct as C# lines."""
+    body = next(b for b, n in re.findall(r"typedef\s+struct\s*\{([^}]*)\}\s*(\w+)\s*;", text) if n == cname)
+    lines = []
+    for decl in filter(None, (" ".join(d.split()) for d in body.split(";"))):
+        m = re.match(r"(?:const )?(\w+)\s*(.*)", decl)
+        names = [n.strip() for n in m.group(2).split(",")]
+        kind = "IntPtr" if names[0].startswith("*") else SCALARS[m.group(1)]
+        fields = []
+        for n in names:
+            n = n.lstrip("* ")
+            parts = [q[0].upper() + q[1:] for q in n.split("_")]
+            name = "".join(parts)
+            fields.append(name)
+        lines.append(f"public {kind} {', '.join(fields)};")
+    return lines
+
+
 def cs_param(p: str) -> str:
     p = p.strip()
     m = re.match(r"(.*?)(\w+)$", p)
@@ -75,6 +95,9 @@ def cs_param(p: str) -> str:
             if st == "prad_timing_t":
                 return f"[In, Out] {cs}[] {pname}"
             return f"out {cs} {pname}"
+    for st, cs in IN_STRUCTS.items():
+        if ctype_n == f"const{st}*":
+            return f"ref {cs} {pname}"
     if ctype_n in SCALARS:
         return f"{SCALARS[ctype_n]} {pname}"
     if ctype_n in OUT_SCALARS and pname.startswith("out"):
@@ -160,6 +183,14 @@ def generate() -> str:
     w("            public long Launches;")
     w("        }")
     w("")
+    for cname, cs in IN_STRUCTS.items():
+        w("        [StructLayout(LayoutKind.Sequential)]")
+        w(f"        public struct {cs}")
+        w("        {")
+        for line in cs_struct(text, cname):
+            w(f"            {line}")
+        w("        }")
+        w("")
     for ret, name, params in fns:
         cs_ret = "IntPtr" if ret.startswith("constchar") else "int"
         w(f"        [DllImport(Lib, CallingConvention = CallingConvention.Cdecl)]")

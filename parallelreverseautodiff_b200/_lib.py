@@ -12,7 +12,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libprad_cuda.so")
 
-vp, i32, i64, f64, sz = C.c_void_p, C.c_int, C.c_int64, C.c_double, C.c_size_t
+vp, i32, i64, f64, sz, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_double, C.c_size_t, C.c_uint64
 pvp = C.POINTER(C.c_void_p)
 pi64 = C.POINTER(C.c_int64)
 
@@ -114,6 +114,16 @@ SIGNATURES = {
     "prad_scale_shift_backward": [vp, i32, vp, vp, vp, vp, vp, vp, i64, i32],
     "prad_rmsnorm_forward": [vp, i32, vp, vp, vp, i64, i32],
     "prad_rmsnorm_backward": [vp, i32, vp, vp, vp, vp, vp, i64, i32],
+    "prad_group_norm_forward": [vp, i32, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, f64, i32],
+    "prad_group_norm_backward": [vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32],
+    "prad_dropout": [vp, i32, vp, vp, vp, i64, f64, u64, u64, vp],
+    "prad_causal_conv_forward": [vp, i32, vp, i64, vp, vp, vp, vp, vp, i64, vp, i32, i64, i32, i32, i32],
+    "prad_causal_conv_backward": [vp, i32, vp, i64, vp, vp, vp, vp, vp, i64, vp, i64, vp, vp, vp, i32, i64, i32, i32, i32],
+    "prad_causal_conv_step": [vp, i32, vp, i64, vp, vp, vp, vp, i64, vp, i64, i32, i32, i32],
+    "prad_selective_scan_saved_bytes": [i32, vp, C.POINTER(sz)],
+    "prad_selective_scan_forward": [vp, i32, vp, vp, i64, vp, vp],
+    "prad_selective_scan_backward": [vp, i32, vp, vp, vp, i64, vp],
+    "prad_selective_scan_step": [vp, i32, vp, vp, i64, vp],
     "prad_mse_forward": [vp, i32, vp, vp, vp, i64, i32],
     "prad_mse_backward": [vp, i32, vp, vp, vp, i64, i32, i64],
     "prad_cce_forward": [vp, i32, vp, vp, vp, i64, i32],
@@ -178,6 +188,21 @@ class DeviceInfo(C.Structure):
 class Timing(C.Structure):
     """prad_timing_t"""
     _fields_ = [("label", C.c_char * 48), ("milliseconds", C.c_double), ("launches", C.c_int64)]
+
+
+class Scan(C.Structure):
+    """prad_scan_t"""
+    _fields_ = [("tokens", C.c_int64), ("sequences", C.c_int32), ("dim", C.c_int32), ("state", C.c_int32), ("groups", C.c_int32),
+                ("delta_softplus", C.c_int32), ("offsets", vp), ("u", vp), ("delta", vp), ("z", vp), ("A", vp), ("B", vp), ("C", vp),
+                ("D", vp), ("delta_bias", vp), ("h0", vp), ("ld_u", C.c_int64), ("ld_delta", C.c_int64), ("ld_z", C.c_int64),
+                ("ld_B", C.c_int64), ("ld_C", C.c_int64)]
+
+
+class ScanGradients(C.Structure):
+    """prad_scan_gradients_t"""
+    _fields_ = [("du", vp), ("ddelta", vp), ("dz", vp), ("dA", vp), ("dB", vp), ("dC", vp), ("dD", vp), ("ddelta_bias", vp),
+                ("dh0", vp), ("ld_du", C.c_int64), ("ld_ddelta", C.c_int64), ("ld_dz", C.c_int64), ("ld_dB", C.c_int64),
+                ("ld_dC", C.c_int64)]
 
 
 _lib = None

@@ -1,0 +1,471 @@
+// The short convolution of a state space layer: per channel c over the tokens of each sequence,
+//   p_t = bias_c + sum_k w[c][k] x_(t - (W - 1) + k),  y_t = p_t or swish(p_t),
+// where the W - 1 rows before a sequence's first token come from its state (zero without one).  Backward, with g = dy swish'(p):
+//   dx_t = sum_k w[c][k] g_(t + W - 1 - k)  over the tokens of the sequence,  dw[c][k] = sum_t g_t x_(t - (W - 1) + k),  dbias = sum g.
+//
+// Bound by memory: a thread takes V neighbouring channels and walks down a run of tokens with the last W rows in registers, so that
+// a row is read once per run and W - 1 rows twice.
+#include "common.cuh"
+#include "packed_sequences.cuh"
+
+namespace prad {
+namespace conv {
+
+using seq::Sequences;
+using seq::swish;
+using seq::swish_slope;
+
+constexpr int LANES = 32, WARPS = 8, THREADS = LANES * WARPS;
+constexpr int RUN = 32;          // tokens of a thread's run
+
+template <typename T> struct Args {
+  Sequences rows;
+  const T *x, *w, *bias, *state, *dy;
+  T *y, *dx, *state_out, *dw, *dbias, *dstate;
+  int64_t ld_x, ld_y, ld_dy, ld_dx;
+  int dim, swish;
+};
+
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+
+// the row at place `p` of sequence s, which begins at row `start`: a token, or below zero a row of its state
+template <typename T, int V, int W>
+__device__ __forceinline__ Pack<T, V> row_at(const Args<T>& a, int s, int64_t start, int64_t p, int c) {
+  Pack<T, V> r;
+  if (p >= 0) return load<T, V>(a.x + (start + p) * a.ld_x + c);
+  if (a.state) return load<T, V>(a.state + ((int64_t)s * (W - 1) + (W - 1) + p) * a.dim + c);
+#pragma unroll
+  for (int j = 0; j < V; ++j) r.v[j] = 0;
+  return r;
+}
+
+template <typename T, int V, int W> struct Weights {
+  T w[W][V], bias[V];
+  __device__ __forceinline__ Weights(const Args<T>& a, int c) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k][j] = a.w[(int64_t)(c + j) * W + k];
+      bias[j] = a.bias ? a.bias[c + j] : (T)0;
+    }
+  }
+};
+
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(THREADS)
+forward_kernel(const Args<T> a) {
+  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
+  if (c >= a.dim) return;
+  const int64_t run = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int64_t lo = a.rows.begin(), hi = a.rows.finish();
+  int64_t t = run * RUN, last = t + RUN;
+  if (t < lo) t = lo;
+  if (last > hi) last = hi;
+  if (t >= last) return;
+  const Weights<T, V, W> wt(a, c);
+  int s = a.rows.at(t);
+  int64_t start = a.rows.start(s), end = a.rows.end(s);
+  if (start > t) start = t;     // (offsets that do not ascend)
+  Pack<T, V> x[W];              // x[W - 1]: the newest row
+#pragma unroll
+  for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, t - start - (W - k), c);
+  Pack<T, V> next = load<T, V>(a.x + t * a.ld_x + c);
+  for (; t < last; ++t) {
+    if (t == end) {
+      do ++s; while (s < a.rows.count && a.rows.end(s) <= t);
+      if (s >= a.rows.count) return;
+      start = t;
+      end = a.rows.end(s);
+#pragma unroll
+      for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, -(W - k), c);
+    }
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k) x[k] = x[k + 1];
+    x[W - 1] = next;
+    if (t + 1 < last) next = load<T, V>(a.x + (t + 1) * a.ld_x + c);
+    Pack<T, V> y;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      T p = wt.bias[j];
+#pragma unroll
+      for (int k = 0; k < W; ++k) p += wt.w[k][j] * x[k].v[j];
+      y.v[j] = a.swish ? swish(p) : p;
+    }
+    *reinterpret_cast<Pack<T, V>*>(a.y + t * a.ld_y + c) = y;
+  }
+}
+
+// state_out[s] = the last W - 1 rows of state[s] followed by the sequence's tokens
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(THREADS)
+state_kernel(const Args<T> a) {
+  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
+  const int64_t i = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (c >= a.dim || i >= (int64_t)a.rows.count * (W - 1)) return;
+  const int s = (int)(i / (W - 1)), k = (int)(i % (W - 1));
+  const int64_t start = a.rows.start(s);
+  int64_t len = a.rows.end(s) - start;
+  if (len < 0) len = 0;
+  *reinterpret_cast<Pack<T, V>*>(a.state_out + i * a.dim + c) = row_at<T, V, W>(a, s, start, len - (W - 1) + k, c);
+}
+
+// g at place q of a sequence
+template <typename T, int V, int W>
+__device__ __forceinline__ void slope(const Weights<T, V, W>& wt, const Pack<T, V> (&x)[W], const Pack<T, V>& dy, int act, T (&g)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    g[j] = dy.v[j];
+    if (act) {
+      T p = wt.bias[j];
+#pragma unroll
+      for (int k = 0; k < W; ++k) p += wt.w[k][j] * x[k].v[j];
+      g[j] *= swish_slope(p);
+    }
+  }
+}
+
+// A thread computes g over its run and the W - 1 tokens behind it, and dx of its run from the last W of them.
+// partial[block][W + 1][dim]: sums for dw (k = 0 .. W - 1) and dbias over the block's runs.
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(THREADS)
+backward_kernel(const Args<T> a, T* __restrict__ partial) {
+  __shared__ T part[WARPS][LANES * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = (blockIdx.y * LANES + lane) * V;
+  const bool on = c < a.dim;
+  const int64_t lo = a.rows.begin(), hi = a.rows.finish();
+  int64_t t = ((int64_t)blockIdx.x * WARPS + warp) * RUN, last = t + RUN;
+  if (t < lo) t = lo;
+  if (last > hi) last = hi;
+  T dw[W][V], db[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    db[j] = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k) dw[k][j] = 0;
+  }
+  if (on && t < last) {
+    const Weights<T, V, W> wt(a, c);
+    int s = a.rows.at(t);
+    while (t < last && s < a.rows.count) {
+      int64_t start = a.rows.start(s);
+      const int64_t end = a.rows.end(s);
+      if (start > t) start = t;                                // (offsets that do not ascend)
+      const int64_t stop = end < last ? end : last;            // of the tokens whose dx is this thread's
+      int64_t ahead = stop + W - 1;                            // of the tokens whose g they take
+      if (ahead > end) ahead = end;
+      Pack<T, V> x[W];
+#pragma unroll
+      for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, t - start - (W - k), c);
+      T g[W][V];                                               // g[W - 1]: the newest token's
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[k][j] = 0;
+      Pack<T, V> nx, nd;
+      if (t < ahead) {
+        nx = load<T, V>(a.x + t * a.ld_x + c);
+        nd = load<T, V>(a.dy + t * a.ld_dy + c);
+      }
+      for (int64_t q = t; q < stop + W - 1; ++q) {
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) {
+          x[k] = x[k + 1];
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[k][j] = g[k + 1][j];
+        }
+        if (q < ahead) {
+          x[W - 1] = nx;
+          const Pack<T, V> d = nd;
+          if (q + 1 < ahead) {
+            nx = load<T, V>(a.x + (q + 1) * a.ld_x + c);
+            nd = load<T, V>(a.dy + (q + 1) * a.ld_dy + c);
+          }
+          slope<T, V, W>(wt, x, d, a.swish, g[W - 1]);
+          if (q < stop)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              db[j] += g[W - 1][j];
+#pragma unroll
+              for (int k = 0; k < W; ++k) dw[k][j] += g[W - 1][j] * x[k].v[j];
+            }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[W - 1][j] = 0;
+        }
+        if (q - (W - 1) >= t) {                                // g[k] belongs to token q - (W - 1) + k
+          Pack<T, V> dx;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            dx.v[j] = 0;
+#pragma unroll
+            for (int k = 0; k < W; ++k) dx.v[j] += wt.w[W - 1 - k][j] * g[k][j];
+          }
+          *reinterpret_cast<Pack<T, V>*>(a.dx + (q - (W - 1)) * a.ld_dx + c) = dx;
+        }
+      }
+      t = stop;
+      do ++s; while (s < a.rows.count && a.rows.end(s) <= t);
+    }
+  }
+  // the warps' sums in the order of the warps
+#pragma unroll
+  for (int k = 0; k <= W; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[warp][lane * V + j] = k < W ? dw[k < W ? k : 0][j] : db[j];
+    __syncthreads();
+    for (int e = threadIdx.x; e < LANES * V; e += THREADS) {
+      const int ch = blockIdx.y * LANES * V + e;
+      T sum = 0;
+#pragma unroll
+      for (int r = 0; r < WARPS; ++r) sum += part[r][e];
+      if (ch < a.dim) partial[((int64_t)blockIdx.x * (W + 1) + k) * a.dim + ch] = sum;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+totals_kernel(const T* __restrict__ partial, int64_t blocks, int dim, int width, T* dw, T* dbias) {
+  __shared__ double part[WARPS][LANES];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * LANES + lane, k = blockIdx.y;
+  double sum = 0.0;
+  if (c < dim)
+#pragma unroll 4
+    for (int64_t b = warp; b < blocks; b += WARPS) sum += (double)partial[(b * (width + 1) + k) * dim + c];
+  part[warp][lane] = sum;
+  __syncthreads();
+  if (warp || c >= dim) return;
+  sum = 0.0;
+#pragma unroll
+  for (int r = 0; r < WARPS; ++r) sum += part[r][lane];
+  if (k < width) {
+    if (dw) dw[(int64_t)c * width + k] = (T)sum;
+  } else if (dbias) {
+    dbias[c] = (T)sum;
+  }
+}
+
+// dstate[s][i], the row at place i - (W - 1): sum over the places q <= i of the sequence of w[i - q] g_q
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(THREADS)
+state_gradient_kernel(const Args<T> a) {
+  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
+  const int64_t s64 = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (c >= a.dim || s64 >= a.rows.count) return;
+  const int s = (int)s64;
+  const int64_t start = a.rows.start(s), len = a.rows.end(s) - start;
+  const Weights<T, V, W> wt(a, c);
+  T sum[W][V];
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[i][j] = 0;
+#pragma unroll
+  for (int q = 0; q < W - 1; ++q)
+    if (q < len) {
+      Pack<T, V> x[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, q - (W - 1) + k, c);
+      T g[V];
+      slope<T, V, W>(wt, x, load<T, V>(a.dy + (start + q) * a.ld_dy + c), a.swish, g);
+#pragma unroll
+      for (int i = q; i < W - 1; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[i][j] += wt.w[i - q][j] * g[j];
+    }
+#pragma unroll
+  for (int i = 0; i < W - 1; ++i) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = sum[i][j];
+    *reinterpret_cast<Pack<T, V>*>(a.dstate + ((int64_t)s * (W - 1) + i) * a.dim + c) = o;
+  }
+}
+
+// one new row of each sequence; state_out may be the state itself
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(THREADS)
+step_kernel(const Args<T> a, int64_t batch) {
+  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
+  const int64_t s = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (c >= a.dim || s >= batch) return;
+  const Weights<T, V, W> wt(a, c);
+  Pack<T, V> x[W];
+#pragma unroll
+  for (int k = 0; k + 1 < W; ++k) x[k] = load<T, V>(a.state + (s * (W - 1) + k) * a.dim + c);
+  x[W - 1] = load<T, V>(a.x + s * a.ld_x + c);
+  Pack<T, V> y;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    T p = wt.bias[j];
+#pragma unroll
+    for (int k = 0; k < W; ++k) p += wt.w[k][j] * x[k].v[j];
+    y.v[j] = a.swish ? swish(p) : p;
+  }
+  *reinterpret_cast<Pack<T, V>*>(a.y + s * a.ld_y + c) = y;
+#pragma unroll
+  for (int k = 0; k + 1 < W; ++k) *reinterpret_cast<Pack<T, V>*>(a.state_out + (s * (W - 1) + k) * a.dim + c) = x[k + 1];
+}
+
+// ---------------------------------------------------------------- launches
+enum class Pass { Forward, Backward, Step };
+
+template <typename T, int V, int W> static prad_status launch(prad_ctx* ctx, const Args<T>& a, Pass pass) {
+  const unsigned across = (unsigned)ceil_div(a.dim, LANES * V);
+  if (pass == Pass::Step) {
+    step_kernel<T, V, W><<<dim3((unsigned)ceil_div(a.rows.tokens, WARPS), across), THREADS, 0, ctx->stream>>>(a, a.rows.tokens);
+    PRAD_LAUNCHED(ctx);
+    return PRAD_OK;
+  }
+  const int64_t blocks = ceil_div(a.rows.tokens, WARPS * RUN);
+  const dim3 grid((unsigned)blocks, across);
+  if (pass == Pass::Forward) {
+    if (blocks) {
+      forward_kernel<T, V, W><<<grid, THREADS, 0, ctx->stream>>>(a);
+      PRAD_LAUNCHED(ctx);
+    }
+    if (W > 1 && a.state_out && a.rows.count) {
+      state_kernel<T, V, W><<<dim3((unsigned)ceil_div((int64_t)a.rows.count * (W - 1), WARPS), across), THREADS, 0, ctx->stream>>>(a);
+      PRAD_LAUNCHED(ctx);
+    }
+    return PRAD_OK;
+  }
+  prad_status st = ensure_workspace(ctx, (size_t)(blocks ? blocks : 1) * (W + 1) * a.dim * sizeof(T));
+  if (st) return st;
+  if (blocks) {
+    backward_kernel<T, V, W><<<grid, THREADS, 0, ctx->stream>>>(a, (T*)ctx->ws);
+    PRAD_LAUNCHED(ctx);
+  }
+  if (a.dw || a.dbias) {
+    totals_kernel<T><<<dim3((unsigned)ceil_div(a.dim, LANES), W + 1), THREADS, 0, ctx->stream>>>((const T*)ctx->ws, blocks, a.dim, W,
+                                                                                              a.dw, a.dbias);
+    PRAD_LAUNCHED(ctx);
+  }
+  if (W > 1 && a.dstate && a.rows.count && !blocks) {
+    PRAD_CUDA(cudaMemsetAsync(a.dstate, 0, (size_t)a.rows.count * (W - 1) * a.dim * sizeof(T), ctx->stream));
+  } else if (W > 1 && a.dstate && a.rows.count) {
+    state_gradient_kernel<T, V, W><<<dim3((unsigned)ceil_div(a.rows.count, WARPS), across), THREADS, 0, ctx->stream>>>(a);
+    PRAD_LAUNCHED(ctx);
+  }
+  return PRAD_OK;
+}
+template <typename T, int V> static prad_status pick(prad_ctx* ctx, const Args<T>& a, Pass pass, int width) {
+  switch (width) {
+    case 1: return launch<T, V, 1>(ctx, a, pass);
+    case 2: return launch<T, V, 2>(ctx, a, pass);
+    case 3: return launch<T, V, 3>(ctx, a, pass);
+    case 4: return launch<T, V, 4>(ctx, a, pass);
+    case 5: return launch<T, V, 5>(ctx, a, pass);
+    case 6: return launch<T, V, 6>(ctx, a, pass);
+    case 7: return launch<T, V, 7>(ctx, a, pass);
+    default: return launch<T, V, 8>(ctx, a, pass);
+  }
+}
+template <typename T> static prad_status run(prad_ctx* ctx, const Args<T>& a, Pass pass, int width) {
+  constexpr int V = 16 / sizeof(T);
+  const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.dx | (uintptr_t)a.state |
+                        (uintptr_t)a.state_out | (uintptr_t)a.dstate;
+  const int64_t pitches = a.dim | a.ld_x | a.ld_y | a.ld_dy | a.ld_dx;
+  if ((all & 15) == 0 && pitches % V == 0) return pick<T, V>(ctx, a, pass, width);
+  return pick<T, 1>(ctx, a, pass, width);
+}
+
+static prad_status check(const char* who, prad_dtype dt, int64_t tokens, int sequences, const void* offsets, int dim, int width) {
+  PRAD_REQUIRE(dtype_ok(dt), PRAD_ERR_INVALID, "%s: unknown dtype %d", who, (int)dt);
+  PRAD_REQUIRE(tokens >= 0 && sequences >= 0 && dim > 0, PRAD_ERR_SHAPE, "%s: bad shape", who);
+  PRAD_REQUIRE(dim <= 1 << 20, PRAD_ERR_UNSUPPORTED, "%s: more than 2^20 channels", who);
+  PRAD_REQUIRE(width >= 1 && width <= PRAD_CONV_MAX_WIDTH, PRAD_ERR_UNSUPPORTED, "%s: widths of 1 to %d, got %d", who,
+               PRAD_CONV_MAX_WIDTH, width);
+  PRAD_REQUIRE(tokens <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens", who);
+  PRAD_REQUIRE(offsets || (sequences > 0 ? tokens % sequences == 0 : tokens == 0), PRAD_ERR_SHAPE,
+               "%s: %lld tokens do not divide into %d sequences", who, (long long)tokens, sequences);
+  PRAD_REQUIRE(((uintptr_t)offsets & 3) == 0, PRAD_ERR_INVALID, "%s: unaligned offsets", who);
+  return PRAD_OK;
+}
+static Sequences sequences_of(int64_t tokens, int sequences, const int32_t* offsets) {
+  return Sequences{offsets, sequences, tokens, offsets || sequences == 0 ? 0 : tokens / sequences};
+}
+static int64_t pitch(int64_t ld, int dim) { return ld ? ld : dim; }
+
+}  // namespace conv
+}  // namespace prad
+
+using namespace prad;
+
+template <typename T>
+static prad_status forward_t(prad_ctx* ctx, const void* x, int64_t ld_x, const void* w, const void* bias, const void* state,
+                             const int32_t* offsets, void* y, int64_t ld_y, void* state_out, int sequences, int64_t tokens, int dim,
+                             int width, int swish, conv::Pass pass) {
+  conv::Args<T> a = {};
+  a.rows = conv::sequences_of(tokens, sequences, offsets);
+  a.x = (const T*)x, a.w = (const T*)w, a.bias = (const T*)bias, a.state = (const T*)state;
+  a.y = (T*)y, a.state_out = (T*)state_out;
+  a.ld_x = ld_x, a.ld_y = ld_y, a.dim = dim, a.swish = swish;
+  return conv::run<T>(ctx, a, pass, width);
+}
+template <typename T>
+static prad_status backward_t(prad_ctx* ctx, const void* x, int64_t ld_x, const void* w, const void* bias, const void* state,
+                              const int32_t* offsets, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, void* dw, void* dbias,
+                              void* dstate, int sequences, int64_t tokens, int dim, int width, int swish) {
+  conv::Args<T> a = {};
+  a.rows = conv::sequences_of(tokens, sequences, offsets);
+  a.x = (const T*)x, a.w = (const T*)w, a.bias = (const T*)bias, a.state = (const T*)state, a.dy = (const T*)dy;
+  a.dx = (T*)dx, a.dw = (T*)dw, a.dbias = (T*)dbias, a.dstate = (T*)dstate;
+  a.ld_x = ld_x, a.ld_dy = ld_dy, a.ld_dx = ld_dx, a.dim = dim, a.swish = swish;
+  return conv::run<T>(ctx, a, conv::Pass::Backward, width);
+}
+
+extern "C" prad_status prad_causal_conv_forward(prad_ctx* ctx, prad_dtype dt, const void* x, int64_t ld_x, const void* w, const void* bias,
+                                                const void* state, const int32_t* offsets, void* y, int64_t ld_y, void* state_out,
+                                                int sequences, int64_t tokens, int dim, int width, int swish) {
+  prad_status st = conv::check("prad_causal_conv_forward", dt, tokens, sequences, offsets, dim, width);
+  if (st) return st;
+  ld_x = conv::pitch(ld_x, dim), ld_y = conv::pitch(ld_y, dim);
+  PRAD_REQUIRE(ld_x >= dim && ld_y >= dim, PRAD_ERR_SHAPE, "prad_causal_conv_forward: a pitch below dim");
+  PRAD_REQUIRE(tokens == 0 || (x && w && y), PRAD_ERR_INVALID, "prad_causal_conv_forward: null pointer");
+  PRAD_REQUIRE(tokens == 0 || y != x, PRAD_ERR_INVALID, "prad_causal_conv_forward: y may not be x");
+  PRAD_REQUIRE(!state_out || state_out != state, PRAD_ERR_INVALID, "prad_causal_conv_forward: state_out may not be the state");
+  PRAD_CHECK_CTX(ctx);
+  return dt == PRAD_F32 ? forward_t<float>(ctx, x, ld_x, w, bias, state, offsets, y, ld_y, state_out, sequences, tokens, dim, width, swish,
+                                           conv::Pass::Forward)
+                        : forward_t<double>(ctx, x, ld_x, w, bias, state, offsets, y, ld_y, state_out, sequences, tokens, dim, width, swish,
+                                            conv::Pass::Forward);
+}
+
+extern "C" prad_status prad_causal_conv_backward(prad_ctx* ctx, prad_dtype dt, const void* x, int64_t ld_x, const void* w, const void* bias,
+                                                 const void* state, const int32_t* offsets, const void* dy, int64_t ld_dy, void* dx,
+                                                 int64_t ld_dx, void* dw, void* dbias, void* dstate, int sequences, int64_t tokens,
+                                                 int dim, int width, int swish) {
+  prad_status st = conv::check("prad_causal_conv_backward", dt, tokens, sequences, offsets, dim, width);
+  if (st) return st;
+  ld_x = conv::pitch(ld_x, dim), ld_dy = conv::pitch(ld_dy, dim), ld_dx = conv::pitch(ld_dx, dim);
+  PRAD_REQUIRE(ld_x >= dim && ld_dy >= dim && ld_dx >= dim, PRAD_ERR_SHAPE, "prad_causal_conv_backward: a pitch below dim");
+  PRAD_REQUIRE(tokens == 0 || (x && w && dy && dx), PRAD_ERR_INVALID, "prad_causal_conv_backward: null pointer");
+  PRAD_REQUIRE(tokens == 0 || (dx != x && dx != dy), PRAD_ERR_INVALID, "prad_causal_conv_backward: dx may not be x or dy");
+  PRAD_CHECK_CTX(ctx);
+  return dt == PRAD_F32 ? backward_t<float>(ctx, x, ld_x, w, bias, state, offsets, dy, ld_dy, dx, ld_dx, dw, dbias, dstate, sequences,
+                                            tokens, dim, width, swish)
+                        : backward_t<double>(ctx, x, ld_x, w, bias, state, offsets, dy, ld_dy, dx, ld_dx, dw, dbias, dstate, sequences,
+                                             tokens, dim, width, swish);
+}
+
+extern "C" prad_status prad_causal_conv_step(prad_ctx* ctx, prad_dtype dt, const void* x, int64_t ld_x, const void* w, const void* bias,
+                                             const void* state, void* y, int64_t ld_y, void* state_out, int64_t batch, int dim, int width,
+                                             int swish) {
+  prad_status st = conv::check("prad_causal_conv_step", dt, batch, 1, nullptr, dim, width);
+  if (st) return st;
+  ld_x = conv::pitch(ld_x, dim), ld_y = conv::pitch(ld_y, dim);
+  PRAD_REQUIRE(ld_x >= dim && ld_y >= dim, PRAD_ERR_SHAPE, "prad_causal_conv_step: a pitch below dim");
+  PRAD_REQUIRE(batch == 0 || (x && w && y && (width == 1 || (state && state_out))), PRAD_ERR_INVALID,
+               "prad_causal_conv_step: null pointer");
+  PRAD_CHECK_CTX(ctx);
+  if (batch == 0) return PRAD_OK;
+  return dt == PRAD_F32 ? forward_t<float>(ctx, x, ld_x, w, bias, state, nullptr, y, ld_y, state_out, 1, batch, dim, width, swish,
+                                           conv::Pass::Step)
+                        : forward_t<double>(ctx, x, ld_x, w, bias, state, nullptr, y, ld_y, state_out, 1, batch, dim, width, swish,
+                                            conv::Pass::Step);
+}

@@ -1,0 +1,656 @@
+// Group normalisation of channels-last data, x[sample][position][channel]: a group is channels / groups neighbouring channels of
+// all positions of a sample,  xhat = (x - mean) rstd,  v = gamma xhat + beta,  y = v or swish(v).  Backward, with dv = dy swish'(v):
+//   dbeta = sum dv,  dgamma = sum dv xhat,  dx = rstd (gamma dv - mean(gamma dv) - xhat mean(gamma dv xhat)).
+//
+// Two shapes of work.  One position per sample (a norm per token): a group's values lie side by side and stay in the registers of
+// a few lanes, one pass over the memory each way.  Several positions: the rows of a sample are cut into blocks, sums of the blocks
+// first, then a pass that reads the values again.
+// Means and variances are summed around a pivot out of the data (the average of the group's first values), so that a mean far
+// from zero takes nothing from the variance; sums go from float to double every few values.
+#include "common.cuh"
+#include "packed_sequences.cuh"
+
+namespace prad {
+namespace gn {
+
+using seq::swish;
+using seq::swish_slope;
+
+constexpr int THREADS = 256;
+
+template <typename T> struct Args {
+  const T *x, *gamma, *beta, *mean, *rstd, *dy;
+  T *y, *mean_out, *rstd_out, *dx, *dgamma, *dbeta;
+  int64_t samples, positions;
+  int channels, groups, per;     // per: channels of a group
+  double eps;
+  int act;
+};
+
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+
+// ---------------------------------------------------------------- one position per sample
+// LW lanes share the values of a (sample, group), E packs of V values each; a lane keeps its channels for all its samples, so the
+// sums for dgamma and dbeta stay in registers as well.  Slot k of the grid takes group k mod groups: neighbouring slots read
+// neighbouring memory.
+template <int LW, typename A> __device__ __forceinline__ A lanes_sum(A v) {
+#pragma unroll
+  for (int o = LW / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, int V, int LW, int E>
+__global__ void __launch_bounds__(THREADS)
+rows_forward_kernel(const Args<T> a, int64_t slots) {
+  const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
+  const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
+  const int64_t step = slots / a.groups;
+  int c[E];
+  bool on[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    c[e] = (l + e * LW) * V;
+    on[e] = c[e] < a.per;
+  }
+  // all lanes of a warp take part in its sums: those beyond the last sample with nothing to add
+  const int64_t first = slot < slots ? slot / a.groups : a.samples;
+  const int64_t rounds = (a.samples + step - 1) / step;
+  for (int64_t k = 0; k < rounds; ++k) {
+    const int64_t s = first + k * step;
+    const bool live = s < a.samples;
+    const T* row = a.x + s * a.channels + (int64_t)g * a.per;
+    Pack<T, V> x[E];
+    T sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[e].v[j] = 0;
+      if (live && on[e]) x[e] = load<T, V>(row + c[e]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += x[e].v[j];
+    }
+    const T mean = lanes_sum<LW>(sum) / (T)a.per;
+    T sq = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const T d = x[e].v[j] - mean;
+        if (on[e]) sq += d * d;
+      }
+    const T var = lanes_sum<LW>(sq) / (T)a.per;
+    const T rstd = (T)(1.0 / sqrt((double)var + a.eps));
+    if (!live) continue;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (on[e]) {
+        const int ch = g * a.per + c[e];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          T v = (x[e].v[j] - mean) * rstd;
+          if (a.gamma) v *= a.gamma[ch + j];
+          if (a.beta) v += a.beta[ch + j];
+          x[e].v[j] = a.act ? swish(v) : v;
+        }
+        *reinterpret_cast<Pack<T, V>*>(a.y + s * a.channels + ch) = x[e];
+      }
+    if (l == 0) {
+      a.mean_out[s * a.groups + g] = mean;
+      a.rstd_out[s * a.groups + g] = rstd;
+    }
+  }
+}
+
+// partial[row block][2][channels]: this slot's sums of dv xhat and of dv
+template <typename T, int V, int LW, int E>
+__global__ void __launch_bounds__(THREADS)
+rows_backward_kernel(const Args<T> a, int64_t slots, T* __restrict__ partial) {
+  const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
+  const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
+  const int64_t step = slots / a.groups;
+  int c[E];
+  bool on[E];
+  Pack<T, V> gamma[E], beta[E], dg[E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    c[e] = (l + e * LW) * V;
+    on[e] = c[e] < a.per;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int ch = g * a.per + c[e] + j;
+      gamma[e].v[j] = on[e] && a.gamma ? a.gamma[ch] : (T)1;
+      beta[e].v[j] = on[e] && a.beta ? a.beta[ch] : (T)0;
+      dg[e].v[j] = db[e].v[j] = 0;
+    }
+  }
+  const int64_t first = slot < slots ? slot / a.groups : a.samples;
+  const int64_t rounds = (a.samples + step - 1) / step;
+  const T inv = (T)1 / (T)a.per;
+  for (int64_t k = 0; k < rounds; ++k) {
+    const int64_t s = first + k * step;
+    const bool live = s < a.samples;
+    const int64_t at = s * a.channels + (int64_t)g * a.per;
+    const T mean = live ? a.mean[s * a.groups + g] : (T)0, rstd = live ? a.rstd[s * a.groups + g] : (T)0;
+    Pack<T, V> x[E], d[E];
+    T s1 = 0, s2 = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (live && on[e]) {
+        x[e] = load<T, V>(a.x + at + c[e]);
+        d[e] = load<T, V>(a.dy + at + c[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (live && on[e]) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const T xh = (x[e].v[j] - mean) * rstd;
+          T dv = d[e].v[j];
+          if (a.act) dv *= swish_slope(xh * gamma[e].v[j] + beta[e].v[j]);
+          dg[e].v[j] += dv * xh;
+          db[e].v[j] += dv;
+          dv *= gamma[e].v[j];
+          s1 += dv;
+          s2 += dv * xh;
+          x[e].v[j] = xh;
+          d[e].v[j] = dv;
+        }
+      }
+    s1 = lanes_sum<LW>(s1) * inv;
+    s2 = lanes_sum<LW>(s2) * inv;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (live && on[e]) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[e].v[j] = rstd * (d[e].v[j] - s1 - x[e].v[j] * s2);
+        *reinterpret_cast<Pack<T, V>*>(a.dx + at + c[e]) = d[e];
+      }
+  }
+  if (slot < slots)
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (on[e])
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          T* to = partial + (slot / a.groups * 2) * a.channels + g * a.per + c[e] + j;
+          to[0] = dg[e].v[j];
+          to[a.channels] = db[e].v[j];
+        }
+}
+
+// out[0][c], out[1][c] = sums over the blocks of partial[block][2][channels], in the order of the blocks within a warp's share
+template <typename P, typename T>
+__global__ void __launch_bounds__(THREADS)
+column_totals_kernel(const P* __restrict__ partial, int64_t blocks, int channels, T* dgamma, T* dbeta) {
+  __shared__ double part[THREADS / 32][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  T* out = blockIdx.y ? dbeta : dgamma;
+  if (!out) return;
+  double sum = 0.0;
+  if (c < channels) {
+    const P* p = partial + (int64_t)blockIdx.y * channels + c;
+#pragma unroll 8
+    for (int64_t b = w; b < blocks; b += THREADS / 32) sum += (double)p[b * 2 * channels];
+  }
+  part[w][lane] = sum;
+  __syncthreads();
+  if (w == 0 && c < channels) {
+    sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < THREADS / 32; ++k) sum += part[k][lane];
+    out[c] = (T)sum;
+  }
+}
+
+// ---------------------------------------------------------------- several positions per sample
+// A CTA takes a block of positions of one sample and a part of the channels: as many whole groups as THREADS packs of V channels
+// hold, the threads in rows of one position each; or one wide group, whose packs the threads walk.
+struct Parts {
+  int64_t blocks, rows;        // blocks of `rows` positions per sample
+  int parts, groups_each;      // of the channels
+};
+template <typename T> struct Place {
+  int64_t s, block, p0, p1;
+  int g0, g1, c0, packs, tx, ty, rows;
+  __device__ __forceinline__ Place(const Args<T>& a, const Parts& k, int V) {
+    s = blockIdx.x / k.blocks;
+    block = blockIdx.x % k.blocks;
+    p0 = block * k.rows;
+    p1 = p0 + k.rows < a.positions ? p0 + k.rows : a.positions;
+    g0 = blockIdx.y * k.groups_each;
+    g1 = g0 + k.groups_each < a.groups ? g0 + k.groups_each : a.groups;
+    c0 = g0 * a.per;
+    packs = (g1 - g0) * a.per / V;
+    const int width = packs < THREADS ? packs : THREADS;
+    tx = threadIdx.x % width;
+    ty = threadIdx.x / width;
+    rows = THREADS / width;
+  }
+};
+
+template <typename T> __device__ __forceinline__ double pivot(const Args<T>& a, int64_t s, int g) {
+  const T* x = a.x + s * a.positions * a.channels + (int64_t)g * a.per;
+  const int across = a.per < 32 ? a.per : 32;
+  const int down = (int)(32 / across < a.positions ? 32 / across : a.positions);
+  double sum = 0.0;
+  for (int p = 0; p < down; ++p)
+    for (int c = 0; c < across; ++c) sum += (double)x[(int64_t)p * a.channels + c];
+  return (double)(T)(sum / (across * down));
+}
+
+constexpr int RUN = 8;     // positions that are summed in T before they go into a double
+
+// sums[sample][block][group][2] = sums of x - pivot and of its square
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
+  __shared__ double part[THREADS][2];
+  __shared__ T piv[THREADS * V + 1];
+  const Place<T> w(a, k, V);
+  for (int g = threadIdx.x; g < w.g1 - w.g0; g += THREADS) piv[g] = (T)pivot(a, w.s, w.g0 + g);
+  __syncthreads();
+  double s1 = 0.0, s2 = 0.0;
+  if (w.ty < w.rows)
+    for (int q = w.tx; q < w.packs; q += THREADS) {
+      const T m = piv[q * V / a.per];
+      const T* x = a.x + (w.s * a.positions) * a.channels + w.c0 + (int64_t)q * V;
+      for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)RUN * w.rows) {
+        T r1 = 0, r2 = 0;
+        Pack<T, V> v[RUN];
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+          const int64_t at = p + (int64_t)i * w.rows;
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[i].v[j] = m;
+          if (at < w.p1) v[i] = load<T, V>(x + at * a.channels);
+        }
+#pragma unroll
+        for (int i = 0; i < RUN; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const T d = v[i].v[j] - m;
+            r1 += d;
+            r2 += d * d;
+          }
+        s1 += (double)r1;
+        s2 += (double)r2;
+      }
+    }
+  part[threadIdx.x][0] = s1;
+  part[threadIdx.x][1] = s2;
+  __syncthreads();
+  // a warp adds up one group: its packs of every row of threads, lanes in a fixed order
+  const int lane = threadIdx.x & 31, width = w.packs < THREADS ? w.packs : THREADS;
+  const int each = w.g1 - w.g0 == 1 ? width : a.per / V;       // threads of a group in one row of threads
+  for (int g = threadIdx.x >> 5; g < w.g1 - w.g0; g += THREADS / 32) {
+    s1 = s2 = 0.0;
+    for (int i = lane; i < each * w.rows; i += 32) {
+      const int t = i / each * width + g * each + i % each;
+      s1 += part[t][0];
+      s2 += part[t][1];
+    }
+    s1 = lanes_sum<32>(s1);
+    s2 = lanes_sum<32>(s2);
+    if (lane == 0) {
+      double* to = sums + ((w.s * k.blocks + w.block) * a.groups + w.g0 + g) * 2;
+      to[0] = s1;
+      to[1] = s2;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+statistics_kernel(const Args<T> a, int64_t blocks, const double* __restrict__ sums) {
+  const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+  if (i >= a.samples * a.groups) return;
+  const int64_t s = i / a.groups;
+  const int g = (int)(i % a.groups);
+  double s1 = 0.0, s2 = 0.0;
+#pragma unroll 8
+  for (int64_t b = 0; b < blocks; ++b) {
+    const double* p = sums + ((s * blocks + b) * a.groups + g) * 2;
+    s1 += p[0];
+    s2 += p[1];
+  }
+  const double n = (double)a.positions * a.per, m = s1 / n;
+  double var = s2 / n - m * m;
+  if (var < 0.0) var = 0.0;        // (a NaN stays)
+  a.mean_out[i] = (T)(pivot(a, s, g) + m);
+  a.rstd_out[i] = (T)(1.0 / sqrt(var + a.eps));
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+apply_kernel(const Args<T> a, const Parts k) {
+  const Place<T> w(a, k, V);
+  if (w.ty >= w.rows) return;
+  for (int q = w.tx; q < w.packs; q += THREADS) {
+    const int c = w.c0 + q * V;
+    const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
+    const T mean = a.mean[i], rstd = a.rstd[i];
+    T gamma[V], beta[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
+      beta[j] = a.beta ? a.beta[c + j] : (T)0;
+    }
+    for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
+      Pack<T, V> v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (p + (int64_t)r * w.rows < w.p1) v[r] = load<T, V>(a.x + at + (p + (int64_t)r * w.rows) * a.channels);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (p + (int64_t)r * w.rows < w.p1) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const T t = (v[r].v[j] - mean) * rstd * gamma[j] + beta[j];
+            v[r].v[j] = a.act ? swish(t) : t;
+          }
+          *reinterpret_cast<Pack<T, V>*>(a.y + at + (p + (int64_t)r * w.rows) * a.channels) = v[r];
+        }
+    }
+  }
+}
+
+// sums[sample][block][2][channels] = sums of dv xhat and of dv over the block
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+block_gradients_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
+  __shared__ double part[2][THREADS * V];
+  const Place<T> w(a, k, V);
+  const int width = w.packs < THREADS ? w.packs : THREADS;
+  for (int q0 = 0; q0 < w.packs; q0 += THREADS) {
+    const int q = q0 + w.tx;
+    const bool on = w.ty < w.rows && q < w.packs;
+    double sg[V], sb[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sg[j] = sb[j] = 0.0;
+    if (on) {
+      const int c = w.c0 + q * V;
+      const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
+      const T mean = a.mean[i], rstd = a.rstd[i];
+      T gamma[V], beta[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
+        beta[j] = a.beta ? a.beta[c + j] : (T)0;
+      }
+      for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
+        Pack<T, V> x[4], d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (p + (int64_t)r * w.rows < w.p1) {
+            x[r] = load<T, V>(a.x + at + (p + (int64_t)r * w.rows) * a.channels);
+            d[r] = load<T, V>(a.dy + at + (p + (int64_t)r * w.rows) * a.channels);
+          }
+        T rg[V], rb[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) rg[j] = rb[j] = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (p + (int64_t)r * w.rows < w.p1) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const T xh = (x[r].v[j] - mean) * rstd;
+              T dv = d[r].v[j];
+              if (a.act) dv *= swish_slope(xh * gamma[j] + beta[j]);
+              rg[j] += dv * xh;
+              rb[j] += dv;
+            }
+          }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          sg[j] += (double)rg[j];
+          sb[j] += (double)rb[j];
+        }
+      }
+    }
+    __syncthreads();
+    if (on)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        part[0][(w.ty * width + w.tx) * V + j] = sg[j];
+        part[1][(w.ty * width + w.tx) * V + j] = sb[j];
+      }
+    __syncthreads();
+    const int here = (w.packs - q0 < THREADS ? w.packs - q0 : THREADS) * V;
+    for (int e = threadIdx.x; e < 2 * here; e += THREADS) {
+      const int c = e % here;
+      double sum = 0.0;
+      for (int r = 0; r < w.rows; ++r) sum += part[e / here][r * width * V + c];
+      sums[((w.s * k.blocks + w.block) * 2 + e / here) * a.channels + w.c0 + q0 * V + c] = sum;
+    }
+  }
+}
+
+// Per sample and group: mean(gamma dv) and mean(gamma dv xhat) of the whole sample; a warp each.
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+group_gradients_kernel(const Args<T> a, int64_t blocks, const double* __restrict__ sums, double* __restrict__ means) {
+  const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (i >= a.samples * a.groups) return;
+  const int64_t s = i / a.groups;
+  const int c0 = (int)(i % a.groups) * a.per;
+  double s1 = 0.0, s2 = 0.0;
+  for (int64_t e = lane; e < blocks * a.per; e += 32) {
+    const int c = c0 + (int)(e % a.per);
+    const double* p = sums + (s * blocks + e / a.per) * 2 * a.channels + c;
+    const double gamma = a.gamma ? (double)a.gamma[c] : 1.0;
+    s2 += gamma * p[0];
+    s1 += gamma * p[a.channels];
+  }
+  s1 = lanes_sum<32>(s1);
+  s2 = lanes_sum<32>(s2);
+  const double n = (double)a.positions * a.per;
+  if (lane == 0) {
+    means[i * 2] = s1 / n;
+    means[i * 2 + 1] = s2 / n;
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+input_gradients_kernel(const Args<T> a, const Parts k, const double* __restrict__ means) {
+  const Place<T> w(a, k, V);
+  if (w.ty >= w.rows) return;
+  for (int q = w.tx; q < w.packs; q += THREADS) {
+    const int c = w.c0 + q * V;
+    const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
+    const T mean = a.mean[i], rstd = a.rstd[i], s1 = (T)means[i * 2], s2 = (T)means[i * 2 + 1];
+    T gamma[V], beta[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
+      beta[j] = a.beta ? a.beta[c + j] : (T)0;
+    }
+    for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
+      Pack<T, V> x[4], d[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (p + (int64_t)r * w.rows < w.p1) {
+          x[r] = load<T, V>(a.x + at + (p + (int64_t)r * w.rows) * a.channels);
+          d[r] = load<T, V>(a.dy + at + (p + (int64_t)r * w.rows) * a.channels);
+        }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (p + (int64_t)r * w.rows < w.p1) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const T xh = (x[r].v[j] - mean) * rstd;
+            T dv = d[r].v[j];
+            if (a.act) dv *= swish_slope(xh * gamma[j] + beta[j]);
+            d[r].v[j] = rstd * (dv * gamma[j] - s1 - xh * s2);
+          }
+          *reinterpret_cast<Pack<T, V>*>(a.dx + at + (p + (int64_t)r * w.rows) * a.channels) = d[r];
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launches
+template <typename T, int V> constexpr int most_in_registers() { return 32 * 8 * V; }
+
+template <typename T, int V, int LW, int E> static prad_status rows(prad_ctx* ctx, const Args<T>& a, bool backward) {
+  // as many slots as fill the device, and a whole number of them per group
+  const int64_t fill = (int64_t)ctx->sm_count * (2048 / 2) / LW;
+  int64_t per_group = fill / a.groups;
+  if (per_group < 1) per_group = 1;
+  if (per_group > a.samples) per_group = a.samples;
+  const int64_t slots = per_group * a.groups;
+  const int64_t grid = ceil_div(slots * LW, THREADS);
+  PRAD_REQUIRE(grid <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "group norm: too many groups");
+  if (!backward) {
+    rows_forward_kernel<T, V, LW, E><<<(unsigned)grid, THREADS, 0, ctx->stream>>>(a, slots);
+    PRAD_LAUNCHED(ctx);
+    return PRAD_OK;
+  }
+  prad_status st = ensure_workspace(ctx, (size_t)per_group * 2 * a.channels * sizeof(T));
+  if (st) return st;
+  rows_backward_kernel<T, V, LW, E><<<(unsigned)grid, THREADS, 0, ctx->stream>>>(a, slots, (T*)ctx->ws);
+  PRAD_LAUNCHED(ctx);
+  if (a.dgamma || a.dbeta) {
+    column_totals_kernel<T, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), THREADS, 0, ctx->stream>>>((const T*)ctx->ws, per_group,
+                                                                                                      a.channels, a.dgamma, a.dbeta);
+    PRAD_LAUNCHED(ctx);
+  }
+  return PRAD_OK;
+}
+template <typename T, int V> static prad_status pick_rows(prad_ctx* ctx, const Args<T>& a, bool backward) {
+  const int packs = a.per / V;
+  if (packs <= 4) return rows<T, V, 4, 1>(ctx, a, backward);
+  if (packs <= 8) return rows<T, V, 8, 1>(ctx, a, backward);
+  if (packs <= 16) return rows<T, V, 16, 1>(ctx, a, backward);
+  if (packs <= 32) return rows<T, V, 32, 1>(ctx, a, backward);
+  if (packs <= 64) return rows<T, V, 32, 2>(ctx, a, backward);
+  if (packs <= 128) return rows<T, V, 32, 4>(ctx, a, backward);
+  return rows<T, V, 32, 8>(ctx, a, backward);
+}
+
+template <typename T, int V> static prad_status blocks(prad_ctx* ctx, Args<T> a, bool backward) {
+  Parts k;
+  k.groups_each = THREADS * V / a.per;
+  if (k.groups_each < 1) k.groups_each = 1;
+  if (k.groups_each > a.groups) k.groups_each = a.groups;
+  k.parts = (int)ceil_div(a.groups, k.groups_each);
+  // eight CTAs an SM; a block has at least 16 values a thread
+  const int64_t want = ceil_div((int64_t)ctx->sm_count * 8, a.samples * k.parts);
+  const int64_t row_values = (int64_t)k.groups_each * a.per;
+  const int64_t least = ceil_div((int64_t)THREADS * 16, row_values);
+  k.rows = ceil_div(a.positions, want);
+  if (k.rows < least) k.rows = least;
+  if (k.rows > a.positions) k.rows = a.positions;
+  k.blocks = ceil_div(a.positions, k.rows);
+  PRAD_REQUIRE(a.samples * k.blocks <= 0x7fffffff && k.parts <= 65535, PRAD_ERR_UNSUPPORTED, "group norm: too many samples or channels");
+  const dim3 grid((unsigned)(a.samples * k.blocks), (unsigned)k.parts);
+  const int64_t each = a.samples * a.groups;
+  PRAD_REQUIRE(ceil_div(each * 32, THREADS) <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "group norm: too many groups");
+  if (!backward) {
+    prad_status st = ensure_workspace(ctx, (size_t)(a.samples * k.blocks * a.groups) * 2 * sizeof(double));
+    if (st) return st;
+    block_sums_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k, (double*)ctx->ws);
+    PRAD_LAUNCHED(ctx);
+    statistics_kernel<T><<<(unsigned)ceil_div(each, THREADS), THREADS, 0, ctx->stream>>>(a, k.blocks, (const double*)ctx->ws);
+    PRAD_LAUNCHED(ctx);
+    a.mean = a.mean_out;
+    a.rstd = a.rstd_out;
+    apply_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k);
+    PRAD_LAUNCHED(ctx);
+    return PRAD_OK;
+  }
+  const size_t columns = (size_t)(a.samples * k.blocks) * 2 * a.channels;
+  prad_status st = ensure_workspace(ctx, (columns + (size_t)each * 2) * sizeof(double));
+  if (st) return st;
+  double *sums = (double*)ctx->ws, *means = sums + columns;
+  block_gradients_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k, sums);
+  PRAD_LAUNCHED(ctx);
+  group_gradients_kernel<T><<<(unsigned)ceil_div(each * 32, THREADS), THREADS, 0, ctx->stream>>>(a, k.blocks, sums, means);
+  PRAD_LAUNCHED(ctx);
+  input_gradients_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k, means);
+  PRAD_LAUNCHED(ctx);
+  if (a.dgamma || a.dbeta) {
+    column_totals_kernel<double, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), THREADS, 0, ctx->stream>>>(
+        sums, a.samples * k.blocks, a.channels, a.dgamma, a.dbeta);
+    PRAD_LAUNCHED(ctx);
+  }
+  return PRAD_OK;
+}
+
+template <typename T> static prad_status run(prad_ctx* ctx, const Args<T>& a, bool backward) {
+  constexpr int V = 16 / sizeof(T);
+  const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.y | (uintptr_t)a.dx;
+  const bool vector = a.per % V == 0 && (all & 15) == 0;
+  if (a.positions == 1 && a.per <= (vector ? most_in_registers<T, V>() : most_in_registers<T, 1>()))
+    return vector ? pick_rows<T, V>(ctx, a, backward) : pick_rows<T, 1>(ctx, a, backward);
+  return vector ? blocks<T, V>(ctx, a, backward) : blocks<T, 1>(ctx, a, backward);
+}
+
+static prad_status check(const char* who, prad_dtype dt, int64_t samples, int64_t positions, int channels, int groups) {
+  PRAD_REQUIRE(dtype_ok(dt), PRAD_ERR_INVALID, "%s: unknown dtype %d", who, (int)dt);
+  PRAD_REQUIRE(samples >= 0 && positions >= 0 && channels > 0 && groups > 0, PRAD_ERR_SHAPE, "%s: bad shape", who);
+  PRAD_REQUIRE(channels % groups == 0, PRAD_ERR_SHAPE, "%s: %d channels do not divide into %d groups", who, channels, groups);
+  return PRAD_OK;
+}
+
+}  // namespace gn
+}  // namespace prad
+
+using namespace prad;
+
+template <typename T>
+static prad_status forward_t(prad_ctx* ctx, const void* x, const void* gamma, const void* beta, void* y, void* mean, void* rstd,
+                             int64_t samples, int64_t positions, int channels, int groups, double eps, int act) {
+  gn::Args<T> a = {};
+  a.x = (const T*)x, a.gamma = (const T*)gamma, a.beta = (const T*)beta;
+  a.y = (T*)y, a.mean_out = (T*)mean, a.rstd_out = (T*)rstd;
+  a.samples = samples, a.positions = positions, a.channels = channels, a.groups = groups, a.per = channels / groups;
+  a.eps = eps, a.act = act;
+  return gn::run(ctx, a, false);
+}
+template <typename T>
+static prad_status backward_t(prad_ctx* ctx, const void* x, const void* gamma, const void* beta, const void* mean, const void* rstd,
+                              const void* dy, void* dx, void* dgamma, void* dbeta, int64_t samples, int64_t positions, int channels,
+                              int groups, int act) {
+  gn::Args<T> a = {};
+  a.x = (const T*)x, a.gamma = (const T*)gamma, a.beta = (const T*)beta, a.mean = (const T*)mean, a.rstd = (const T*)rstd;
+  a.dy = (const T*)dy, a.dx = (T*)dx, a.dgamma = (T*)dgamma, a.dbeta = (T*)dbeta;
+  a.samples = samples, a.positions = positions, a.channels = channels, a.groups = groups, a.per = channels / groups;
+  a.act = act;
+  return gn::run(ctx, a, true);
+}
+
+extern "C" prad_status prad_group_norm_forward(prad_ctx* ctx, prad_dtype dt, const void* x, const void* gamma, const void* beta, void* y,
+                                               void* mean, void* rstd, int64_t samples, int64_t positions, int channels, int groups,
+                                               double eps, int swish) {
+  prad_status st = gn::check("prad_group_norm_forward", dt, samples, positions, channels, groups);
+  if (st) return st;
+  PRAD_REQUIRE(eps >= 0.0, PRAD_ERR_INVALID, "prad_group_norm_forward: eps must not be negative");
+  PRAD_REQUIRE(samples == 0 || positions == 0 || (x && y && mean && rstd), PRAD_ERR_INVALID, "prad_group_norm_forward: null pointer");
+  PRAD_CHECK_CTX(ctx);
+  if (samples == 0 || positions == 0) return PRAD_OK;
+  return dt == PRAD_F32 ? forward_t<float>(ctx, x, gamma, beta, y, mean, rstd, samples, positions, channels, groups, eps, swish)
+                        : forward_t<double>(ctx, x, gamma, beta, y, mean, rstd, samples, positions, channels, groups, eps, swish);
+}
+
+extern "C" prad_status prad_group_norm_backward(prad_ctx* ctx, prad_dtype dt, const void* x, const void* gamma, const void* beta,
+                                                const void* mean, const void* rstd, const void* dy, void* dx, void* dgamma, void* dbeta,
+                                                int64_t samples, int64_t positions, int channels, int groups, int swish) {
+  prad_status st = gn::check("prad_group_norm_backward", dt, samples, positions, channels, groups);
+  if (st) return st;
+  PRAD_REQUIRE(samples == 0 || positions == 0 || (x && mean && rstd && dy && dx), PRAD_ERR_INVALID,
+               "prad_group_norm_backward: null pointer");
+  PRAD_CHECK_CTX(ctx);
+  if (samples == 0 || positions == 0) {      // nothing was normalised: the parameters' gradients are zero
+    if (dgamma) PRAD_CUDA(cudaMemsetAsync(dgamma, 0, channels * dtype_size(dt), ctx->stream));
+    if (dbeta) PRAD_CUDA(cudaMemsetAsync(dbeta, 0, channels * dtype_size(dt), ctx->stream));
+    return PRAD_OK;
+  }
+  return dt == PRAD_F32
+             ? backward_t<float>(ctx, x, gamma, beta, mean, rstd, dy, dx, dgamma, dbeta, samples, positions, channels, groups, swish)
+             : backward_t<double>(ctx, x, gamma, beta, mean, rstd, dy, dx, dgamma, dbeta, samples, positions, channels, groups, swish);
+}

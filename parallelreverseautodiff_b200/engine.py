@@ -34,6 +34,15 @@ def dtype_code(dtype) -> int:
         raise TypeError(f"only float32 (PRADLite) and float64 (PRAD) are supported, got {dtype}")
 
 
+_byref, _size_t = C.byref, C.c_size_t      # (C is also the name of a scan's matrix)
+
+
+def _divided(n: int, by: int, what: str, parts: str) -> int:
+    if by < 1 or n % by:
+        raise _lib.PradError(_lib.ERR_SHAPE, f"{n} {what} do not divide into {by} {parts}")
+    return n // by
+
+
 class DeviceMatrix:
     """A dense row-major device buffer: Matrix (2-D) or DeepMatrix (3-D, depth first)."""
 
@@ -827,6 +836,135 @@ class Engine:
         check(self.lib.prad_rmsnorm_backward(self.ctx, dtype_code(x.dtype), x.ptr, g.ptr, dy.ptr, dx.ptr, dg.ptr,
                                              x.shape[0], x.shape[1]))
         return dx, dg
+
+    # ------------------------------------------------------------ state space layers
+    def _upload_raw(self, a: np.ndarray) -> DeviceMatrix:
+        """Device copy of an array of any type: row numbers and counters, which are no matrices of the library."""
+        p = C.c_void_p()
+        check(self.lib.prad_alloc(self.ctx, a.nbytes, C.byref(p)))
+        m = DeviceMatrix(self, p.value, a.shape, a.dtype)
+        check(self.lib.prad_upload(self.ctx, m.ptr, a.ctypes.data, a.nbytes))
+        return m
+
+    def sequence_offsets(self, lengths) -> DeviceMatrix:
+        """`offsets` of packed sequences with these many tokens each (int32 on the device, one more than sequences)."""
+        marks = np.concatenate([[0], np.cumsum(np.asarray(lengths, np.int64).reshape(-1))])
+        if (np.diff(marks) < 0).any() or marks[-1] > 0x7FFFFFFF:
+            raise ValueError("lengths must not be negative and add up to less than 2^31")
+        return self._upload_raw(marks.astype(np.int32))
+
+    def dropout_step(self, value: int = 0) -> DeviceMatrix:
+        """A `step` for dropout(): a uint64 on the device, counted on with upload() between replays of a recorded sequence."""
+        return self._upload_raw(np.array([value], np.uint64))
+
+    def dropout(self, x, p, seed, offset=0, residual=None, step=None, out=None):
+        """x / (1 - p) where the generator keeps it, else 0, plus the residual; on dy with the same seed and offset it is the
+        Backward (prad_dropout)."""
+        out = out or self.empty(x.shape, x.dtype)
+        check(self.lib.prad_dropout(self.ctx, dtype_code(x.dtype), x.ptr, self._p(residual), out.ptr, x.size, p, seed, offset,
+                                    self._p(step)))
+        return out
+
+    def group_norm_forward(self, x, groups, gamma=None, beta=None, positions=1, eps=1e-5, swish=False, out=None):
+        """Group norm of [samples * positions x channels], channels last (prad_group_norm_forward).  Returns (y, mean, rstd)."""
+        rows, channels = x.size // x.shape[-1], x.shape[-1]
+        samples = _divided(rows, positions, "rows", "positions")
+        y, mean, rstd = out or (self.empty(x.shape, x.dtype), self.empty((samples, groups), x.dtype),
+                                self.empty((samples, groups), x.dtype))
+        check(self.lib.prad_group_norm_forward(self.ctx, dtype_code(x.dtype), x.ptr, self._p(gamma), self._p(beta), y.ptr, mean.ptr,
+                                               rstd.ptr, samples, positions, channels, groups, eps, int(swish)))
+        return y, mean, rstd
+
+    def group_norm_backward(self, x, mean, rstd, dy, groups, gamma=None, beta=None, positions=1, swish=False, out=None):
+        """Returns (dx, dgamma, dbeta)."""
+        rows, channels = x.size // x.shape[-1], x.shape[-1]
+        samples = _divided(rows, positions, "rows", "positions")
+        dx, dgamma, dbeta = out or (self.empty(x.shape, x.dtype), self.empty((channels,), x.dtype), self.empty((channels,), x.dtype))
+        check(self.lib.prad_group_norm_backward(self.ctx, dtype_code(x.dtype), x.ptr, self._p(gamma), self._p(beta), mean.ptr, rstd.ptr,
+                                                dy.ptr, dx.ptr, self._p(dgamma), self._p(dbeta), samples, positions, channels, groups,
+                                                int(swish)))
+        return dx, dgamma, dbeta
+
+    def causal_conv_forward(self, x, w, bias=None, state=None, offsets=None, sequences=1, swish=True, out=None, state_out=None,
+                            ld_x=0, ld_y=0):
+        """Causal convolution per channel over packed sequences (prad_causal_conv_forward); w is [dim x width].  `state_out`: a
+        matrix, or True for a new one, to take the state behind each sequence.  Returns (y, state_out)."""
+        (tokens, dim), width = x.shape, w.shape[1]
+        out = out or self.empty((tokens, dim), x.dtype)
+        if state_out is True:
+            state_out = self.empty((sequences, (width - 1) * dim), x.dtype)
+        check(self.lib.prad_causal_conv_forward(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), self._p(state),
+                                                self._p(offsets), out.ptr, ld_y, self._p(state_out), sequences, tokens, dim, width,
+                                                int(swish)))
+        return out, state_out
+
+    def causal_conv_backward(self, x, w, dy, bias=None, state=None, offsets=None, sequences=1, swish=True, out=None, ld_x=0, ld_dy=0,
+                             ld_dx=0):
+        """Gradients by name: x, w, and bias and state where there are any."""
+        (tokens, dim), width = x.shape, w.shape[1]
+        if out is None:
+            out = {k: self.empty(m.shape, x.dtype) for k, m in (("x", x), ("w", w), ("bias", bias), ("state", state)) if m is not None}
+        check(self.lib.prad_causal_conv_backward(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), self._p(state),
+                                                 self._p(offsets), dy.ptr, ld_dy, out["x"].ptr, ld_dx, self._p(out.get("w")),
+                                                 self._p(out.get("bias")), self._p(out.get("state")), sequences, tokens, dim, width,
+                                                 int(swish)))
+        return out
+
+    def causal_conv_step(self, x, w, state, bias=None, swish=True, out=None, state_out=None, ld_x=0, ld_y=0):
+        """One new row of each sequence; the state is replaced, or goes to `state_out`.  Returns y."""
+        (batch, dim), width = x.shape, w.shape[1]
+        out = out or self.empty((batch, dim), x.dtype)
+        check(self.lib.prad_causal_conv_step(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), state.ptr, out.ptr, ld_y,
+                                             state.ptr if state_out is None else state_out.ptr, batch, dim, width, int(swish)))
+        return out
+
+    @staticmethod
+    def _scan(u, delta, A, B, C_, D, z, delta_bias, h0, offsets, sequences, groups, delta_softplus, pitches):
+        dim, state = A.shape
+        s = _lib.Scan(u.shape[0], sequences, dim, state, groups, int(delta_softplus), *[None if m is None else m.ptr for m in (
+            offsets, u, delta, z, A, B, C_, D, delta_bias, h0)])
+        for k, ld in (pitches or {}).items():
+            setattr(s, "ld_" + k, ld)
+        return s
+
+    def selective_scan_forward(self, u, delta, A, B, C, D=None, z=None, delta_bias=None, h0=None, offsets=None, sequences=1, groups=1,
+                               delta_softplus=True, out=None, h_last=None, save=False, pitches=None, ld_y=0):
+        """Selective scan over packed sequences (prad_selective_scan_forward).  `h_last`: a matrix, or True for a new one, to take
+        the final states; `save`: keep what the backward needs (or a matrix to keep it in); `pitches`: of u, delta, z, B or C by
+        name, where they are columns of wider matrices.  Returns (y, h_last, saved)."""
+        s = self._scan(u, delta, A, B, C, D, z, delta_bias, h0, offsets, sequences, groups, delta_softplus, pitches)
+        dt, ref = dtype_code(u.dtype), _byref(s)
+        out = out or self.empty(u.shape, u.dtype)
+        if h_last is True:
+            h_last = self.empty((sequences, s.dim * s.state), u.dtype)
+        if save is True:
+            n = _size_t()
+            check(self.lib.prad_selective_scan_saved_bytes(dt, ref, _byref(n)))
+            save = self.empty((max(1, n.value // u.dtype.itemsize),), u.dtype)
+        save = save or None
+        check(self.lib.prad_selective_scan_forward(self.ctx, dt, ref, out.ptr, ld_y, self._p(h_last), self._p(save)))
+        return out, h_last, save
+
+    def selective_scan_backward(self, u, delta, A, B, C, saved, dy, D=None, z=None, delta_bias=None, h0=None, offsets=None, sequences=1,
+                                groups=1, delta_softplus=True, out=None, pitches=None, ld_dy=0, gradient_pitches=None):
+        """Gradients by the names of the arguments; `out` gives the matrices to write (u, delta, A, B and C, z with a z)."""
+        s = self._scan(u, delta, A, B, C, D, z, delta_bias, h0, offsets, sequences, groups, delta_softplus, pitches)
+        if out is None:
+            out = {k: self.empty(m.shape, u.dtype) for k, m in (("u", u), ("delta", delta), ("z", z), ("A", A), ("B", B), ("C", C),
+                                                                ("D", D), ("delta_bias", delta_bias), ("h0", h0)) if m is not None}
+        g = _lib.ScanGradients(*[self._p(out.get(k)) for k in ("u", "delta", "z", "A", "B", "C", "D", "delta_bias", "h0")])
+        for k, ld in (gradient_pitches or {}).items():
+            setattr(g, "ld_d" + k, ld)
+        check(self.lib.prad_selective_scan_backward(self.ctx, dtype_code(u.dtype), _byref(s), self._p(saved), dy.ptr, ld_dy, _byref(g)))
+        return out
+
+    def selective_scan_step(self, u, delta, A, B, C, h, D=None, z=None, delta_bias=None, groups=1, delta_softplus=True, out=None,
+                            h_out=None, pitches=None, ld_y=0):
+        """One new token for each sequence; the states `h` are replaced, or go to `h_out`.  Returns y."""
+        s = self._scan(u, delta, A, B, C, D, z, delta_bias, h, None, u.shape[0], groups, delta_softplus, pitches)
+        out = out or self.empty(u.shape, u.dtype)
+        check(self.lib.prad_selective_scan_step(self.ctx, dtype_code(u.dtype), _byref(s), out.ptr, ld_y, (h_out or h).ptr))
+        return out
 
     # ------------------------------------------------------------ losses
     def _loss_fwd(self, fn, out, target):
