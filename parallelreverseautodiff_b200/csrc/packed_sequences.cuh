@@ -34,7 +34,18 @@ struct Sequences {
   }
 };
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
+// 1 / (1 + 2^(-x log2 e)): two steps of the special function unit, each within 2 units of the last place
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid(float x) { return reciprocal(1.0f + exp2_approx(x * -1.4426950408889634f)); }
 __device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
 template <typename T> __device__ __forceinline__ T swish(T x) { return x * sigmoid(x); }
 // d swish / dx

@@ -25,14 +25,15 @@ using seq::swish;
 using seq::swish_slope;
 
 constexpr int THREADS = 128;
-template <typename T> constexpr int tile() { return sizeof(T) == 8 ? 16 : 32; }     // TT; also tokens per checkpoint
+template <typename T> constexpr int tile() { return sizeof(T) == 8 ? 16 : 32; }     // TT of the passes without a history
+constexpr int POINT = 16;        // tokens per checkpoint, and TT of the main backward pass
 constexpr int MAX_STATE = 128;
 
 template <typename T> struct Args {
   Sequences rows;
   int64_t span;                 // tokens of a span
   int spans, dim, state, groups, per, blocks;   // per: channels of a group, in `blocks` CTAs
-  int softplus;
+  int softplus, wide_B, wide_C;      // rows of B, C that can be copied 16 bytes at a time
   int64_t ld_u, ld_delta, ld_z, ld_B, ld_C, ld_y, ld_dy, ld_du, ld_ddelta, ld_dz, ld_dB, ld_dC;
   const T *u, *delta, *z, *A, *B, *C, *D, *bias, *h0, *dy;
   T *y, *h_last, *saved;
@@ -45,11 +46,7 @@ template <typename T> struct Args {
 };
 
 // exp(dt A): in float as 2^(dt A') with A' = A log2 e
-__device__ __forceinline__ float decay(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+__device__ __forceinline__ float decay(float x) { return seq::exp2_approx(x); }
 __device__ __forceinline__ double decay(double x) { return exp(x); }
 template <typename T> __device__ __forceinline__ T rate(T a);
 template <> __device__ __forceinline__ float rate(float a) { return a * 1.4426950408889634f; }
@@ -58,12 +55,91 @@ template <typename T> __device__ __forceinline__ T per_rate();         // A per 
 template <> __device__ __forceinline__ float per_rate<float>() { return 0.6931471805599453f; }
 template <> __device__ __forceinline__ double per_rate<double>() { return 1.0; }
 
-__device__ __forceinline__ float log1p_(float x) { return log1pf(x); }
-__device__ __forceinline__ double log1p_(double x) { return log1p(x); }
-__device__ __forceinline__ float exp_(float x) { return expf(x); }
-__device__ __forceinline__ double exp_(double x) { return exp(x); }
-template <typename T> __device__ __forceinline__ T softplus(T x) {
-  return (x > (T)0 ? x : (T)0) + log1p_(exp_(x > (T)0 ? -x : x));
+// log(1 + e^x) = max(x, 0) + log(1 + w) with w = e^-|x|.  In float log(1 + w) = 2 atanh(r), r = w / (2 + w) <= 1/3, by a polynomial
+// in r^2: the Chebyshev interpolation of atanh(r) / r over r^2 <= 1/9, off by 4e-9 of the value; this keeps the small time steps
+// of very negative x to their last bits, at a third of the instructions of log1p and exp.
+__device__ __forceinline__ float softplus(float x) {
+  const float w = seq::exp2_approx(fabsf(x) * -1.4426950408889634f), r = w * seq::reciprocal(w + 2.0f), q = r * r;
+  float p = 0.140788892f;
+  p = fmaf(p, q, 0.139825789f);
+  p = fmaf(p, q, 0.200122976f);
+  p = fmaf(p, q, 0.333331608f);
+  p = fmaf(p, q, 1.0f);
+  return fmaf(r + r, p, fmaxf(x, 0.0f));
+}
+__device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+
+// two values side by side: float works on both with one instruction
+template <typename T> struct Two;
+template <> struct Two<float> {
+  unsigned long long v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+template <> struct Two<double> {
+  double a_, b_;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(double a, double b) : a_(a), b_(b) {}
+  __device__ __forceinline__ void get(double& a, double& b) const { a = a_, b = b_; }
+};
+__device__ __forceinline__ Two<float> mul(Two<float> a, Two<float> b) {
+  Two<float> r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) {
+  Two<float> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two<double> mul(Two<double> a, Two<double> b) { return {a.a_ * b.a_, a.b_ * b.b_}; }
+__device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) {
+  return {::fma(a.a_, b.a_, c.a_), ::fma(a.b_, b.b_, c.b_)};
+}
+template <typename T> __device__ __forceinline__ Two<T> decay(Two<T> x) {
+  T a, b;
+  x.get(a, b);
+  return {decay(a), decay(b)};
+}
+template <typename T> __device__ __forceinline__ T total(Two<T> x) {
+  T a, b;
+  x.get(a, b);
+  return a + b;
+}
+// S values of shared memory (16-byte aligned for float) as pairs
+template <int P> __device__ __forceinline__ void read(const float* m, Two<float> (&v)[P]) {
+  if constexpr (P == 2) {
+    const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(m);
+    v[0].v = q.x;
+    v[1].v = q.y;
+  } else {
+    v[0].v = *reinterpret_cast<const unsigned long long*>(m);
+  }
+}
+template <int P> __device__ __forceinline__ void read(const double* m, Two<double> (&v)[P]) {
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const double2 q = *reinterpret_cast<const double2*>(m + 2 * j);
+    v[j] = {q.x, q.y};
+  }
+}
+// a token's time step and dt u of a channel, each twice in float
+struct alignas(16) StepF { float dt, dt_, x, x_; };
+struct alignas(16) StepD { double dt, x; };
+template <typename T> struct StepOf { using type = StepF; };
+template <> struct StepOf<double> { using type = StepD; };
+__device__ __forceinline__ void write(StepF* m, float dt, float x) { *reinterpret_cast<float4*>(m) = make_float4(dt, dt, x, x); }
+__device__ __forceinline__ void write(StepD* m, double dt, double x) { *reinterpret_cast<double2*>(m) = make_double2(dt, x); }
+__device__ __forceinline__ void read(const StepF* m, Two<float>& dt, Two<float>& x) {
+  const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(m);
+  dt.v = q.x;
+  x.v = q.y;
+}
+__device__ __forceinline__ void read(const StepD* m, Two<double>& dt, Two<double>& x) {
+  const double2 q = *reinterpret_cast<const double2*>(m);
+  dt = {q.x, q.x};
+  x = {q.y, q.y};
 }
 
 template <typename T, int S> struct alignas(sizeof(T) * S) Pack { T v[S]; };
@@ -120,18 +196,31 @@ template <int TT> __device__ __forceinline__ uint32_t starts_in(const Sequences&
   return mask;
 }
 
-// B and C rows of a tile, by asynchronous copies
+// B or C rows of a tile, by asynchronous copies; rows without a token are zero
 template <typename T, int N, int TT>
-__device__ __forceinline__ void fetch_rows(T (*to)[N], const T* from, int64_t ld, int first, int state, int64_t tile0, int64_t begin,
-                                           int64_t finish) {
+__device__ __forceinline__ void fetch_rows(T (*to)[N], const T* from, int64_t ld, int first, int state, int wide, int64_t tile0, int begin,
+                                           int finish) {
+  constexpr int V = 16 / sizeof(T);
+  from += tile0 * ld + first;
+  if (wide && N % V == 0) {
 #pragma unroll
-  for (int i = 0; i < (TT * N + THREADS - 1) / THREADS; ++i) {
-    const int e = threadIdx.x + i * THREADS, t = e / N, n = e % N;
-    if (TT * N % THREADS != 0 && e >= TT * N) break;
-    const bool live = tile0 + t >= begin && tile0 + t < finish && n < state;
+    for (int i = 0; i < (TT * N / V + THREADS - 1) / THREADS; ++i) {
+      const int e = threadIdx.x + i * THREADS, t = e / (N / V), n = e % (N / V) * V;
+      if (TT * N / V % THREADS != 0 && e >= TT * N / V) break;
+      const bool live = t >= begin && t < finish && n < state;
+      const uint32_t d = (uint32_t)__cvta_generic_to_shared(&to[t][n]);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from + (live ? t * ld + n : begin * ld)), "r"(live ? 16 : 0)
+                   : "memory");
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int e = threadIdx.x; e < TT * N; e += THREADS) {
+    const int t = e / N, n = e % N;
+    const bool live = t >= begin && t < finish && n < state;
     const uint32_t d = (uint32_t)__cvta_generic_to_shared(&to[t][n]);
-    const T* src = live ? from + (tile0 + t) * ld + first + n : from;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"((int)sizeof(T)), "r"(live ? (int)sizeof(T) : 0)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(from + (live ? t * ld + n : begin * ld)),
+                 "n"((int)sizeof(T)), "r"(live ? (int)sizeof(T) : 0)
                  : "memory");
   }
 }
@@ -153,13 +242,15 @@ template <typename T> struct Span {
 template <typename T, int L, int S> struct Forward {
   static constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S;
   alignas(16) T B[2][TT][N], C[2][TT][N];
-  T dt[TT][CH], x[TT][CH], y[TT][CH];
+  typename StepOf<T>::type step[TT][CH];
+  T y[TT][CH + 8];              // (four tokens of eight channels at a time: no two in one bank)
 };
+
 // EDGES: only the state that the span ends in when it begins with zero, and the sum of its time steps.
 template <typename T, int L, int S, bool EDGES>
 __global__ void __launch_bounds__(THREADS)
 forward_kernel(const Args<T> a) {
-  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, CELLS = TT * CH, E = (CELLS + THREADS - 1) / THREADS;
+  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2, CELLS = TT * CH, E = (CELLS + THREADS - 1) / THREADS;
   extern __shared__ __align__(16) unsigned char raw[];
   Forward<T, L, S>& m = *reinterpret_cast<Forward<T, L, S>*>(raw);
   const Place<T, L, S> me(a);
@@ -167,122 +258,155 @@ forward_kernel(const Args<T> a) {
   const Span<T> span(a, p);
   int64_t begin = span.begin;
   const int64_t finish = span.finish;
-  T A[S], h[S];
-  me.load(a, a.A, A);
+  const int64_t states = (int64_t)a.dim * a.state;
+  Two<T> A[P], h[P];
+  {
+    T w[S];
+    me.load(a, a.A, w);
 #pragma unroll
-  for (int j = 0; j < S; ++j) {
-    A[j] = rate(A[j]);
-    h[j] = 0;
+    for (int j = 0; j < P; ++j) A[j] = {rate(w[2 * j]), rate(w[2 * j + 1])};
   }
-  const auto from_h0 = [&](int s, T(&h)[S]) {
+  const auto set = [&](const T* from) {        // null: zero
+    T w[S];
 #pragma unroll
-    for (int j = 0; j < S; ++j) h[j] = 0;
-    if (a.h0) me.load(a, a.h0 + (int64_t)s * a.dim * a.state, h);
+    for (int j = 0; j < S; ++j) w[j] = 0;
+    if (from) me.load(a, from, w);
+#pragma unroll
+    for (int j = 0; j < P; ++j) h[j] = {w[2 * j], w[2 * j + 1]};
   };
+  const auto keep = [&](T* to) {
+    T w[S];
+#pragma unroll
+    for (int j = 0; j < P; ++j) h[j].get(w[2 * j], w[2 * j + 1]);
+    me.store(a, to, w);
+  };
+  const auto initial = [&](int s) { return a.h0 ? a.h0 + s * states : nullptr; };
   // sequences without a token in front of all others
   const int64_t lo = a.rows.begin();
   if (!EDGES && a.h_last && ((span.first <= lo && lo < span.first + a.span) || (p == a.spans - 1 && lo >= span.first + a.span)))
     for (int s = 0; s < a.rows.count && a.rows.end(s) <= lo; ++s) {
-      T k[S];
-      from_h0(s, k);
-      me.store(a, a.h_last + (int64_t)s * a.dim * a.state, k);
+      set(initial(s));
+      keep(a.h_last + s * states);
     }
+  set(nullptr);
   if (EDGES) {
-    // what comes before the last sequence that begins in the span does not reach its end
+    // what comes before the last sequence that begins in the span does not reach its end, and nothing does beyond it if another
+    // sequence begins there
     const int64_t start = begin < finish ? a.rows.start(a.rows.at(finish - 1)) : begin;
     const bool all = start < begin;
     if (!all && start < finish) begin = start;
+    if (begin < finish && a.rows.end(a.rows.at(finish - 1)) <= finish) begin = finish;
     if (threadIdx.x == 0 && blockIdx.x == 0) a.passes[p] = all;
   }
-  T total = 0;
+  T sum = 0;
   if (begin < finish) {
     int s = a.rows.at(begin);
-    if (a.rows.start(s) >= begin) from_h0(s, h);
-    else if (!EDGES && p > 0) me.load(a, a.edge + (int64_t)p * a.dim * a.state, h);
+    int64_t end = a.rows.end(s);                // of sequence s, the one that the next token belongs to
+    if (a.rows.start(s) >= begin) set(initial(s));
+    else if (!EDGES && p > 0) set(a.edge + p * states);
     const int64_t tiles0 = begin / TT * TT;
+    // element i of this thread in a tile: token row0 + i L, channel col
+    const int col = threadIdx.x % CH, row0 = threadIdx.x / CH;
+    const bool in = col < me.channels && (CELLS % THREADS == 0 || threadIdx.x < CELLS);
+    const bool all = me.channels == CH && CELLS % THREADS == 0;
     T u[E], d[E], z[E];
-    const T bias = a.bias && threadIdx.x % CH < me.channels ? a.bias[me.c0 + threadIdx.x % CH] : (T)0;
-    const T D = !EDGES && a.D && threadIdx.x % CH < me.channels ? a.D[me.c0 + threadIdx.x % CH] : (T)0;
-    // element e of a tile: token e / CH, channel e % CH
+    const T bias = a.bias && in ? a.bias[me.c0 + col] : (T)0;
+    const T D = !EDGES && a.D && in ? a.D[me.c0 + col] : (T)0;
+    const T* pu = a.u + (tiles0 + row0) * a.ld_u + me.c0 + col;
+    const T* pd = a.delta + (tiles0 + row0) * a.ld_delta + me.c0 + col;
+    const T* pz = a.z ? a.z + (tiles0 + row0) * a.ld_z + me.c0 + col : nullptr;
     const auto fetch = [&](int64_t tile0) {
+      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
+      if (all && to - from == TT) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int e = threadIdx.x + i * THREADS, c = e % CH;
-        const int64_t t = tile0 + e / CH;
-        const bool live = t >= begin && t < finish && c < me.channels && (CELLS % THREADS == 0 || e < CELLS);
-        u[i] = live ? a.u[t * a.ld_u + me.c0 + c] : (T)0;
-        d[i] = live ? a.delta[t * a.ld_delta + me.c0 + c] : (T)0;
-        if (!EDGES) z[i] = live && a.z ? a.z[t * a.ld_z + me.c0 + c] : (T)0;
+        for (int i = 0; i < E; ++i) {
+          u[i] = pu[i * L * a.ld_u];
+          d[i] = pd[i * L * a.ld_delta];
+        }
+        if (!EDGES && a.z)
+#pragma unroll
+          for (int i = 0; i < E; ++i) z[i] = pz[i * L * a.ld_z];
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int r = row0 + i * L;
+          const bool live = in && r >= from && r < to;
+          u[i] = live ? pu[i * L * a.ld_u] : (T)0;
+          d[i] = live ? pd[i * L * a.ld_delta] : (T)0;
+          if (!EDGES) z[i] = live && a.z ? pz[i * L * a.ld_z] : (T)0;
+        }
       }
+      pu += TT * a.ld_u;
+      pd += TT * a.ld_delta;
+      if (!EDGES) pz += TT * a.ld_z;
+      fetch_rows<T, N, TT>(m.B[tile0 / TT & 1], a.B, a.ld_B, me.q * a.state, a.state, a.wide_B, tile0, from, to);
+      if (!EDGES) fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, tile0, from, to);
     };
     fetch(tiles0);
-    fetch_rows<T, N, TT>(m.B[0], a.B, a.ld_B, me.q * a.state, a.state, tiles0, begin, finish);
-    if constexpr (!EDGES) fetch_rows<T, N, TT>(m.C[0], a.C, a.ld_C, me.q * a.state, a.state, tiles0, begin, finish);
     commit();
-    int buf = 0;
-    for (int64_t tile0 = tiles0; tile0 < finish; tile0 += TT, buf ^= 1) {
+    T* py = EDGES ? nullptr : a.y + (tiles0 + row0) * a.ld_y + me.c0 + col;
+    for (int64_t tile0 = tiles0; tile0 < finish; tile0 += TT) {
+      const int buf = (int)(tile0 / TT & 1);
+      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
       T kept_u[E], kept_z[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int e = threadIdx.x + i * THREADS, c = e % CH;
-        const int64_t t = tile0 + e / CH;
+        const int r = row0 + i * L;
         T dt = d[i] + bias;
         if (a.softplus) dt = softplus(dt);
-        if (!(t >= begin && t < finish && c < me.channels)) dt = 0;
-        if (CELLS % THREADS == 0 || e < CELLS) {
-          m.dt[e / CH][c] = dt;
-          m.x[e / CH][c] = dt * u[i];
-        }
+        if (!(in && r >= from && r < to)) dt = 0;
+        if (CELLS % THREADS == 0 || threadIdx.x < CELLS) write(&m.step[r][col], dt, dt * u[i]);
         kept_u[i] = u[i];
         if (!EDGES) kept_z[i] = z[i];
       }
-      if (tile0 + TT < finish) {
-        fetch(tile0 + TT);
-        fetch_rows<T, N, TT>(m.B[buf ^ 1], a.B, a.ld_B, me.q * a.state, a.state, tile0 + TT, begin, finish);
-        if constexpr (!EDGES) fetch_rows<T, N, TT>(m.C[buf ^ 1], a.C, a.ld_C, me.q * a.state, a.state, tile0 + TT, begin, finish);
-      }
+      if (tile0 + TT < finish) fetch(tile0 + TT);
       commit();
       landed<1>();
       __syncthreads();
-      if (!EDGES && a.saved && tile0 >= begin) me.store(a, a.saved + tile0 / TT * a.dim * a.state, h);
-      uint32_t starts = starts_in<TT>(a.rows, s, tile0, finish);
-      if (tile0 <= begin) starts &= ~(1u << (int)(begin - tile0));       // (the state there is set)
+      const uint32_t starts = end < tile0 + TT && end < finish ? starts_in<TT>(a.rows, s, tile0, finish) : 0;
+      const T(*rows_B)[N] = m.B[buf];
+      const T(*rows_C)[N] = m.C[buf];
+      const auto token = [&](int t) {
+        Two<T> dt, x, B[P], r;
+        read(&m.step[t][me.ch], dt, x);
+        read(&rows_B[t][me.n0], B);
+        if (EDGES) {
+          T one, two;
+          dt.get(one, two);
+          sum += one;
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) h[j] = fma(decay(mul(dt, A[j])), h[j], mul(x, B[j]));
+        if (EDGES) return (T)0;
+        Two<T> C[P];
+        read(&rows_C[t][me.n0], C);
+        r = mul(C[0], h[0]);
+#pragma unroll
+        for (int j = 1; j < P; ++j) r = fma(C[j], h[j], r);
+        return total(r);
+      };
 #pragma unroll 2
       for (int t0 = 0; t0 < TT; t0 += 4) {
         T part[4];
+        if (!EDGES && t0 % POINT == 0 && a.saved && t0 >= from && t0 < to) keep(a.saved + (tile0 + t0) / POINT * states);
+        if ((starts >> t0 & 15) == 0) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = t0 + k;
-          if (starts >> t & 1) {
-            // the sequences that end here, and the ones without a token behind them
-            const int64_t here = tile0 + t;
-            for (; s + 1 < a.rows.count && a.rows.end(s) <= here; ++s) {
-              if (!EDGES && a.h_last) {
-                T k0[S];
-                if (a.rows.start(s) >= here) from_h0(s, h);
+          for (int k = 0; k < 4; ++k) part[k] = token(t0 + k);
+        } else {
 #pragma unroll
-                for (int j = 0; j < S; ++j) k0[j] = h[j];
-                me.store(a, a.h_last + (int64_t)s * a.dim * a.state, k0);
+          for (int k = 0; k < 4; ++k) {
+            if (starts >> (t0 + k) & 1) {
+              // the sequence that ends here, and the ones without a token behind it
+              const int64_t here = tile0 + t0 + k;
+              for (; s + 1 < a.rows.count && a.rows.end(s) <= here; ++s) {
+                if (a.rows.start(s) >= here) set(initial(s));
+                if (!EDGES && a.h_last) keep(a.h_last + s * states);
               }
+              set(initial(s));
+              end = a.rows.end(s);
+              sum = 0;
             }
-            from_h0(s, h);
-            total = 0;
-          }
-          const T dt = m.dt[t][me.ch], x = m.x[t][me.ch];
-          const Pack<T, S> B = *reinterpret_cast<const Pack<T, S>*>(&m.B[buf][t][me.n0]);
-          if (EDGES) {
-            total += dt;
-#pragma unroll
-            for (int j = 0; j < S; ++j) h[j] = decay(dt * A[j]) * h[j] + x * B.v[j];
-          } else {
-            const Pack<T, S> C = *reinterpret_cast<const Pack<T, S>*>(&m.C[buf][t][me.n0]);
-            T sum = 0;
-#pragma unroll
-            for (int j = 0; j < S; ++j) {
-              h[j] = decay(dt * A[j]) * h[j] + x * B.v[j];
-              sum += C.v[j] * h[j];
-            }
-            part[k] = sum;
+            part[k] = token(t0 + k);
           }
         }
         if (!EDGES) {
@@ -291,28 +415,34 @@ forward_kernel(const Args<T> a) {
         }
       }
       __syncthreads();
-      if (!EDGES)
+      if (!EDGES) {
+        T y[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int e = threadIdx.x + i * THREADS, c = e % CH;
-          const int64_t t = tile0 + e / CH;
-          if (t >= begin && t < finish && c < me.channels && (CELLS % THREADS == 0 || e < CELLS)) {
-            T r = m.y[e / CH][c] + D * kept_u[i];
-            if (a.z) r *= swish(kept_z[i]);
-            a.y[t * a.ld_y + me.c0 + c] = r;
-          }
+        for (int i = 0; i < E; ++i) y[i] = (CELLS % THREADS == 0 || threadIdx.x < CELLS ? m.y[row0 + i * L][col] : (T)0) + D * kept_u[i];
+        if (a.z)
+#pragma unroll
+          for (int i = 0; i < E; ++i) y[i] *= swish(kept_z[i]);
+        if (all && to - from == TT) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) py[i * L * a.ld_y] = y[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; ++i)
+            if (in && row0 + i * L >= from && row0 + i * L < to) py[i * L * a.ld_y] = y[i];
         }
+        py += TT * a.ld_y;
+      }
     }
     landed<0>();
     if (!EDGES && a.h_last)
       for (; s < a.rows.count && a.rows.end(s) <= finish; ++s) {
-        if (a.rows.start(s) >= finish) from_h0(s, h);
-        me.store(a, a.h_last + (int64_t)s * a.dim * a.state, h);
+        if (a.rows.start(s) >= finish) set(initial(s));
+        keep(a.h_last + s * states);
       }
   }
   if (EDGES) {
-    me.store(a, a.edge + (int64_t)(p + 1) * a.dim * a.state, h);
-    if (me.on && me.lane == 0) a.sum[(int64_t)p * a.dim + me.c0 + me.ch] = total;
+    keep(a.edge + (p + 1) * states);
+    if (me.on && me.lane == 0) a.sum[(int64_t)p * a.dim + me.c0 + me.ch] = sum;
   }
 }
 
@@ -326,107 +456,122 @@ join_kernel(const Args<T> a) {
   const T A = rate(a.A[i]);
   const int c = (int)(i / a.state);
   T carry = 0;
-  if (FORWARD) {
-#pragma unroll 4
-    for (int p = 0; p + 1 < a.spans; ++p) {
-      const T own = a.edge[(p + 1) * each + i];
-      const T through = decay(A * a.sum[(int64_t)p * a.dim + c]) * carry;
-      carry = own + (a.passes[p] ? through : (T)0);
-      a.edge[(p + 1) * each + i] = carry;
+  const int spans = FORWARD ? a.spans - 1 : a.spans;
+  constexpr int AHEAD = 8;             // spans whose values are on their way at the same time
+  for (int k0 = 0; k0 < spans; k0 += AHEAD) {
+    T own[AHEAD], through[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int p = FORWARD ? k0 + k : spans - 1 - k0 - k;
+      own[k] = through[k] = 0;
+      if (k0 + k < spans) {
+        own[k] = a.edge[(p + FORWARD) * each + i];
+        through[k] = a.passes[p] ? decay(A * a.sum[(int64_t)p * a.dim + c]) : (T)-1;
+      }
     }
-  } else {
-#pragma unroll 4
-    for (int p = a.spans - 1; p >= 0; --p) {
-      const T own = a.edge[p * each + i];
-      const T through = decay(A * a.sum[(int64_t)p * a.dim + c]) * carry;
-      a.edge[p * each + i] = carry;
-      carry = own + (a.passes[p] ? through : (T)0);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int p = FORWARD ? k0 + k : spans - 1 - k0 - k;
+      if (k0 + k >= spans) break;
+      if (!FORWARD) a.edge[p * each + i] = carry;
+      carry = through[k] < (T)0 ? own[k] : own[k] + through[k] * carry;      // (a decay is never negative)
+      if (FORWARD) a.edge[(p + 1) * each + i] = carry;
     }
   }
 }
 
 // ---------------------------------------------------------------- backward
 // What a span hands to the one above it when it is handed zero: a_n g_n of its first token.
+template <typename T, int L, int S> struct Edges {
+  static constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S;
+  alignas(16) T C[2][TT][N];
+  typename StepOf<T>::type step[TT][CH];        // dt and v
+};
 template <typename T, int L, int S>
 __global__ void __launch_bounds__(THREADS)
 backward_edges_kernel(const Args<T> a) {
-  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, CELLS = TT * CH, E = (CELLS + THREADS - 1) / THREADS;
-  __shared__ T s_dt[TT][CH], s_v[TT][CH];
-  __shared__ __align__(16) T s_C[2][TT][N];
+  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2, CELLS = TT * CH, E = (CELLS + THREADS - 1) / THREADS;
+  extern __shared__ __align__(16) unsigned char raw[];
+  Edges<T, L, S>& m = *reinterpret_cast<Edges<T, L, S>*>(raw);
   const Place<T, L, S> me(a);
   const int p = blockIdx.y;
   const Span<T> span(a, p);
   const int64_t begin = span.begin;
   int64_t finish = span.finish;
-  T A[S], e[S], total = 0;
-  me.load(a, a.A, A);
+  Two<T> A[P], e[P];
+  T sum = 0, w[S];
+  me.load(a, a.A, w);
 #pragma unroll
-  for (int j = 0; j < S; ++j) {
-    A[j] = rate(A[j]);
-    e[j] = 0;
+  for (int j = 0; j < P; ++j) {
+    A[j] = {rate(w[2 * j]), rate(w[2 * j + 1])};
+    e[j] = {(T)0, (T)0};
   }
   int passes = 0;
-  if (begin < finish) {
-    const int64_t end = a.rows.end(a.rows.at(begin));       // what comes behind the first sequence does not reach the span's start
+  if (begin < finish && p > 0 && a.rows.start(a.rows.at(begin)) < begin) {
+    const int64_t end = a.rows.end(a.rows.at(begin));       // what comes behind this sequence does not reach the span's start
     passes = end > finish;
     if (end < finish) finish = end;
-    T d[E], v[E];
-    const T bias = a.bias && threadIdx.x % CH < me.channels ? a.bias[me.c0 + threadIdx.x % CH] : (T)0;
+    const int col = threadIdx.x % CH, row0 = threadIdx.x / CH;
+    const bool in = col < me.channels && (CELLS % THREADS == 0 || threadIdx.x < CELLS);
+    T d[E], v[E], z[E];
+    const T bias = a.bias && in ? a.bias[me.c0 + col] : (T)0;
     const auto fetch = [&](int64_t tile0) {
+      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
+      const T* pd = a.delta + (tile0 + row0) * a.ld_delta + me.c0 + col;
+      const T* pv = a.dy + (tile0 + row0) * a.ld_dy + me.c0 + col;
+      const T* pz = a.z ? a.z + (tile0 + row0) * a.ld_z + me.c0 + col : nullptr;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int x = threadIdx.x + i * THREADS, c = x % CH;
-        const int64_t t = tile0 + x / CH;
-        const bool live = t >= begin && t < finish && c < me.channels && (CELLS % THREADS == 0 || x < CELLS);
-        d[i] = live ? a.delta[t * a.ld_delta + me.c0 + c] : (T)0;
-        v[i] = live ? a.dy[t * a.ld_dy + me.c0 + c] : (T)0;
-        if (a.z) v[i] *= live ? swish(a.z[t * a.ld_z + me.c0 + c]) : (T)0;
+        const int r = row0 + i * L;
+        const bool live = in && r >= from && r < to;
+        d[i] = live ? pd[i * L * a.ld_delta] : (T)0;
+        v[i] = live ? pv[i * L * a.ld_dy] : (T)0;
+        z[i] = live && a.z ? pz[i * L * a.ld_z] : (T)0;
       }
+      fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, tile0, from, to);
     };
     const int64_t top = (finish - 1) / TT * TT, bottom = begin / TT * TT;
     fetch(top);
-    fetch_rows<T, N, TT>(s_C[0], a.C, a.ld_C, me.q * a.state, a.state, top, begin, finish);
     commit();
-    int buf = 0;
-    for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT, buf ^= 1) {
+    for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT) {
+      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int x = threadIdx.x + i * THREADS, c = x % CH;
-        const int64_t t = tile0 + x / CH;
+        const int r = row0 + i * L;
         T dt = d[i] + bias;
         if (a.softplus) dt = softplus(dt);
-        if (!(t >= begin && t < finish && c < me.channels)) dt = 0;
-        if (CELLS % THREADS == 0 || x < CELLS) {
-          s_dt[x / CH][c] = dt;
-          s_v[x / CH][c] = v[i];
-        }
+        if (!(in && r >= from && r < to)) dt = 0;
+        if (CELLS % THREADS == 0 || threadIdx.x < CELLS) write(&m.step[r][col], dt, a.z ? v[i] * swish(z[i]) : v[i]);
       }
-      if (tile0 > bottom) {
-        fetch(tile0 - TT);
-        fetch_rows<T, N, TT>(s_C[buf ^ 1], a.C, a.ld_C, me.q * a.state, a.state, tile0 - TT, begin, finish);
-      }
+      if (tile0 > bottom) fetch(tile0 - TT);
       commit();
       landed<1>();
       __syncthreads();
+      const T(*rows)[N] = m.C[tile0 / TT & 1];
 #pragma unroll 4
       for (int t = TT - 1; t >= 0; --t) {
-        const T dt = s_dt[t][me.ch], vt = s_v[t][me.ch];
-        const Pack<T, S> C = *reinterpret_cast<const Pack<T, S>*>(&s_C[buf][t][me.n0]);
-        total += dt;
+        Two<T> dt, v2, C[P];
+        read(&m.step[t][me.ch], dt, v2);
+        read(&rows[t][me.n0], C);
+        T one, two;
+        dt.get(one, two);
+        sum += one;
 #pragma unroll
-        for (int j = 0; j < S; ++j) e[j] = decay(dt * A[j]) * (C.v[j] * vt + e[j]);
+        for (int j = 0; j < P; ++j) e[j] = mul(decay(mul(dt, A[j])), fma(C[j], v2, e[j]));
       }
       __syncthreads();
     }
     landed<0>();
   }
-  me.store(a, a.edge + (int64_t)p * a.dim * a.state, e);
-  if (me.on && me.lane == 0) a.sum[(int64_t)p * a.dim + me.c0 + me.ch] = total;
+#pragma unroll
+  for (int j = 0; j < P; ++j) e[j].get(w[2 * j], w[2 * j + 1]);
+  me.store(a, a.edge + (int64_t)p * a.dim * a.state, w);
+  if (me.on && me.lane == 0) a.sum[(int64_t)p * a.dim + me.c0 + me.ch] = sum;
   if (threadIdx.x == 0 && blockIdx.x == 0) a.passes[p] = passes;
 }
 
-// Values of 2 S sums a lane (dB, then dC of its states) over the warp's 32 / L channels: lanes L apart hold the same states.  As in
-// sum4, half of the values change hands in each step until one is left; returns how many are left and which they are.
+// Values of 2 S sums a lane (dB, then dC of its states) over the warp's 32 / L lanes that hold the same states of other channels.  As
+// in sum4, half of the values change hands in each step until one is left; returns how many are left and which they are.
 template <int L, int S, typename T> __device__ __forceinline__ void channel_sums(T (&v)[2 * S], int warp_lane, int& first, int& count) {
   first = 0;
   count = 2 * S;
@@ -448,222 +593,351 @@ template <int L, int S, typename T> __device__ __forceinline__ void channel_sums
   }
 }
 
-// The main pass: a tile's states again from its checkpoint, forwards, into shared memory, then the tile backwards.
+// The main pass: a tile's states again from its checkpoint, forwards, into shared memory, then the tile backwards.  A thread has its
+// states of CC channels: what is summed over the channels (dB, dC) is added up within the thread first, and the exchange between
+// the lanes, a quarter of the instructions, is paid once for both.
 template <typename T, int L, int S> struct Backward {
-  static constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, CELLS = TT * CH, E = (CELLS + THREADS - 1) / THREADS;
-  static constexpr int WARPS = THREADS / 32;
-  static constexpr int FT = TT * 16 / N < TT ? (TT * 16 / N) : TT;      // tokens whose dB and dC are gathered at a time
+  static constexpr int CC = sizeof(T) == 8 && L < 32 ? 1 : 2, HALF = THREADS / L, CH = CC * HALF, TT = POINT, N = L * S, P = S / 2;
+  static constexpr int E = TT * CH / THREADS, ROWS = THREADS / CH > 0 ? THREADS / CH : 1, WARPS = THREADS / 32;
+  static constexpr int FT = TT * 16 / N < TT ? TT * 16 / N : TT;      // tokens whose dB and dC are gathered at a time
+  struct alignas(16) Step { T dt, gB, x, gA; };                       // in float first {dt, dt, x, x}
   struct Shared {
-    Pack<T, S> h[TT][THREADS];
-    alignas(16) T B[TT][N], C[TT][N];
+    Pack<T, S> h[CC][TT][THREADS];
+    alignas(16) T B[2][TT][N], C[2][TT][N];
+    Step step[TT][CH];
     T red[WARPS][FT][2 * N];
-    T dt[TT][CH], u[TT][CH], v[TT][CH], r[TT][CH], gB[TT][CH], gA[TT][CH];
+    T v[TT][CH], u[TT][CH], slope[TT][CH], w[TT][CH];      // slope: d dt / d delta, w: dz / r
+    T r[TT][CH + 8];
   };
 };
+__device__ __forceinline__ void read_step(const float* m, Two<float>& dt, Two<float>& x) {
+  const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(m);
+  dt.v = q.x;
+  x.v = q.y;
+}
+__device__ __forceinline__ void read_step(const double* m, Two<double>& dt, Two<double>& x) {
+  dt = {m[0], m[0]};
+  x = {m[2], m[2]};
+}
 
 template <typename T, int L, int S>
 __global__ void __launch_bounds__(THREADS)
 backward_kernel(const Args<T> a) {
   using K = Backward<T, L, S>;
-  constexpr int CH = K::CH, TT = K::TT, N = K::N, CELLS = K::CELLS, E = K::E, FT = K::FT;
+  constexpr int CC = K::CC, HALF = K::HALF, CH = K::CH, TT = K::TT, N = K::N, P = K::P, E = K::E, FT = K::FT;
+  static_assert(TT * CH % THREADS == 0 && THREADS % CH == 0, "whole rows of threads");
   extern __shared__ __align__(16) unsigned char raw[];
   typename K::Shared& m = *reinterpret_cast<typename K::Shared*>(raw);
-  const Place<T, L, S> me(a);
-  const int p = blockIdx.y, wl = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // channels of the CTA: CH of a group; of a thread: ch[0], ch[0] + HALF
+  const int q = blockIdx.x / a.blocks, chan0 = blockIdx.x % a.blocks * CH, c0 = q * a.per + chan0;
+  const int channels = a.per - chan0 < CH ? a.per - chan0 : CH;
+  const int lane = threadIdx.x % L, n0 = lane * S, wl = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t states = (int64_t)a.dim * a.state;
+  const int p = blockIdx.y;
   const Span<T> span(a, p);
   const int64_t begin = span.begin, finish = span.finish;
-  T A[S], e[S], dA[S];
-  me.load(a, a.A, A);
+  const auto load = [&](const T* from, int k, Two<T>(&h)[P]) {       // null: zero
+    const int ch = threadIdx.x / L + k * HALF;
+    T w[S];
 #pragma unroll
-  for (int j = 0; j < S; ++j) {
-    A[j] = rate(A[j]);
-    e[j] = dA[j] = 0;
+    for (int j = 0; j < S; ++j) w[j] = from && ch < channels && n0 + j < a.state ? from[(int64_t)(c0 + ch) * a.state + n0 + j] : (T)0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) h[j] = {w[2 * j], w[2 * j + 1]};
+  };
+  const auto store = [&](T* to, int k, const Two<T>(&h)[P]) {
+    const int ch = threadIdx.x / L + k * HALF;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      T w[2];
+      h[j].get(w[0], w[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (ch < channels && n0 + 2 * j + i < a.state) to[(int64_t)(c0 + ch) * a.state + n0 + 2 * j + i] = w[i];
+    }
+  };
+  Two<T> A[CC][P], e[CC][P], dA[CC][P];
+#pragma unroll
+  for (int k = 0; k < CC; ++k) {
+    load(a.A, k, A[k]);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      T x, y;
+      A[k][j].get(x, y);
+      A[k][j] = {rate(x), rate(y)};
+      e[k][j] = dA[k][j] = {(T)0, (T)0};
+    }
   }
-  const int cc = threadIdx.x % CH;
-  const bool here = cc < me.channels;
-  const T bias = a.bias && here ? a.bias[me.c0 + cc] : (T)0, D = a.D && here ? a.D[me.c0 + cc] : (T)0;
+  const int col = threadIdx.x % CH, row0 = threadIdx.x / CH;
+  constexpr int ROWS = K::ROWS;                 // element i of this thread in a tile: token row0 + i ROWS, channel col
+  const bool in = col < channels;
+  const T bias = a.bias && in ? a.bias[c0 + col] : (T)0, D = a.D && in ? a.D[c0 + col] : (T)0;
   T dD = 0, dbias = 0;
   if (begin < finish) {
-    int s = a.rows.at(finish - 1);                     // the sequence of the token that is looked at
-    if (a.rows.end(s) > finish && p + 1 < a.spans) me.load(a, a.edge + (int64_t)p * a.dim * a.state, e);
+    if (p + 1 < a.spans && a.rows.end(a.rows.at(finish - 1)) > finish)
+#pragma unroll
+      for (int k = 0; k < CC; ++k) load(a.edge + p * states, k, e[k]);
     const int64_t top = (finish - 1) / TT * TT, bottom = begin / TT * TT;
-    for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT) {
-      const int64_t from = tile0 > begin ? tile0 : begin, to = tile0 + TT < finish ? tile0 + TT : finish;
-      fetch_rows<T, N, TT>(m.B, a.B, a.ld_B, me.q * a.state, a.state, tile0, begin, finish);
-      fetch_rows<T, N, TT>(m.C, a.C, a.ld_C, me.q * a.state, a.state, tile0, begin, finish);
-      commit();
-      T x_d[E], x_z[E], x_dy[E];
+    T u[E], d[E], z[E], dy[E];
+    Two<T> next[CC][P];                         // the checkpoint of the tile that is fetched
+    const auto fetch = [&](int64_t tile0) {
+      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
+      const T* pu = a.u + (tile0 + row0) * a.ld_u + c0 + col;
+      const T* pd = a.delta + (tile0 + row0) * a.ld_delta + c0 + col;
+      const T* pv = a.dy + (tile0 + row0) * a.ld_dy + c0 + col;
+      const T* pz = a.z ? a.z + (tile0 + row0) * a.ld_z + c0 + col : nullptr;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int x = threadIdx.x + i * THREADS;
-        const int64_t t = tile0 + x / CH;
-        const bool in = CELLS % THREADS == 0 || x < CELLS, live = t >= from && t < to && here && in;
-        const T u = live ? a.u[t * a.ld_u + me.c0 + cc] : (T)0;
-        x_d[i] = live ? a.delta[t * a.ld_delta + me.c0 + cc] + bias : (T)0;
-        x_z[i] = live && a.z ? a.z[t * a.ld_z + me.c0 + cc] : (T)0;
-        x_dy[i] = live ? a.dy[t * a.ld_dy + me.c0 + cc] : (T)0;
-        const T dt = a.softplus ? softplus(x_d[i]) : x_d[i];
-        if (in) {
-          m.dt[x / CH][cc] = live ? dt : (T)0;
-          m.u[x / CH][cc] = u;
-          m.v[x / CH][cc] = a.z ? x_dy[i] * swish(x_z[i]) : x_dy[i];
-        }
+        const int r = row0 + i * ROWS;
+        const bool live = in && r >= from && r < to;
+        u[i] = live ? pu[i * ROWS * a.ld_u] : (T)0;
+        d[i] = live ? pd[i * ROWS * a.ld_delta] : (T)0;
+        dy[i] = live ? pv[i * ROWS * a.ld_dy] : (T)0;
+        z[i] = live && a.z ? pz[i * ROWS * a.ld_z] : (T)0;
       }
-      // the state in front of the tile, and the tokens at which it is replaced
-      int s0 = a.rows.at(from);
-      T h[S], first[S];
+      fetch_rows<T, N, TT>(m.B[tile0 / TT & 1], a.B, a.ld_B, q * a.state, a.state, a.wide_B, tile0, from, to);
+      fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, q * a.state, a.state, a.wide_C, tile0, from, to);
 #pragma unroll
-      for (int j = 0; j < S; ++j) h[j] = 0;
-      if (a.rows.start(s0) < from) me.load(a, a.saved + tile0 / TT * a.dim * a.state, h);
-      uint32_t starts = starts_in<TT>(a.rows, s0, tile0, to);
-      if (a.rows.start(s0) >= from) starts |= 1u << (int)(from - tile0);
+      for (int k = 0; k < CC; ++k) load(from == 0 ? a.saved + tile0 / TT * states : nullptr, k, next[k]);
+    };
+    int s = a.rows.at(finish - 1);              // the sequence of the last token of the tile, and its first token
+    int64_t start = a.rows.start(s);
+    fetch(top);
+    commit();
+    for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT) {
+      const int buf = (int)(tile0 / TT & 1);
+      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
 #pragma unroll
-      for (int j = 0; j < S; ++j) first[j] = h[j];
-      landed<0>();
-      __syncthreads();
-#pragma unroll 2
-      for (int t0 = 0; t0 < TT; t0 += 4) {
-        T part[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = t0 + k;
-          if (starts >> t & 1) {
-            const int q = a.rows.at(tile0 + t);
-#pragma unroll
-            for (int j = 0; j < S; ++j) h[j] = 0;
-            if (a.h0) me.load(a, a.h0 + (int64_t)q * a.dim * a.state, h);
-          }
-          const T dt = m.dt[t][me.ch], x = dt * m.u[t][me.ch];
-          const Pack<T, S> B = *reinterpret_cast<const Pack<T, S>*>(&m.B[t][me.n0]);
-          const Pack<T, S> C = *reinterpret_cast<const Pack<T, S>*>(&m.C[t][me.n0]);
-          Pack<T, S> now;
-          T sum = 0;
-#pragma unroll
-          for (int j = 0; j < S; ++j) {
-            h[j] = decay(dt * A[j]) * h[j] + x * B.v[j];
-            now.v[j] = h[j];
-            sum += C.v[j] * h[j];
-          }
-          m.h[t][threadIdx.x] = now;
-          part[k] = sum;
+      for (int i = 0; i < E; ++i) {
+        const int r = row0 + i * ROWS;
+        const T x = d[i] + bias;
+        T dt = x, slope = 1, v = dy[i], w = 0;
+        if (a.softplus) {
+          dt = softplus(x);
+          slope = seq::sigmoid(x);
         }
-        const T r = sum4<L>(part, me.lane);
-        if (me.lane < 4) m.r[t0 + me.lane][me.ch] = r;
+        if (!(in && r >= from && r < to)) dt = 0;
+        if (a.z) {
+          const T g = seq::sigmoid(z[i]);
+          w = dy[i] * (g * ((T)1 + z[i] * ((T)1 - g)));
+          v *= z[i] * g;
+        }
+        const typename K::Step st = {dt, dt, dt * u[i], dt * u[i]};
+        m.step[r][col] = st;
+        m.v[r][col] = v;
+        m.u[r][col] = u[i];
+        m.slope[r][col] = slope;
+        m.w[r][col] = w;
+      }
+      Two<T> h[CC][P], first[CC][P];
+#pragma unroll
+      for (int k = 0; k < CC; ++k)
+#pragma unroll
+        for (int j = 0; j < P; ++j) h[k][j] = first[k][j] = next[k][j];
+      if (tile0 > bottom) fetch(tile0 - TT);
+      commit();
+      // the tokens that begin sequences
+      uint32_t starts = 0;
+      while (start >= tile0 + from) {
+        if (start < tile0 + to) starts |= 1u << (int)(start - tile0);
+        if (s == 0) {
+          start = -1;
+          break;
+        }
+        start = a.rows.start(--s);
+      }
+      landed<1>();
+      __syncthreads();
+      const T(*rows_B)[N] = m.B[buf];
+      const T(*rows_C)[N] = m.C[buf];
+#pragma unroll 1
+      for (int t0 = 0; t0 < TT; t0 += 4) {
+        T part[CC][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = t0 + i;
+          if (starts >> t & 1) {
+            const T* from0 = a.h0 ? a.h0 + a.rows.at(tile0 + t) * states : nullptr;
+#pragma unroll
+            for (int k = 0; k < CC; ++k) load(from0, k, h[k]);
+          }
+          Two<T> B[P], C[P];
+          read(&rows_B[t][n0], B);
+          read(&rows_C[t][n0], C);
+#pragma unroll
+          for (int k = 0; k < CC; ++k) {
+            Two<T> dt, x;
+            read_step(&m.step[t][threadIdx.x / L + k * HALF].dt, dt, x);
+            Pack<T, S> now;
+            Two<T> r;
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+              h[k][j] = fma(decay(mul(dt, A[k][j])), h[k][j], mul(x, B[j]));
+              h[k][j].get(now.v[2 * j], now.v[2 * j + 1]);
+              r = j ? fma(C[j], h[k][j], r) : mul(C[j], h[k][j]);
+            }
+            m.h[k][t][threadIdx.x] = now;
+            part[k][i] = total(r);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < CC; ++k) {
+          const T r = sum4<L>(part[k], lane);
+          if (lane < 4) m.r[t0 + lane][threadIdx.x / L + k * HALF] = r;
+        }
       }
       // backwards
-      T tile_dA[S];
+      Two<T> tile_dA[CC][P];
 #pragma unroll
-      for (int j = 0; j < S; ++j) tile_dA[j] = 0;
+      for (int k = 0; k < CC; ++k)
+#pragma unroll
+        for (int j = 0; j < P; ++j) tile_dA[k][j] = {(T)0, (T)0};
       for (int f = TT - FT; f >= 0; f -= FT) {
+        Two<T> now[CC][P];                      // the state behind the token that is looked at
+#pragma unroll
+        for (int k = 0; k < CC; ++k) read(m.h[k][f + FT - 1][threadIdx.x].v, now[k]);
 #pragma unroll 1
         for (int t0 = f + FT - 2; t0 >= f; t0 -= 2) {
-          T two[4];
+          T two[CC][4];
 #pragma unroll
-          for (int k = 1; k >= 0; --k) {
-            const int t = t0 + k;
-            const bool start = starts >> t & 1;
-            T before[S];
-            if (start) {
+          for (int i = 1; i >= 0; --i) {
+            const int t = t0 + i;
+            const bool begins = starts >> t & 1;
+            Two<T> before[CC][P], kept[CC][P];
+            if (t > 0) {
 #pragma unroll
-              for (int j = 0; j < S; ++j) before[j] = 0;
-              if (a.h0) me.load(a, a.h0 + (int64_t)a.rows.at(tile0 + t) * a.dim * a.state, before);
-            } else if (t > 0) {
-              const Pack<T, S> b = m.h[t - 1][threadIdx.x];
+              for (int k = 0; k < CC; ++k) {
+                read(m.h[k][t - 1][threadIdx.x].v, kept[k]);
 #pragma unroll
-              for (int j = 0; j < S; ++j) before[j] = b.v[j];
+                for (int j = 0; j < P; ++j) before[k][j] = kept[k][j];
+              }
             } else {
 #pragma unroll
-              for (int j = 0; j < S; ++j) before[j] = first[j];
-            }
-            const Pack<T, S> now = m.h[t][threadIdx.x];
-            const T dt = m.dt[t][me.ch], x = dt * m.u[t][me.ch], v = m.v[t][me.ch];
-            const Pack<T, S> B = *reinterpret_cast<const Pack<T, S>*>(&m.B[t][me.n0]);
-            const Pack<T, S> C = *reinterpret_cast<const Pack<T, S>*>(&m.C[t][me.n0]);
-            T gB = 0, gA = 0, rows[2 * S];
+              for (int k = 0; k < CC; ++k)
 #pragma unroll
-            for (int j = 0; j < S; ++j) {
-              const T g = C.v[j] * v + e[j], ag = decay(dt * A[j]) * g;
-              const T w = ag * before[j];
-              gB += g * B.v[j];
-              gA += w * A[j];
-              tile_dA[j] += w * dt;
-              rows[j] = g * x;
-              rows[S + j] = now.v[j] * v;
-              e[j] = ag;
+                for (int j = 0; j < P; ++j) before[k][j] = kept[k][j] = first[k][j];
             }
-            two[2 * k] = gB;
-            two[2 * k + 1] = gA;
+            if (begins) {
+              const T* from0 = a.h0 ? a.h0 + a.rows.at(tile0 + t) * states : nullptr;
+#pragma unroll
+              for (int k = 0; k < CC; ++k) load(from0, k, before[k]);
+            }
+            Two<T> B[P], C[P], dB[P], dC[P];
+            read(&rows_B[t][n0], B);
+            read(&rows_C[t][n0], C);
+#pragma unroll
+            for (int k = 0; k < CC; ++k) {
+              Two<T> dt, x, gB, gA;
+              const int ch = threadIdx.x / L + k * HALF;
+              read_step(&m.step[t][ch].dt, dt, x);
+              const T v1 = m.v[t][ch];
+              const Two<T> v = {v1, v1};
+#pragma unroll
+              for (int j = 0; j < P; ++j) {
+                const Two<T> g = fma(C[j], v, e[k][j]);
+                e[k][j] = mul(decay(mul(dt, A[k][j])), g);
+                const Two<T> w = mul(e[k][j], before[k][j]);
+                gB = j ? fma(g, B[j], gB) : mul(g, B[j]);
+                gA = j ? fma(w, A[k][j], gA) : mul(w, A[k][j]);
+                tile_dA[k][j] = fma(w, dt, tile_dA[k][j]);
+                dB[j] = k ? fma(g, x, dB[j]) : mul(g, x);
+                dC[j] = k ? fma(now[k][j], v, dC[j]) : mul(now[k][j], v);
+                now[k][j] = kept[k][j];
+              }
+              two[k][2 * i] = total(gB);
+              two[k][2 * i + 1] = total(gA);
+            }
+            T rows[2 * S];
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+              dB[j].get(rows[2 * j], rows[2 * j + 1]);
+              dC[j].get(rows[S + 2 * j], rows[S + 2 * j + 1]);
+            }
             int at, left;
             channel_sums<L, S>(rows, wl, at, left);
-            // value i of the 2 S: dB (i < S) or dC of state n0 + i mod S
+            // value x of the 2 S: dB (x < S) or dC of state n0 + x mod S
 #pragma unroll
             for (int j = 0; j < 2 * S; ++j)
               if (j < left) {      // (lanes that hold the same sum write the same value)
-                const int i = at + j;
-                m.red[warp][t - f][(i < S ? 0 : N) + me.n0 + i % S] = rows[j];
+                const int x = at + j;
+                m.red[warp][t - f][(x < S ? 0 : N) + n0 + x % S] = rows[j];
               }
-            if (start) {
-              if (a.dh0) me.store(a, a.dh0 + (int64_t)a.rows.at(tile0 + t) * a.dim * a.state, e);
+            if (begins) {
 #pragma unroll
-              for (int j = 0; j < S; ++j) e[j] = 0;
+              for (int k = 0; k < CC; ++k) {
+                if (a.dh0) store(a.dh0 + a.rows.at(tile0 + t) * states, k, e[k]);
+#pragma unroll
+                for (int j = 0; j < P; ++j) e[k][j] = {(T)0, (T)0};
+              }
             }
           }
-          const T r = sum4<L>(two, me.lane);
-          if (me.lane < 4) (me.lane & 1 ? m.gA : m.gB)[t0 + (me.lane >> 1)][me.ch] = r;
+          // over the second dt and dt u, which the channel's lanes have read
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < CC; ++k) {
+            const T r = sum4<L>(two[k], lane);
+            if (lane < 4) {
+              typename K::Step& st = m.step[t0 + (lane >> 1)][threadIdx.x / L + k * HALF];
+              (lane & 1 ? st.gA : st.gB) = r;
+            }
+          }
         }
         __syncthreads();
         // the warps' sums, in the order of the warps
         for (int i = threadIdx.x; i < FT * 2 * N; i += THREADS) {
           const int t = i / (2 * N), n = i % (2 * N), state = n < N ? n : n - N;
           const int64_t row = tile0 + f + t;
-          if (row >= from && row < to && state < a.state) {
+          if (f + t >= from && f + t < to && state < a.state) {
             T sum = 0;
 #pragma unroll
             for (int w = 0; w < K::WARPS; ++w) sum += m.red[w][t][n];
             if (a.blocks > 1)
-              a.part_BC[((((int64_t)(blockIdx.x % a.blocks) * a.rows.tokens + row) * a.groups + me.q) * 2 + (n >= N)) * a.state + state] = sum;
-            else if (n < N) a.dB[row * a.ld_dB + me.q * a.state + state] = sum;
-            else a.dC[row * a.ld_dC + me.q * a.state + state] = sum;
+              a.part_BC[((((int64_t)(blockIdx.x % a.blocks) * a.rows.tokens + row) * a.groups + q) * 2 + (n >= N)) * a.state + state] = sum;
+            else if (n < N) a.dB[row * a.ld_dB + q * a.state + state] = sum;
+            else a.dC[row * a.ld_dC + q * a.state + state] = sum;
           }
         }
-        __syncthreads();
+        if (f > 0) __syncthreads();
       }
 #pragma unroll
-      for (int j = 0; j < S; ++j) dA[j] += tile_dA[j];
+      for (int k = 0; k < CC; ++k)
+#pragma unroll
+        for (int j = 0; j < P; ++j) dA[k][j] = fma(tile_dA[k][j], Two<T>((T)1, (T)1), dA[k][j]);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int x = threadIdx.x + i * THREADS, tt = x / CH;
-        const int64_t t = tile0 + tt;
-        if (t >= from && t < to && here && (CELLS % THREADS == 0 || x < CELLS)) {
-          const T dt = m.dt[tt][cc], u = m.u[tt][cc], v = m.v[tt][cc], gB = m.gB[tt][cc];
-          T dd = u * gB + per_rate<T>() * m.gA[tt][cc];
-          if (a.softplus) dd *= seq::sigmoid(x_d[i]);
-          a.du[t * a.ld_du + me.c0 + cc] = dt * gB + D * v;
-          a.ddelta[t * a.ld_ddelta + me.c0 + cc] = dd;
-          if (a.z) a.dz[t * a.ld_dz + me.c0 + cc] = x_dy[i] * (m.r[tt][cc] + D * u) * swish_slope(x_z[i]);
-          dD += v * u;
+        const int r = row0 + i * ROWS;
+        if (in && r >= from && r < to) {
+          const int64_t t = tile0 + r;
+          const typename K::Step st = m.step[r][col];
+          const T ut = m.u[r][col], v = m.v[r][col];
+          const T dd = (ut * st.gB + per_rate<T>() * st.gA) * m.slope[r][col];
+          a.du[t * a.ld_du + c0 + col] = st.dt * st.gB + D * v;
+          a.ddelta[t * a.ld_ddelta + c0 + col] = dd;
+          if (a.z) a.dz[t * a.ld_dz + c0 + col] = m.w[r][col] * (m.r[r][col] + D * ut);
+          dD += v * ut;
           dbias += dd;
         }
       }
       __syncthreads();
     }
+    landed<0>();
   }
-  me.store(a, a.part_A + (int64_t)p * a.dim * a.state, dA);
+#pragma unroll
+  for (int k = 0; k < CC; ++k) store(a.part_A + p * states, k, dA[k]);
   // the threads of a channel, in their order
   __syncthreads();
   T* const sums = reinterpret_cast<T*>(m.h);
   sums[threadIdx.x] = dD;
   sums[THREADS + threadIdx.x] = dbias;
   __syncthreads();
-  if (threadIdx.x < me.channels) {
+  if (threadIdx.x < channels) {
     dD = dbias = 0;
 #pragma unroll
-    for (int k = 0; k < L; ++k) {
+    for (int k = 0; k < ROWS; ++k) {
       dD += sums[k * CH + threadIdx.x];
       dbias += sums[THREADS + k * CH + threadIdx.x];
     }
-    a.part_D[(int64_t)p * a.dim + me.c0 + threadIdx.x] = dD;
-    a.part_bias[(int64_t)p * a.dim + me.c0 + threadIdx.x] = dbias;
+    a.part_D[(int64_t)p * a.dim + c0 + threadIdx.x] = dD;
+    a.part_bias[(int64_t)p * a.dim + c0 + threadIdx.x] = dbias;
   }
 }
 
@@ -744,20 +1018,34 @@ step_kernel(const Args<T> a) {
 // ---------------------------------------------------------------- launches
 enum class Pass { Forward, Backward, Step };
 
-// How the token axis is cut: by sequences where they are of equal length and give CTAs enough for the device, else into spans of
-// whole tiles.
-template <typename T> static void cut(prad_ctx* ctx, Args<T>& a, int64_t ctas_across) {
-  const int64_t full = (int64_t)ctx->sm_count * 4;
-  if (!a.rows.offsets && a.rows.count > 0 && (a.rows.count * ctas_across >= full / 2 || a.rows.each <= 2 * tile<T>()) &&
-      a.rows.count <= 65535) {
+// CTAs of a kernel that the device holds at a time
+template <auto Kernel> static int64_t resident(prad_ctx* ctx, int smem) {
+  static std::atomic<int> each{0};           // per SM: the same for every device this library is built for
+  int n = each.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, THREADS, smem) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = 1;
+    }
+    each.store(n, std::memory_order_relaxed);
+  }
+  return (int64_t)n * ctx->sm_count;
+}
+
+// How the token axis is cut: by sequences where they are of equal length and fill at least half of the device (the edges' pass is
+// about half of the work again), else into spans of whole tiles, as many as the device holds at a time: one CTA more takes as long
+// as twice as many.
+template <typename T> static void cut(Args<T>& a, int64_t across, int64_t full) {
+  if (!a.rows.offsets && a.rows.count > 0 && a.rows.count <= 65535 && (a.rows.count * across >= full / 2 || a.rows.each <= 2 * tile<T>())) {
     a.span = a.rows.each > 0 ? a.rows.each : 1;
     a.spans = a.rows.count;
     return;
   }
-  int64_t spans = ceil_div(full, ctas_across);
+  int64_t spans = full / across;
+  if (spans < 1) spans = 1;
+  if (spans > 65535) spans = 65535;
   int64_t span = ceil_div(ceil_div(a.rows.tokens, spans), tile<T>()) * tile<T>();
   if (span < 2 * tile<T>()) span = 2 * tile<T>();
-  if (ceil_div(a.rows.tokens, span) > 65535) span = ceil_div(ceil_div(a.rows.tokens, 65535), tile<T>()) * tile<T>();
   a.span = span;
   a.spans = (int)ceil_div(a.rows.tokens, span);
   if (a.spans < 1) a.spans = 1;
@@ -792,8 +1080,11 @@ template <typename T> static size_t carve(Args<T>& a, bool backward, void* ws) {
 }
 
 template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Args<T> a, Pass pass) {
-  constexpr int CH = THREADS / L;
-  a.blocks = (int)ceil_div(a.per, CH);
+  using Main = Backward<T, L, S>;
+  const bool backward = pass == Pass::Backward;
+  // the edges' pass has THREADS / L channels a CTA, the main backward pass CC times as many
+  const int edge_blocks = (int)ceil_div(a.per, THREADS / L);
+  a.blocks = backward ? (int)ceil_div(a.per, Main::CH) : edge_blocks;
   const int64_t across = (int64_t)a.groups * a.blocks;
   PRAD_REQUIRE(across <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many channels");
   if (pass == Pass::Step) {
@@ -808,35 +1099,34 @@ template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Arg
     }
     return PRAD_OK;
   }
-  cut(ctx, a, across);
-  const bool backward = pass == Pass::Backward;
-  prad_status st = ensure_workspace(ctx, carve(a, backward, nullptr));
+  using Shared = typename Main::Shared;
+  constexpr int bytes = (int)sizeof(Forward<T, L, S>);
+  prad_status st = backward ? allow_smem<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : allow_smem<forward_kernel<T, L, S, false>>(ctx, bytes);
+  constexpr int edge_bytes = (int)sizeof(Edges<T, L, S>);
+  if (!st) st = backward ? allow_smem<backward_edges_kernel<T, L, S>>(ctx, edge_bytes) : allow_smem<forward_kernel<T, L, S, true>>(ctx, bytes);
+  if (st) return st;
+  cut(a, across, backward ? resident<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : resident<forward_kernel<T, L, S, false>>(ctx, bytes));
+  st = ensure_workspace(ctx, carve(a, backward, nullptr));
   if (st) return st;
   carve(a, backward, ctx->ws);
   const int64_t states = (int64_t)a.dim * a.state;
   const unsigned x = (unsigned)across;
   if (!backward) {
-    constexpr int bytes = (int)sizeof(Forward<T, L, S>);
     if (joined(a)) {
-      st = allow_smem<forward_kernel<T, L, S, true>>(ctx, bytes);
-      if (st) return st;
       forward_kernel<T, L, S, true><<<dim3(x, (unsigned)a.spans - 1), THREADS, bytes, ctx->stream>>>(a);
       PRAD_LAUNCHED(ctx);
       join_kernel<T, true><<<(unsigned)ceil_div(states, THREADS), THREADS, 0, ctx->stream>>>(a);
       PRAD_LAUNCHED(ctx);
     }
-    st = allow_smem<forward_kernel<T, L, S, false>>(ctx, bytes);
-    if (st) return st;
     forward_kernel<T, L, S, false><<<dim3(x, (unsigned)a.spans), THREADS, bytes, ctx->stream>>>(a);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
-  using Shared = typename Backward<T, L, S>::Shared;
-  st = allow_smem<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared));
-  if (st) return st;
   if (a.dh0) PRAD_CUDA(cudaMemsetAsync(a.dh0, 0, (size_t)a.rows.count * states * sizeof(T), ctx->stream));
   if (joined(a)) {
-    backward_edges_kernel<T, L, S><<<dim3(x, (unsigned)a.spans), THREADS, 0, ctx->stream>>>(a);
+    Args<T> b = a;
+    b.blocks = edge_blocks;
+    backward_edges_kernel<T, L, S><<<dim3((unsigned)(a.groups * edge_blocks), (unsigned)a.spans), THREADS, edge_bytes, ctx->stream>>>(b);
     PRAD_LAUNCHED(ctx);
     join_kernel<T, false><<<(unsigned)ceil_div(states, THREADS), THREADS, 0, ctx->stream>>>(a);
     PRAD_LAUNCHED(ctx);
@@ -853,7 +1143,6 @@ template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Arg
   return PRAD_OK;
 }
 template <typename T> static prad_status pick(prad_ctx* ctx, const Args<T>& a, Pass pass) {
-  if (a.state <= 4) return launch<T, 4, 1>(ctx, a, pass);
   if (a.state <= 8) return launch<T, 4, 2>(ctx, a, pass);
   if (a.state <= 16) return launch<T, 4, 4>(ctx, a, pass);
   if (a.state <= 32) return launch<T, 8, 4>(ctx, a, pass);
@@ -889,8 +1178,11 @@ template <typename T> static Args<T> args_of(const prad_scan_t* s) {
   a.rows = Sequences{s->offsets, s->sequences, s->tokens, s->offsets || s->sequences == 0 ? 0 : s->tokens / s->sequences};
   a.dim = s->dim, a.state = s->state, a.groups = s->groups, a.per = s->dim / s->groups;
   a.softplus = s->delta_softplus;
+  constexpr int V = 16 / sizeof(T);
+  const auto wide = [&](const void* m, int64_t ld) { return ((uintptr_t)m & 15) == 0 && ld % V == 0 && s->state % V == 0; };
   a.ld_u = s->ld_u ? s->ld_u : s->dim, a.ld_delta = s->ld_delta ? s->ld_delta : s->dim, a.ld_z = s->ld_z ? s->ld_z : s->dim;
   a.ld_B = s->ld_B ? s->ld_B : rows, a.ld_C = s->ld_C ? s->ld_C : rows;
+  a.wide_B = wide(s->B, a.ld_B), a.wide_C = wide(s->C, a.ld_C);
   a.u = (const T*)s->u, a.delta = (const T*)s->delta, a.z = (const T*)s->z, a.A = (const T*)s->A, a.B = (const T*)s->B;
   a.C = (const T*)s->C, a.D = (const T*)s->D, a.bias = (const T*)s->delta_bias, a.h0 = (const T*)s->h0;
   return a;
@@ -924,8 +1216,7 @@ extern "C" prad_status prad_selective_scan_saved_bytes(prad_dtype dt, const prad
   prad_status st = ssm::check("prad_selective_scan_saved_bytes", dt, scan);
   if (st) return st;
   PRAD_REQUIRE(out_bytes, PRAD_ERR_INVALID, "prad_selective_scan_saved_bytes: null output");
-  const int64_t tile = dt == PRAD_F64 ? ssm::tile<double>() : ssm::tile<float>();
-  *out_bytes = (size_t)ceil_div(scan->tokens, tile) * scan->dim * scan->state * dtype_size(dt);
+  *out_bytes = (size_t)ceil_div(scan->tokens, ssm::POINT) * scan->dim * scan->state * dtype_size(dt);
   return PRAD_OK;
 }
 
