@@ -33,7 +33,8 @@ template <typename T> struct Args {
   Sequences rows;
   int64_t span;                 // tokens of a span
   int spans, dim, state, groups, per, blocks;   // per: channels of a group, in `blocks` CTAs
-  int softplus, wide_B, wide_C;      // rows of B, C that can be copied 16 bytes at a time
+  int softplus;
+  int wide, wide_B, wide_C;     // the token matrices, B and C can be read and written 16 bytes at a time
   int64_t ld_u, ld_delta, ld_z, ld_B, ld_C, ld_y, ld_dy, ld_du, ld_ddelta, ld_dz, ld_dB, ld_dC;
   const T *u, *delta, *z, *A, *B, *C, *D, *bias, *h0, *dy;
   T *y, *h_last, *saved;
@@ -66,6 +67,16 @@ __device__ __forceinline__ float softplus(float x) {
   p = fmaf(p, q, 0.333331608f);
   p = fmaf(p, q, 1.0f);
   return fmaf(r + r, p, fmaxf(x, 0.0f));
+}
+// the same and its derivative, the sigmoid
+__device__ __forceinline__ float softplus(float x, float& slope) {
+  const float w = seq::exp2_approx(fabsf(x) * -1.4426950408889634f), i = seq::reciprocal(1.0f + w);
+  slope = x > 0.0f ? i : w * i;
+  return softplus(x);
+}
+__device__ __forceinline__ double softplus(double x, double& slope) {
+  slope = seq::sigmoid(x);
+  return fmax(x, 0.0) + log1p(exp(-fabs(x)));
 }
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
@@ -144,6 +155,27 @@ __device__ __forceinline__ void read(const StepD* m, Two<double>& dt, Two<double
 
 template <typename T, int S> struct alignas(sizeof(T) * S) Pack { T v[S]; };
 
+// How a warp's lanes share channels and states: a lane's number among the L of its channel is made of the lane's bits 1, 4, 3, 2, 0 (as
+// many as L needs), its channel's number of the others.  A 128-bit read of shared memory takes two cycles if its address does not
+// depend on bit 0 or does not depend on bit 1 of the lane, and four otherwise: so the reads by channel and those by state both take two.
+template <int L> struct Lanes {
+  static constexpr int STATE_BITS = L == 4 ? 2 : L == 8 ? 3 : L == 16 ? 4 : 5;
+  __host__ __device__ static constexpr int state_bit(int i) { return i == 0 ? 1 : i == 4 ? 0 : 5 - i; }
+  __host__ __device__ static constexpr int channel_bit(int i) { return i == 0 ? 0 : i + 1; }
+  __device__ static __forceinline__ int state(int lane) {
+    int l = 0;
+#pragma unroll
+    for (int i = 0; i < STATE_BITS; ++i) l |= (lane >> state_bit(i) & 1) << i;
+    return l;
+  }
+  __device__ static __forceinline__ int channel(int lane) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < 5 - STATE_BITS; ++i) c |= (lane >> channel_bit(i) & 1) << i;
+    return c;
+  }
+};
+
 // A CTA's channels and a thread's place among them.
 template <typename T, int L, int S> struct Place {
   static constexpr int CH = THREADS / L;
@@ -154,8 +186,8 @@ template <typename T, int L, int S> struct Place {
     const int first = blockIdx.x % a.blocks * CH;
     c0 = q * a.per + first;
     channels = a.per - first < CH ? a.per - first : CH;
-    ch = threadIdx.x / L;
-    lane = threadIdx.x % L;
+    ch = threadIdx.x / 32 * (32 / L) + Lanes<L>::channel(threadIdx.x % 32);
+    lane = Lanes<L>::state(threadIdx.x % 32);
     n0 = lane * S;
     on = ch < channels;
   }
@@ -172,16 +204,16 @@ template <typename T, int L, int S> struct Place {
 };
 
 // Four values a lane, one for each of four tokens, summed over the L lanes of a channel: afterwards lane l holds the sum of token
-// l mod 4 (L >= 4).  Half of the values change hands in each of the first two steps.
+// l mod 4.  Half of the values change hands in each of the first two steps.
 template <int L, typename T> __device__ __forceinline__ T sum4(const T (&v)[4], int lane) {
   const bool hi = lane & 2, odd = lane & 1;
   T a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
-  a += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 2);
-  b += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 2);
+  a += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 1 << Lanes<L>::state_bit(1));
+  b += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 1 << Lanes<L>::state_bit(1));
   T c = odd ? b : a;
-  c += __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+  c += __shfl_xor_sync(0xffffffffu, odd ? a : b, 1 << Lanes<L>::state_bit(0));
 #pragma unroll
-  for (int o = 4; o < L; o <<= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+  for (int i = 2; i < Lanes<L>::STATE_BITS; ++i) c += __shfl_xor_sync(0xffffffffu, c, 1 << Lanes<L>::state_bit(i));
   return c;
 }
 
@@ -238,23 +270,95 @@ template <typename T> struct Span {
   }
 };
 
+// The token matrices' part of a tile: a thread has V neighbouring channels of E rows.
+template <typename T, int CH, int TT> struct Cells {
+  static constexpr int V = 16 / sizeof(T), ACROSS = CH / V, ROWS = THREADS / ACROSS, E = TT > ROWS ? TT / ROWS : 1;
+  static_assert(CH % V == 0 && (TT % ROWS == 0 || ROWS % TT == 0), "whole rows of threads");
+  int col, row, mine;            // mine: of the V channels, those that exist
+  bool wide;
+  __device__ __forceinline__ Cells(int channels, bool aligned) {
+    col = threadIdx.x % ACROSS * V;
+    row = threadIdx.x / ACROSS;
+    mine = channels - col < V ? channels - col : V;
+    wide = aligned && mine == V;
+  }
+  // whether row e of this thread lies in the tile
+  __device__ __forceinline__ bool in(int e) const { return ROWS <= TT || row < TT; }
+  // rows [from, to) of the tile; what lies outside, and channels that do not exist, as zero
+  __device__ __forceinline__ void load(const T* tile, int64_t ld, int from, int to, T (&v)[E][V]) const {
+    const T* at = tile + row * ld + col;
+#pragma unroll
+    for (int e = 0; e < E; ++e, at += ROWS * ld) {
+      const bool live = row + e * ROWS >= from && row + e * ROWS < to;
+      if (wide) {
+        Pack<T, V> w;
+#pragma unroll
+        for (int j = 0; j < V; ++j) w.v[j] = 0;
+        if (live) w = *reinterpret_cast<const Pack<T, V>*>(at);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[e][j] = w.v[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[e][j] = live && j < mine ? at[j] : (T)0;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* tile, int64_t ld, int from, int to, const T (&v)[E][V]) const {
+    T* at = tile + row * ld + col;
+#pragma unroll
+    for (int e = 0; e < E; ++e, at += ROWS * ld) {
+      const bool live = row + e * ROWS >= from && row + e * ROWS < to;
+      if (wide) {
+        Pack<T, V> w;
+#pragma unroll
+        for (int j = 0; j < V; ++j) w.v[j] = v[e][j];
+        if (live) *reinterpret_cast<Pack<T, V>*>(at) = w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (live && j < mine) at[j] = v[e][j];
+      }
+    }
+  }
+  // one value per channel
+  __device__ __forceinline__ void per_channel(const T* m, T (&v)[V]) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = m && j < mine ? m[col + j] : (T)0;
+  }
+};
+// Where channel c's entry of 16 bytes lies in a row of shared memory: threads that write V channels each, and warps that read eight,
+// spread over all banks.
+template <typename T> __device__ __forceinline__ int spot(int c) { return c ^ (c >> 3 & (16 / (int)sizeof(T) - 1)); }
+// V values side by side in shared memory
+template <int V, typename T> __device__ __forceinline__ void put(T* m, const T (&v)[V]) {
+  Pack<T, V> w;
+#pragma unroll
+  for (int j = 0; j < V; ++j) w.v[j] = v[j];
+  *reinterpret_cast<Pack<T, V>*>(m) = w;
+}
+template <int V, typename T> __device__ __forceinline__ void pick(const T* m, T (&v)[V]) {
+  const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(m);
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = w.v[j];
+}
+
 // ---------------------------------------------------------------- forward
 template <typename T, int L, int S> struct Forward {
   static constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S;
   alignas(16) T B[2][TT][N], C[2][TT][N];
   typename StepOf<T>::type step[TT][CH];
-  T y[TT][CH + 8];              // (four tokens of eight channels at a time: no two in one bank)
+  alignas(16) T y[TT][CH + 8];  // (four tokens of eight channels at a time: no two in one bank)
 };
 
 // EDGES: only the state that the span ends in when it begins with zero, and the sum of its time steps.
 template <typename T, int L, int S, bool EDGES>
 __global__ void __launch_bounds__(THREADS)
 forward_kernel(const Args<T> a) {
-  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2, CELLS = TT * CH, E = (CELLS + THREADS - 1) / THREADS;
+  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
   Forward<T, L, S>& m = *reinterpret_cast<Forward<T, L, S>*>(raw);
   const Place<T, L, S> me(a);
-  const int p = blockIdx.y;
+  const int p = blockIdx.y, at = spot<T>(me.ch);
   const Span<T> span(a, p);
   int64_t begin = span.begin;
   const int64_t finish = span.finish;
@@ -305,59 +409,38 @@ forward_kernel(const Args<T> a) {
     if (a.rows.start(s) >= begin) set(initial(s));
     else if (!EDGES && p > 0) set(a.edge + p * states);
     const int64_t tiles0 = begin / TT * TT;
-    // element i of this thread in a tile: token row0 + i L, channel col
-    const int col = threadIdx.x % CH, row0 = threadIdx.x / CH;
-    const bool in = col < me.channels && (CELLS % THREADS == 0 || threadIdx.x < CELLS);
-    const bool all = me.channels == CH && CELLS % THREADS == 0;
-    T u[E], d[E], z[E];
-    const T bias = a.bias && in ? a.bias[me.c0 + col] : (T)0;
-    const T D = !EDGES && a.D && in ? a.D[me.c0 + col] : (T)0;
-    const T* pu = a.u + (tiles0 + row0) * a.ld_u + me.c0 + col;
-    const T* pd = a.delta + (tiles0 + row0) * a.ld_delta + me.c0 + col;
-    const T* pz = a.z ? a.z + (tiles0 + row0) * a.ld_z + me.c0 + col : nullptr;
+    const Cells<T, CH, TT> mine(me.channels, a.wide);
+    constexpr int E = Cells<T, CH, TT>::E, V = Cells<T, CH, TT>::V, ROWS = Cells<T, CH, TT>::ROWS;
+    T u[E][V], d[E][V], z[E][V], bias[V], D[V];
+    mine.per_channel(a.bias ? a.bias + me.c0 : nullptr, bias);
+    mine.per_channel(!EDGES && a.D ? a.D + me.c0 : nullptr, D);
     const auto fetch = [&](int64_t tile0) {
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      if (all && to - from == TT) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          u[i] = pu[i * L * a.ld_u];
-          d[i] = pd[i * L * a.ld_delta];
-        }
-        if (!EDGES && a.z)
-#pragma unroll
-          for (int i = 0; i < E; ++i) z[i] = pz[i * L * a.ld_z];
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int r = row0 + i * L;
-          const bool live = in && r >= from && r < to;
-          u[i] = live ? pu[i * L * a.ld_u] : (T)0;
-          d[i] = live ? pd[i * L * a.ld_delta] : (T)0;
-          if (!EDGES) z[i] = live && a.z ? pz[i * L * a.ld_z] : (T)0;
-        }
-      }
-      pu += TT * a.ld_u;
-      pd += TT * a.ld_delta;
-      if (!EDGES) pz += TT * a.ld_z;
+      mine.load(a.u + tile0 * a.ld_u + me.c0, a.ld_u, from, to, u);
+      mine.load(a.delta + tile0 * a.ld_delta + me.c0, a.ld_delta, from, to, d);
+      if (!EDGES && a.z) mine.load(a.z + tile0 * a.ld_z + me.c0, a.ld_z, from, to, z);
       fetch_rows<T, N, TT>(m.B[tile0 / TT & 1], a.B, a.ld_B, me.q * a.state, a.state, a.wide_B, tile0, from, to);
       if (!EDGES) fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, tile0, from, to);
     };
     fetch(tiles0);
     commit();
-    T* py = EDGES ? nullptr : a.y + (tiles0 + row0) * a.ld_y + me.c0 + col;
     for (int64_t tile0 = tiles0; tile0 < finish; tile0 += TT) {
       const int buf = (int)(tile0 / TT & 1);
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      T kept_u[E], kept_z[E];
+      T kept_u[E][V], kept_z[E][V];
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int r = row0 + i * L;
-        T dt = d[i] + bias;
-        if (a.softplus) dt = softplus(dt);
-        if (!(in && r >= from && r < to)) dt = 0;
-        if (CELLS % THREADS == 0 || threadIdx.x < CELLS) write(&m.step[r][col], dt, dt * u[i]);
-        kept_u[i] = u[i];
-        if (!EDGES) kept_z[i] = z[i];
+      for (int e = 0; e < E; ++e) {
+        const int r = mine.row + e * ROWS;
+        const bool live = r >= from && r < to;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          T dt = d[e][j] + bias[j];
+          if (a.softplus) dt = softplus(dt);
+          if (!live) dt = 0;
+          if (mine.in(e)) write(&m.step[r][spot<T>(mine.col + j)], dt, dt * u[e][j]);
+          kept_u[e][j] = u[e][j];
+          if (!EDGES) kept_z[e][j] = z[e][j];
+        }
       }
       if (tile0 + TT < finish) fetch(tile0 + TT);
       commit();
@@ -368,7 +451,7 @@ forward_kernel(const Args<T> a) {
       const T(*rows_C)[N] = m.C[buf];
       const auto token = [&](int t) {
         Two<T> dt, x, B[P], r;
-        read(&m.step[t][me.ch], dt, x);
+        read(&m.step[t][at], dt, x);
         read(&rows_B[t][me.n0], B);
         if (EDGES) {
           T one, two;
@@ -416,21 +499,17 @@ forward_kernel(const Args<T> a) {
       }
       __syncthreads();
       if (!EDGES) {
-        T y[E];
+        T y[E][V];
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = (CELLS % THREADS == 0 || threadIdx.x < CELLS ? m.y[row0 + i * L][col] : (T)0) + D * kept_u[i];
-        if (a.z)
+        for (int e = 0; e < E; ++e) {
+          pick(&m.y[mine.in(e) ? mine.row + e * ROWS : 0][mine.col], y[e]);
 #pragma unroll
-          for (int i = 0; i < E; ++i) y[i] *= swish(kept_z[i]);
-        if (all && to - from == TT) {
-#pragma unroll
-          for (int i = 0; i < E; ++i) py[i * L * a.ld_y] = y[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < E; ++i)
-            if (in && row0 + i * L >= from && row0 + i * L < to) py[i * L * a.ld_y] = y[i];
+          for (int j = 0; j < V; ++j) {
+            y[e][j] += D[j] * kept_u[e][j];
+            if (a.z) y[e][j] *= swish(kept_z[e][j]);
+          }
         }
-        py += TT * a.ld_y;
+        mine.store(a.y + tile0 * a.ld_y + me.c0, a.ld_y, from, to, y);
       }
     }
     landed<0>();
@@ -490,11 +569,11 @@ template <typename T, int L, int S> struct Edges {
 template <typename T, int L, int S>
 __global__ void __launch_bounds__(THREADS)
 backward_edges_kernel(const Args<T> a) {
-  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2, CELLS = TT * CH, E = (CELLS + THREADS - 1) / THREADS;
+  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
   Edges<T, L, S>& m = *reinterpret_cast<Edges<T, L, S>*>(raw);
   const Place<T, L, S> me(a);
-  const int p = blockIdx.y;
+  const int p = blockIdx.y, at = spot<T>(me.ch);
   const Span<T> span(a, p);
   const int64_t begin = span.begin;
   int64_t finish = span.finish;
@@ -511,23 +590,15 @@ backward_edges_kernel(const Args<T> a) {
     const int64_t end = a.rows.end(a.rows.at(begin));       // what comes behind this sequence does not reach the span's start
     passes = end > finish;
     if (end < finish) finish = end;
-    const int col = threadIdx.x % CH, row0 = threadIdx.x / CH;
-    const bool in = col < me.channels && (CELLS % THREADS == 0 || threadIdx.x < CELLS);
-    T d[E], v[E], z[E];
-    const T bias = a.bias && in ? a.bias[me.c0 + col] : (T)0;
+    const Cells<T, CH, TT> mine(me.channels, a.wide);
+    constexpr int E = Cells<T, CH, TT>::E, V = Cells<T, CH, TT>::V, ROWS = Cells<T, CH, TT>::ROWS;
+    T d[E][V], v[E][V], z[E][V], bias[V];
+    mine.per_channel(a.bias ? a.bias + me.c0 : nullptr, bias);
     const auto fetch = [&](int64_t tile0) {
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      const T* pd = a.delta + (tile0 + row0) * a.ld_delta + me.c0 + col;
-      const T* pv = a.dy + (tile0 + row0) * a.ld_dy + me.c0 + col;
-      const T* pz = a.z ? a.z + (tile0 + row0) * a.ld_z + me.c0 + col : nullptr;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int r = row0 + i * L;
-        const bool live = in && r >= from && r < to;
-        d[i] = live ? pd[i * L * a.ld_delta] : (T)0;
-        v[i] = live ? pv[i * L * a.ld_dy] : (T)0;
-        z[i] = live && a.z ? pz[i * L * a.ld_z] : (T)0;
-      }
+      mine.load(a.delta + tile0 * a.ld_delta + me.c0, a.ld_delta, from, to, d);
+      mine.load(a.dy + tile0 * a.ld_dy + me.c0, a.ld_dy, from, to, v);
+      if (a.z) mine.load(a.z + tile0 * a.ld_z + me.c0, a.ld_z, from, to, z);
       fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, tile0, from, to);
     };
     const int64_t top = (finish - 1) / TT * TT, bottom = begin / TT * TT;
@@ -536,12 +607,16 @@ backward_edges_kernel(const Args<T> a) {
     for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT) {
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int r = row0 + i * L;
-        T dt = d[i] + bias;
-        if (a.softplus) dt = softplus(dt);
-        if (!(in && r >= from && r < to)) dt = 0;
-        if (CELLS % THREADS == 0 || threadIdx.x < CELLS) write(&m.step[r][col], dt, a.z ? v[i] * swish(z[i]) : v[i]);
+      for (int e0 = 0; e0 < E; ++e0) {
+        const int r = mine.row + e0 * ROWS;
+        const bool live = r >= from && r < to;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          T dt = d[e0][j] + bias[j];
+          if (a.softplus) dt = softplus(dt);
+          if (!live) dt = 0;
+          if (mine.in(e0)) write(&m.step[r][spot<T>(mine.col + j)], dt, a.z ? v[e0][j] * swish(z[e0][j]) : v[e0][j]);
+        }
       }
       if (tile0 > bottom) fetch(tile0 - TT);
       commit();
@@ -551,7 +626,7 @@ backward_edges_kernel(const Args<T> a) {
 #pragma unroll 4
       for (int t = TT - 1; t >= 0; --t) {
         Two<T> dt, v2, C[P];
-        read(&m.step[t][me.ch], dt, v2);
+        read(&m.step[t][at], dt, v2);
         read(&rows[t][me.n0], C);
         T one, two;
         dt.get(one, two);
@@ -576,7 +651,8 @@ template <int L, int S, typename T> __device__ __forceinline__ void channel_sums
   first = 0;
   count = 2 * S;
 #pragma unroll
-  for (int o = 16; o >= L; o >>= 1) {
+  for (int i = 0; i < 5 - Lanes<L>::STATE_BITS; ++i) {
+    const int o = 1 << Lanes<L>::channel_bit(i);
     const bool upper = warp_lane & o;
     if (count > 1) {
       count >>= 1;
@@ -598,16 +674,17 @@ template <int L, int S, typename T> __device__ __forceinline__ void channel_sums
 // the lanes, a quarter of the instructions, is paid once for both.
 template <typename T, int L, int S> struct Backward {
   static constexpr int CC = sizeof(T) == 8 && L < 32 ? 1 : 2, HALF = THREADS / L, CH = CC * HALF, TT = POINT, N = L * S, P = S / 2;
-  static constexpr int E = TT * CH / THREADS, ROWS = THREADS / CH > 0 ? THREADS / CH : 1, WARPS = THREADS / 32;
-  static constexpr int FT = TT * 16 / N < TT ? TT * 16 / N : TT;      // tokens whose dB and dC are gathered at a time
+  static constexpr int WARPS = THREADS / 32;
+  // tokens whose dB and dC are gathered at a time
+  static constexpr int FT = 8 * 16 / N < 2 ? 2 : 8 * 16 / N < 8 ? 8 * 16 / N : 8;
   struct alignas(16) Step { T dt, gB, x, gA; };                       // in float first {dt, dt, x, x}
   struct Shared {
-    Pack<T, S> h[CC][TT][THREADS];
+    Pack<T, S> h[CC][TT + 1][THREADS];                                // the state in front of each token, and behind the last
     alignas(16) T B[2][TT][N], C[2][TT][N];
     Step step[TT][CH];
     T red[WARPS][FT][2 * N];
-    T v[TT][CH], u[TT][CH], slope[TT][CH], w[TT][CH];      // slope: d dt / d delta, w: dz / r
-    T r[TT][CH + 8];
+    alignas(16) T v[TT][CH], u[TT][CH], slope[TT][CH], w[TT][CH];      // slope: d dt / d delta, w: dz / r
+    alignas(16) T r[TT][CH + 8];
   };
 };
 __device__ __forceinline__ void read_step(const float* m, Two<float>& dt, Two<float>& x) {
@@ -624,20 +701,23 @@ template <typename T, int L, int S>
 __global__ void __launch_bounds__(THREADS)
 backward_kernel(const Args<T> a) {
   using K = Backward<T, L, S>;
-  constexpr int CC = K::CC, HALF = K::HALF, CH = K::CH, TT = K::TT, N = K::N, P = K::P, E = K::E, FT = K::FT;
-  static_assert(TT * CH % THREADS == 0 && THREADS % CH == 0, "whole rows of threads");
+  constexpr int CC = K::CC, HALF = K::HALF, CH = K::CH, TT = K::TT, N = K::N, P = K::P, FT = K::FT;
   extern __shared__ __align__(16) unsigned char raw[];
   typename K::Shared& m = *reinterpret_cast<typename K::Shared*>(raw);
   // channels of the CTA: CH of a group; of a thread: ch[0], ch[0] + HALF
   const int q = blockIdx.x / a.blocks, chan0 = blockIdx.x % a.blocks * CH, c0 = q * a.per + chan0;
   const int channels = a.per - chan0 < CH ? a.per - chan0 : CH;
-  const int lane = threadIdx.x % L, n0 = lane * S, wl = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wl = threadIdx.x & 31, warp = threadIdx.x >> 5, lane = Lanes<L>::state(wl), n0 = lane * S;
+  const int ch0 = warp * (32 / L) + Lanes<L>::channel(wl);
+  int at0[CC];                                  // of this thread's entries of `step`
+#pragma unroll
+  for (int k = 0; k < CC; ++k) at0[k] = spot<T>(ch0 + k * HALF);
   const int64_t states = (int64_t)a.dim * a.state;
   const int p = blockIdx.y;
   const Span<T> span(a, p);
   const int64_t begin = span.begin, finish = span.finish;
   const auto load = [&](const T* from, int k, Two<T>(&h)[P]) {       // null: zero
-    const int ch = threadIdx.x / L + k * HALF;
+    const int ch = ch0 + k * HALF;
     T w[S];
 #pragma unroll
     for (int j = 0; j < S; ++j) w[j] = from && ch < channels && n0 + j < a.state ? from[(int64_t)(c0 + ch) * a.state + n0 + j] : (T)0;
@@ -645,7 +725,7 @@ backward_kernel(const Args<T> a) {
     for (int j = 0; j < P; ++j) h[j] = {w[2 * j], w[2 * j + 1]};
   };
   const auto store = [&](T* to, int k, const Two<T>(&h)[P]) {
-    const int ch = threadIdx.x / L + k * HALF;
+    const int ch = ch0 + k * HALF;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       T w[2];
@@ -667,33 +747,26 @@ backward_kernel(const Args<T> a) {
       e[k][j] = dA[k][j] = {(T)0, (T)0};
     }
   }
-  const int col = threadIdx.x % CH, row0 = threadIdx.x / CH;
-  constexpr int ROWS = K::ROWS;                 // element i of this thread in a tile: token row0 + i ROWS, channel col
-  const bool in = col < channels;
-  const T bias = a.bias && in ? a.bias[c0 + col] : (T)0, D = a.D && in ? a.D[c0 + col] : (T)0;
-  T dD = 0, dbias = 0;
+  const Cells<T, CH, TT> mine(channels, a.wide);
+  constexpr int E = Cells<T, CH, TT>::E, V = Cells<T, CH, TT>::V, ROWS = Cells<T, CH, TT>::ROWS;
+  T bias[V], D[V], dD[V], dbias[V];
+  mine.per_channel(a.bias ? a.bias + c0 : nullptr, bias);
+  mine.per_channel(a.D ? a.D + c0 : nullptr, D);
+#pragma unroll
+  for (int j = 0; j < V; ++j) dD[j] = dbias[j] = 0;
   if (begin < finish) {
     if (p + 1 < a.spans && a.rows.end(a.rows.at(finish - 1)) > finish)
 #pragma unroll
       for (int k = 0; k < CC; ++k) load(a.edge + p * states, k, e[k]);
     const int64_t top = (finish - 1) / TT * TT, bottom = begin / TT * TT;
-    T u[E], d[E], z[E], dy[E];
+    T u[E][V], d[E][V], z[E][V], dy[E][V];
     Two<T> next[CC][P];                         // the checkpoint of the tile that is fetched
     const auto fetch = [&](int64_t tile0) {
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      const T* pu = a.u + (tile0 + row0) * a.ld_u + c0 + col;
-      const T* pd = a.delta + (tile0 + row0) * a.ld_delta + c0 + col;
-      const T* pv = a.dy + (tile0 + row0) * a.ld_dy + c0 + col;
-      const T* pz = a.z ? a.z + (tile0 + row0) * a.ld_z + c0 + col : nullptr;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int r = row0 + i * ROWS;
-        const bool live = in && r >= from && r < to;
-        u[i] = live ? pu[i * ROWS * a.ld_u] : (T)0;
-        d[i] = live ? pd[i * ROWS * a.ld_delta] : (T)0;
-        dy[i] = live ? pv[i * ROWS * a.ld_dy] : (T)0;
-        z[i] = live && a.z ? pz[i * ROWS * a.ld_z] : (T)0;
-      }
+      mine.load(a.u + tile0 * a.ld_u + c0, a.ld_u, from, to, u);
+      mine.load(a.delta + tile0 * a.ld_delta + c0, a.ld_delta, from, to, d);
+      mine.load(a.dy + tile0 * a.ld_dy + c0, a.ld_dy, from, to, dy);
+      if (a.z) mine.load(a.z + tile0 * a.ld_z + c0, a.ld_z, from, to, z);
       fetch_rows<T, N, TT>(m.B[tile0 / TT & 1], a.B, a.ld_B, q * a.state, a.state, a.wide_B, tile0, from, to);
       fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, q * a.state, a.state, a.wide_C, tile0, from, to);
 #pragma unroll
@@ -708,31 +781,44 @@ backward_kernel(const Args<T> a) {
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int r = row0 + i * ROWS;
-        const T x = d[i] + bias;
-        T dt = x, slope = 1, v = dy[i], w = 0;
-        if (a.softplus) {
-          dt = softplus(x);
-          slope = seq::sigmoid(x);
+        const int r = mine.row + i * ROWS;
+        const bool live = r >= from && r < to;
+        T v[V], slope[V], w[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const T x = d[i][j] + bias[j];
+          T dt = x;
+          slope[j] = 1;
+          if (a.softplus) dt = softplus(x, slope[j]);
+          if (!live) dt = 0;
+          v[j] = dy[i][j];
+          w[j] = 0;
+          if (a.z) {
+            const T g = seq::sigmoid(z[i][j]);
+            w[j] = v[j] * (g * ((T)1 + z[i][j] * ((T)1 - g)));
+            v[j] *= z[i][j] * g;
+          }
+          const typename K::Step st = {dt, dt, dt * u[i][j], dt * u[i][j]};
+          if (mine.in(i)) m.step[r][spot<T>(mine.col + j)] = st;
         }
-        if (!(in && r >= from && r < to)) dt = 0;
-        if (a.z) {
-          const T g = seq::sigmoid(z[i]);
-          w = dy[i] * (g * ((T)1 + z[i] * ((T)1 - g)));
-          v *= z[i] * g;
+        if (mine.in(i)) {
+          put(&m.v[r][mine.col], v);
+          put(&m.u[r][mine.col], u[i]);
+          put(&m.slope[r][mine.col], slope);
+          put(&m.w[r][mine.col], w);
         }
-        const typename K::Step st = {dt, dt, dt * u[i], dt * u[i]};
-        m.step[r][col] = st;
-        m.v[r][col] = v;
-        m.u[r][col] = u[i];
-        m.slope[r][col] = slope;
-        m.w[r][col] = w;
       }
-      Two<T> h[CC][P], first[CC][P];
+      Two<T> h[CC][P];
 #pragma unroll
-      for (int k = 0; k < CC; ++k)
+      for (int k = 0; k < CC; ++k) {
+        Pack<T, S> w;
 #pragma unroll
-        for (int j = 0; j < P; ++j) h[k][j] = first[k][j] = next[k][j];
+        for (int j = 0; j < P; ++j) {
+          h[k][j] = next[k][j];
+          h[k][j].get(w.v[2 * j], w.v[2 * j + 1]);
+        }
+        m.h[k][0][threadIdx.x] = w;
+      }
       if (tile0 > bottom) fetch(tile0 - TT);
       commit();
       // the tokens that begin sequences
@@ -749,87 +835,72 @@ backward_kernel(const Args<T> a) {
       __syncthreads();
       const T(*rows_B)[N] = m.B[buf];
       const T(*rows_C)[N] = m.C[buf];
+      const auto initial = [&](int t) { return a.h0 ? a.h0 + a.rows.at(tile0 + t) * states : nullptr; };
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += 4) {
         T part[CC][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        const auto token = [&](int i) {
           const int t = t0 + i;
-          if (starts >> t & 1) {
-            const T* from0 = a.h0 ? a.h0 + a.rows.at(tile0 + t) * states : nullptr;
-#pragma unroll
-            for (int k = 0; k < CC; ++k) load(from0, k, h[k]);
-          }
           Two<T> B[P], C[P];
           read(&rows_B[t][n0], B);
           read(&rows_C[t][n0], C);
 #pragma unroll
           for (int k = 0; k < CC; ++k) {
-            Two<T> dt, x;
-            read_step(&m.step[t][threadIdx.x / L + k * HALF].dt, dt, x);
+            Two<T> dt, x, r;
+            read_step(&m.step[t][at0[k]].dt, dt, x);
             Pack<T, S> now;
-            Two<T> r;
 #pragma unroll
             for (int j = 0; j < P; ++j) {
               h[k][j] = fma(decay(mul(dt, A[k][j])), h[k][j], mul(x, B[j]));
               h[k][j].get(now.v[2 * j], now.v[2 * j + 1]);
               r = j ? fma(C[j], h[k][j], r) : mul(C[j], h[k][j]);
             }
-            m.h[k][t][threadIdx.x] = now;
+            m.h[k][t + 1][threadIdx.x] = now;
             part[k][i] = total(r);
+          }
+        };
+        if ((starts >> t0 & 15) == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) token(i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (starts >> (t0 + i) & 1)
+#pragma unroll
+              for (int k = 0; k < CC; ++k) load(initial(t0 + i), k, h[k]);
+            token(i);
           }
         }
 #pragma unroll
         for (int k = 0; k < CC; ++k) {
           const T r = sum4<L>(part[k], lane);
-          if (lane < 4) m.r[t0 + lane][threadIdx.x / L + k * HALF] = r;
+          if (lane < 4) m.r[t0 + lane][ch0 + k * HALF] = r;
         }
       }
       // backwards
-      Two<T> tile_dA[CC][P];
+      Two<T> tile_dA[CC][P], now[CC][P];        // now: the state behind the token that is looked at
 #pragma unroll
       for (int k = 0; k < CC; ++k)
 #pragma unroll
-        for (int j = 0; j < P; ++j) tile_dA[k][j] = {(T)0, (T)0};
+        for (int j = 0; j < P; ++j) {
+          tile_dA[k][j] = {(T)0, (T)0};
+          now[k][j] = h[k][j];
+        }
       for (int f = TT - FT; f >= 0; f -= FT) {
-        Two<T> now[CC][P];                      // the state behind the token that is looked at
-#pragma unroll
-        for (int k = 0; k < CC; ++k) read(m.h[k][f + FT - 1][threadIdx.x].v, now[k]);
 #pragma unroll 1
         for (int t0 = f + FT - 2; t0 >= f; t0 -= 2) {
           T two[CC][4];
-#pragma unroll
-          for (int i = 1; i >= 0; --i) {
+          // one token: its gradients from the state in front of it
+          const auto token = [&](int i, const Two<T>(&before)[CC][P]) {
             const int t = t0 + i;
-            const bool begins = starts >> t & 1;
-            Two<T> before[CC][P], kept[CC][P];
-            if (t > 0) {
-#pragma unroll
-              for (int k = 0; k < CC; ++k) {
-                read(m.h[k][t - 1][threadIdx.x].v, kept[k]);
-#pragma unroll
-                for (int j = 0; j < P; ++j) before[k][j] = kept[k][j];
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < CC; ++k)
-#pragma unroll
-                for (int j = 0; j < P; ++j) before[k][j] = kept[k][j] = first[k][j];
-            }
-            if (begins) {
-              const T* from0 = a.h0 ? a.h0 + a.rows.at(tile0 + t) * states : nullptr;
-#pragma unroll
-              for (int k = 0; k < CC; ++k) load(from0, k, before[k]);
-            }
             Two<T> B[P], C[P], dB[P], dC[P];
             read(&rows_B[t][n0], B);
             read(&rows_C[t][n0], C);
 #pragma unroll
             for (int k = 0; k < CC; ++k) {
               Two<T> dt, x, gB, gA;
-              const int ch = threadIdx.x / L + k * HALF;
-              read_step(&m.step[t][ch].dt, dt, x);
-              const T v1 = m.v[t][ch];
+              read_step(&m.step[t][at0[k]].dt, dt, x);
+              const T v1 = m.v[t][ch0 + k * HALF];
               const Two<T> v = {v1, v1};
 #pragma unroll
               for (int j = 0; j < P; ++j) {
@@ -841,7 +912,6 @@ backward_kernel(const Args<T> a) {
                 tile_dA[k][j] = fma(w, dt, tile_dA[k][j]);
                 dB[j] = k ? fma(g, x, dB[j]) : mul(g, x);
                 dC[j] = k ? fma(now[k][j], v, dC[j]) : mul(now[k][j], v);
-                now[k][j] = kept[k][j];
               }
               two[k][2 * i] = total(gB);
               two[k][2 * i + 1] = total(gA);
@@ -855,46 +925,84 @@ backward_kernel(const Args<T> a) {
             int at, left;
             channel_sums<L, S>(rows, wl, at, left);
             // value x of the 2 S: dB (x < S) or dC of state n0 + x mod S
+            T* const to = &m.red[warp][t - f][n0 + (at < S ? at : N + at - S)];
 #pragma unroll
             for (int j = 0; j < 2 * S; ++j)
-              if (j < left) {      // (lanes that hold the same sum write the same value)
-                const int x = at + j;
-                m.red[warp][t - f][(x < S ? 0 : N) + n0 + x % S] = rows[j];
-              }
-            if (begins) {
+              if (j < left) to[left > S && j >= S ? N + j - S : j] = rows[j];      // (lanes with the same sum write the same value)
+          };
+          const auto in_front = [&](int t, Two<T>(&to)[CC][P]) {
+#pragma unroll
+            for (int k = 0; k < CC; ++k) read(m.h[k][t][threadIdx.x].v, to[k]);
+          };
+          Two<T> one[CC][P], zero[CC][P];
+          in_front(t0 + 1, one);
+          in_front(t0, zero);
+          if ((starts >> t0 & 3) == 0) {
+            token(1, one);
+#pragma unroll
+            for (int k = 0; k < CC; ++k)
+#pragma unroll
+              for (int j = 0; j < P; ++j) now[k][j] = one[k][j];
+            token(0, zero);
+          } else {
+#pragma unroll
+            for (int i = 1; i >= 0; --i) {
+              const bool begins = starts >> (t0 + i) & 1;
+              Two<T> before[CC][P];
 #pragma unroll
               for (int k = 0; k < CC; ++k) {
-                if (a.dh0) store(a.dh0 + a.rows.at(tile0 + t) * states, k, e[k]);
 #pragma unroll
-                for (int j = 0; j < P; ++j) e[k][j] = {(T)0, (T)0};
+                for (int j = 0; j < P; ++j) before[k][j] = i ? one[k][j] : zero[k][j];
+                if (begins) load(initial(t0 + i), k, before[k]);
+              }
+              token(i, before);
+#pragma unroll
+              for (int k = 0; k < CC; ++k) {
+                if (begins && a.dh0) store(a.dh0 + a.rows.at(tile0 + t0 + i) * states, k, e[k]);
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                  if (begins) e[k][j] = {(T)0, (T)0};
+                  if (i) now[k][j] = one[k][j];
+                }
               }
             }
           }
+#pragma unroll
+          for (int k = 0; k < CC; ++k)
+#pragma unroll
+            for (int j = 0; j < P; ++j) now[k][j] = zero[k][j];
           // over the second dt and dt u, which the channel's lanes have read
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < CC; ++k) {
             const T r = sum4<L>(two[k], lane);
             if (lane < 4) {
-              typename K::Step& st = m.step[t0 + (lane >> 1)][threadIdx.x / L + k * HALF];
+              typename K::Step& st = m.step[t0 + (lane >> 1)][at0[k]];
               (lane & 1 ? st.gA : st.gB) = r;
             }
           }
         }
         __syncthreads();
         // the warps' sums, in the order of the warps
-        for (int i = threadIdx.x; i < FT * 2 * N; i += THREADS) {
-          const int t = i / (2 * N), n = i % (2 * N), state = n < N ? n : n - N;
-          const int64_t row = tile0 + f + t;
-          if (f + t >= from && f + t < to && state < a.state) {
-            T sum = 0;
-#pragma unroll
-            for (int w = 0; w < K::WARPS; ++w) sum += m.red[w][t][n];
-            if (a.blocks > 1)
-              a.part_BC[((((int64_t)(blockIdx.x % a.blocks) * a.rows.tokens + row) * a.groups + q) * 2 + (n >= N)) * a.state + state] = sum;
-            else if (n < N) a.dB[row * a.ld_dB + q * a.state + state] = sum;
-            else a.dC[row * a.ld_dC + q * a.state + state] = sum;
+        constexpr int ACROSS = 2 * N < THREADS ? 2 * N : THREADS;
+        for (int n = threadIdx.x % ACROSS; n < 2 * N; n += ACROSS) {
+          const int state = n < N ? n : n - N;
+          if (state >= a.state) continue;
+          T* to0 = n < N ? a.dB + q * a.state + state : a.dC + q * a.state + state;
+          int64_t ld = n < N ? a.ld_dB : a.ld_dC;
+          if (a.blocks > 1) {
+            to0 = a.part_BC + ((int64_t)(blockIdx.x % a.blocks) * a.rows.tokens * a.groups + q) * 2 * a.state + (n < N ? 0 : a.state) + state;
+            ld = (int64_t)a.groups * 2 * a.state;
           }
+          to0 += (tile0 + f) * ld;
+#pragma unroll
+          for (int t = threadIdx.x / ACROSS; t < FT; t += THREADS / ACROSS)
+            if (f + t >= from && f + t < to) {
+              T sum = 0;
+#pragma unroll
+              for (int w = 0; w < K::WARPS; ++w) sum += m.red[w][t][n];
+              to0[t * ld] = sum;
+            }
         }
         if (f > 0) __syncthreads();
       }
@@ -902,21 +1010,32 @@ backward_kernel(const Args<T> a) {
       for (int k = 0; k < CC; ++k)
 #pragma unroll
         for (int j = 0; j < P; ++j) dA[k][j] = fma(tile_dA[k][j], Two<T>((T)1, (T)1), dA[k][j]);
+      T du[E][V], dd[E][V], dz[E][V];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int r = row0 + i * ROWS;
-        if (in && r >= from && r < to) {
-          const int64_t t = tile0 + r;
-          const typename K::Step st = m.step[r][col];
-          const T ut = m.u[r][col], v = m.v[r][col];
-          const T dd = (ut * st.gB + per_rate<T>() * st.gA) * m.slope[r][col];
-          a.du[t * a.ld_du + c0 + col] = st.dt * st.gB + D * v;
-          a.ddelta[t * a.ld_ddelta + c0 + col] = dd;
-          if (a.z) a.dz[t * a.ld_dz + c0 + col] = m.w[r][col] * (m.r[r][col] + D * ut);
-          dD += v * ut;
-          dbias += dd;
+        const int r = mine.in(i) ? mine.row + i * ROWS : 0;
+        const bool live = mine.in(i) && r >= from && r < to;
+        T ut[V], v[V], slope[V], w[V], rt[V];
+        pick(&m.u[r][mine.col], ut);
+        pick(&m.v[r][mine.col], v);
+        pick(&m.slope[r][mine.col], slope);
+        pick(&m.w[r][mine.col], w);
+        pick(&m.r[r][mine.col], rt);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const typename K::Step st = m.step[r][spot<T>(mine.col + j)];
+          du[i][j] = st.dt * st.gB + D[j] * v[j];
+          dd[i][j] = (ut[j] * st.gB + per_rate<T>() * st.gA) * slope[j];
+          dz[i][j] = w[j] * (rt[j] + D[j] * ut[j]);
+          if (live) {
+            dD[j] += v[j] * ut[j];
+            dbias[j] += dd[i][j];
+          }
         }
       }
+      mine.store(a.du + tile0 * a.ld_du + c0, a.ld_du, from, to, du);
+      mine.store(a.ddelta + tile0 * a.ld_ddelta + c0, a.ld_ddelta, from, to, dd);
+      if (a.z) mine.store(a.dz + tile0 * a.ld_dz + c0, a.ld_dz, from, to, dz);
       __syncthreads();
     }
     landed<0>();
@@ -925,19 +1044,19 @@ backward_kernel(const Args<T> a) {
   for (int k = 0; k < CC; ++k) store(a.part_A + p * states, k, dA[k]);
   // the threads of a channel, in their order
   __syncthreads();
-  T* const sums = reinterpret_cast<T*>(m.h);
-  sums[threadIdx.x] = dD;
-  sums[THREADS + threadIdx.x] = dbias;
-  __syncthreads();
-  if (threadIdx.x < channels) {
-    dD = dbias = 0;
+  T(*const sums)[2][CH] = reinterpret_cast<T(*)[2][CH]>(m.h);
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-      dD += sums[k * CH + threadIdx.x];
-      dbias += sums[THREADS + k * CH + threadIdx.x];
-    }
-    a.part_D[(int64_t)p * a.dim + c0 + threadIdx.x] = dD;
-    a.part_bias[(int64_t)p * a.dim + c0 + threadIdx.x] = dbias;
+  for (int j = 0; j < V; ++j) {
+    sums[mine.row][0][mine.col + j] = dD[j];
+    sums[mine.row][1][mine.col + j] = dbias[j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * CH; i += THREADS) {
+    const int c = i % CH;
+    T sum = 0;
+#pragma unroll
+    for (int k = 0; k < (ROWS < TT ? ROWS : TT); ++k) sum += sums[k][i / CH][c];
+    if (c < channels) (i < CH ? a.part_D : a.part_bias)[(int64_t)p * a.dim + c0 + c] = sum;
   }
 }
 
@@ -1007,7 +1126,7 @@ step_kernel(const Args<T> a) {
   }
   me.store(a, a.h_last + row * a.dim * a.state, h);
 #pragma unroll
-  for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int i = 0; i < Lanes<L>::STATE_BITS; ++i) sum += __shfl_xor_sync(0xffffffffu, sum, 1 << Lanes<L>::state_bit(i));
   if (me.on && me.lane == 0) {
     if (a.D) sum += a.D[c] * u;
     if (a.z) sum *= swish(a.z[row * a.ld_z + c]);
@@ -1142,7 +1261,12 @@ template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Arg
   }
   return PRAD_OK;
 }
-template <typename T> static prad_status pick(prad_ctx* ctx, const Args<T>& a, Pass pass) {
+template <typename T> static prad_status pick(prad_ctx* ctx, Args<T> a, Pass pass) {
+  constexpr int V = 16 / sizeof(T);
+  const uintptr_t all = (uintptr_t)a.u | (uintptr_t)a.delta | (uintptr_t)a.z | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.du |
+                        (uintptr_t)a.ddelta | (uintptr_t)a.dz;
+  const int64_t pitches = a.ld_u | a.ld_delta | a.ld_z | a.ld_y | a.ld_dy | a.ld_du | a.ld_ddelta | a.ld_dz;
+  a.wide = (all & 15) == 0 && pitches % V == 0 && (a.groups == 1 || a.per % V == 0);
   if (a.state <= 8) return launch<T, 4, 2>(ctx, a, pass);
   if (a.state <= 16) return launch<T, 4, 4>(ctx, a, pass);
   if (a.state <= 32) return launch<T, 8, 4>(ctx, a, pass);
