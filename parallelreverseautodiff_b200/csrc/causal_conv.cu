@@ -3,8 +3,8 @@
 // where the W - 1 rows before a sequence's first token come from its state (zero without one).  Backward, with g = dy swish'(p):
 //   dx_t = sum_k w[c][k] g_(t + W - 1 - k)  over the tokens of the sequence,  dw[c][k] = sum_t g_t x_(t - (W - 1) + k),  dbias = sum g.
 //
-// Bound by memory: a thread takes V neighbouring channels and walks down a run of tokens with the last W rows in registers, so that
-// a row is read once per run and W - 1 rows twice.
+// Bound by memory: a thread takes V neighbouring channels and walks down a run of tokens with the last W rows in registers and the
+// next four on their way, so that a row is read once per run and W - 1 rows twice.
 #include "common.cuh"
 #include "packed_sequences.cuh"
 
@@ -16,14 +16,16 @@ using seq::swish;
 using seq::swish_slope;
 
 constexpr int LANES = 32, WARPS = 8, THREADS = LANES * WARPS;
-constexpr int RUN = 32;          // tokens of a thread's run
+constexpr int AHEAD = 4;         // rows on their way
 
 template <typename T> struct Args {
   Sequences rows;
   const T *x, *w, *bias, *state, *dy;
   T *y, *dx, *state_out, *dw, *dbias, *dstate;
   int64_t ld_x, ld_y, ld_dy, ld_dx;
-  int dim, swish;
+  int dim, swish, wide_w;        // wide_w: w can be read V values at a time
+  int run;                       // tokens of a thread's run
+  unsigned blocks;               // CTAs along the tokens; those behind them see to the states
 };
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
@@ -43,23 +45,52 @@ __device__ __forceinline__ Pack<T, V> row_at(const Args<T>& a, int s, int64_t st
 template <typename T, int V, int W> struct Weights {
   T w[W][V], bias[V];
   __device__ __forceinline__ Weights(const Args<T>& a, int c) {
+    T all[W * V];                // V rows of w, which lie one behind the other
+    if (a.wide_w) {
+#pragma unroll
+      for (int i = 0; i < W * V; i += V) {
+        const Pack<T, V> r = load<T, V>(a.w + (int64_t)c * W + i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) all[i + j] = r.v[j];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < W * V; ++i) all[i] = a.w[(int64_t)c * W + i];
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) w[k][j] = a.w[(int64_t)(c + j) * W + k];
+      for (int k = 0; k < W; ++k) w[k][j] = all[j * W + k];
       bias[j] = a.bias ? a.bias[c + j] : (T)0;
     }
   }
 };
 
+// state_out[s] = the last W - 1 rows of state[s] followed by the sequence's tokens
+template <typename T, int V, int W>
+__device__ __forceinline__ void final_states(const Args<T>& a, int64_t block) {
+  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
+  const int64_t i = block * WARPS + (threadIdx.x >> 5);
+  if (c >= a.dim || i >= (int64_t)a.rows.count * (W - 1)) return;
+  const int s = (int)(i / (W - 1)), k = (int)(i % (W - 1));
+  const int64_t start = a.rows.start(s);
+  int64_t len = a.rows.end(s) - start;
+  if (len < 0) len = 0;
+  *reinterpret_cast<Pack<T, V>*>(a.state_out + i * a.dim + c) = row_at<T, V, W>(a, s, start, len - (W - 1) + k, c);
+}
+
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(THREADS)
 forward_kernel(const Args<T> a) {
+  if (blockIdx.x >= a.blocks) {
+    if constexpr (W > 1) final_states<T, V, W>(a, blockIdx.x - a.blocks);
+    return;
+  }
   const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
   if (c >= a.dim) return;
   const int64_t run = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
   const int64_t lo = a.rows.begin(), hi = a.rows.finish();
-  int64_t t = run * RUN, last = t + RUN;
+  int64_t t = run * a.run, last = t + a.run;
   if (t < lo) t = lo;
   if (last > hi) last = hi;
   if (t >= last) return;
@@ -70,44 +101,46 @@ forward_kernel(const Args<T> a) {
   Pack<T, V> x[W];              // x[W - 1]: the newest row
 #pragma unroll
   for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, t - start - (W - k), c);
-  Pack<T, V> next = load<T, V>(a.x + t * a.ld_x + c);
-  for (; t < last; ++t) {
-    if (t == end) {
-      do ++s; while (s < a.rows.count && a.rows.end(s) <= t);
-      if (s >= a.rows.count) return;
-      start = t;
-      end = a.rows.end(s);
+  Pack<T, V> next[AHEAD];
+  const T* px = a.x + t * a.ld_x + c;
+  T* py = a.y + t * a.ld_y + c;
 #pragma unroll
-      for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, -(W - k), c);
+  for (int i = 0; i < AHEAD; ++i)
+    if (t + i < last) next[i] = load<T, V>(px + i * a.ld_x);
+  while (t < last) {
+    Pack<T, V> now[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) now[i] = next[i];
+    px += AHEAD * a.ld_x;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (t + AHEAD + i < last) next[i] = load<T, V>(px + i * a.ld_x);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (t == end) {
+        do ++s; while (s < a.rows.count && a.rows.end(s) <= t);
+        if (s >= a.rows.count) return;
+        start = t;
+        end = a.rows.end(s);
+#pragma unroll
+        for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, -(W - k), c);
+      }
+#pragma unroll
+      for (int k = 0; k + 1 < W; ++k) x[k] = x[k + 1];
+      x[W - 1] = now[i];
+      Pack<T, V> y;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        T p = wt.bias[j];
+#pragma unroll
+        for (int k = 0; k < W; ++k) p += wt.w[k][j] * x[k].v[j];
+        y.v[j] = a.swish ? swish(p) : p;
+      }
+      *reinterpret_cast<Pack<T, V>*>(py) = y;
+      py += a.ld_y;
+      if (++t == last) return;
     }
-#pragma unroll
-    for (int k = 0; k + 1 < W; ++k) x[k] = x[k + 1];
-    x[W - 1] = next;
-    if (t + 1 < last) next = load<T, V>(a.x + (t + 1) * a.ld_x + c);
-    Pack<T, V> y;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      T p = wt.bias[j];
-#pragma unroll
-      for (int k = 0; k < W; ++k) p += wt.w[k][j] * x[k].v[j];
-      y.v[j] = a.swish ? swish(p) : p;
-    }
-    *reinterpret_cast<Pack<T, V>*>(a.y + t * a.ld_y + c) = y;
   }
-}
-
-// state_out[s] = the last W - 1 rows of state[s] followed by the sequence's tokens
-template <typename T, int V, int W>
-__global__ void __launch_bounds__(THREADS)
-state_kernel(const Args<T> a) {
-  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
-  const int64_t i = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (c >= a.dim || i >= (int64_t)a.rows.count * (W - 1)) return;
-  const int s = (int)(i / (W - 1)), k = (int)(i % (W - 1));
-  const int64_t start = a.rows.start(s);
-  int64_t len = a.rows.end(s) - start;
-  if (len < 0) len = 0;
-  *reinterpret_cast<Pack<T, V>*>(a.state_out + i * a.dim + c) = row_at<T, V, W>(a, s, start, len - (W - 1) + k, c);
 }
 
 // g at place q of a sequence
@@ -125,17 +158,57 @@ __device__ __forceinline__ void slope(const Weights<T, V, W>& wt, const Pack<T, 
   }
 }
 
+// dstate[s][i], the row at place i - (W - 1): sum over the places q <= i of the sequence of w[i - q] g_q
+template <typename T, int V, int W>
+__device__ __forceinline__ void state_gradients(const Args<T>& a, int64_t block) {
+  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
+  const int64_t s64 = block * WARPS + (threadIdx.x >> 5);
+  if (c >= a.dim || s64 >= a.rows.count) return;
+  const int s = (int)s64;
+  const int64_t start = a.rows.start(s), len = a.rows.end(s) - start;
+  const Weights<T, V, W> wt(a, c);
+  T sum[W][V];
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[i][j] = 0;
+#pragma unroll
+  for (int q = 0; q < W - 1; ++q)
+    if (q < len) {
+      Pack<T, V> x[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, q - (W - 1) + k, c);
+      T g[V];
+      slope<T, V, W>(wt, x, load<T, V>(a.dy + (start + q) * a.ld_dy + c), a.swish, g);
+#pragma unroll
+      for (int i = q; i < W - 1; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[i][j] += wt.w[i - q][j] * g[j];
+    }
+#pragma unroll
+  for (int i = 0; i < W - 1; ++i) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = sum[i][j];
+    *reinterpret_cast<Pack<T, V>*>(a.dstate + ((int64_t)s * (W - 1) + i) * a.dim + c) = o;
+  }
+}
+
 // A thread computes g over its run and the W - 1 tokens behind it, and dx of its run from the last W of them.
 // partial[block][W + 1][dim]: sums for dw (k = 0 .. W - 1) and dbias over the block's runs.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(THREADS)
 backward_kernel(const Args<T> a, T* __restrict__ partial) {
+  if (blockIdx.x >= a.blocks) {
+    if constexpr (W > 1) state_gradients<T, V, W>(a, blockIdx.x - a.blocks);
+    return;
+  }
   __shared__ T part[WARPS][LANES * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = (blockIdx.y * LANES + lane) * V;
   const bool on = c < a.dim;
   const int64_t lo = a.rows.begin(), hi = a.rows.finish();
-  int64_t t = ((int64_t)blockIdx.x * WARPS + warp) * RUN, last = t + RUN;
+  int64_t t = ((int64_t)blockIdx.x * WARPS + warp) * a.run, last = t + a.run;
   if (t < lo) t = lo;
   if (last > hi) last = hi;
   T dw[W][V], db[V];
@@ -163,46 +236,63 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
       for (int k = 0; k < W; ++k)
 #pragma unroll
         for (int j = 0; j < V; ++j) g[k][j] = 0;
-      Pack<T, V> nx, nd;
-      if (t < ahead) {
-        nx = load<T, V>(a.x + t * a.ld_x + c);
-        nd = load<T, V>(a.dy + t * a.ld_dy + c);
-      }
-      for (int64_t q = t; q < stop + W - 1; ++q) {
+      const T *px = a.x + t * a.ld_x + c, *pd = a.dy + t * a.ld_dy + c;
+      T* po = a.dx + t * a.ld_dx + c;
+      const int all = (int)(stop - t) + W - 1, taken = (int)(ahead - t), own = (int)(stop - t);
+      Pack<T, V> nx[AHEAD], nd[AHEAD];
 #pragma unroll
-        for (int k = 0; k + 1 < W; ++k) {
-          x[k] = x[k + 1];
-#pragma unroll
-          for (int j = 0; j < V; ++j) g[k][j] = g[k + 1][j];
+      for (int i = 0; i < AHEAD; ++i)
+        if (i < taken) {
+          nx[i] = load<T, V>(px + i * a.ld_x);
+          nd[i] = load<T, V>(pd + i * a.ld_dy);
         }
-        if (q < ahead) {
-          x[W - 1] = nx;
-          const Pack<T, V> d = nd;
-          if (q + 1 < ahead) {
-            nx = load<T, V>(a.x + (q + 1) * a.ld_x + c);
-            nd = load<T, V>(a.dy + (q + 1) * a.ld_dy + c);
+      for (int q0 = 0; q0 < all; q0 += AHEAD) {
+        Pack<T, V> cx[AHEAD], cd[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) cx[i] = nx[i], cd[i] = nd[i];
+        px += AHEAD * a.ld_x;
+        pd += AHEAD * a.ld_dy;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          if (q0 + AHEAD + i < taken) {
+            nx[i] = load<T, V>(px + i * a.ld_x);
+            nd[i] = load<T, V>(pd + i * a.ld_dy);
           }
-          slope<T, V, W>(wt, x, d, a.swish, g[W - 1]);
-          if (q < stop)
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const int q = q0 + i;
+          if (q >= all) break;
+#pragma unroll
+          for (int k = 0; k + 1 < W; ++k) {
+            x[k] = x[k + 1];
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[k][j] = g[k + 1][j];
+          }
+          if (q < taken) {
+            x[W - 1] = cx[i];
+            slope<T, V, W>(wt, x, cd[i], a.swish, g[W - 1]);
+            if (q < own)
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                db[j] += g[W - 1][j];
+#pragma unroll
+                for (int k = 0; k < W; ++k) dw[k][j] += g[W - 1][j] * x[k].v[j];
+              }
+          } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[W - 1][j] = 0;
+          }
+          if (q >= W - 1) {                                    // g[k] belongs to the token W - 1 - k before q
+            Pack<T, V> dx;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              db[j] += g[W - 1][j];
+              dx.v[j] = 0;
 #pragma unroll
-              for (int k = 0; k < W; ++k) dw[k][j] += g[W - 1][j] * x[k].v[j];
+              for (int k = 0; k < W; ++k) dx.v[j] += wt.w[W - 1 - k][j] * g[k][j];
             }
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) g[W - 1][j] = 0;
-        }
-        if (q - (W - 1) >= t) {                                // g[k] belongs to token q - (W - 1) + k
-          Pack<T, V> dx;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            dx.v[j] = 0;
-#pragma unroll
-            for (int k = 0; k < W; ++k) dx.v[j] += wt.w[W - 1 - k][j] * g[k][j];
+            *reinterpret_cast<Pack<T, V>*>(po) = dx;
+            po += a.ld_dx;
           }
-          *reinterpret_cast<Pack<T, V>*>(a.dx + (q - (W - 1)) * a.ld_dx + c) = dx;
         }
       }
       t = stop;
@@ -249,43 +339,6 @@ totals_kernel(const T* __restrict__ partial, int64_t blocks, int dim, int width,
   }
 }
 
-// dstate[s][i], the row at place i - (W - 1): sum over the places q <= i of the sequence of w[i - q] g_q
-template <typename T, int V, int W>
-__global__ void __launch_bounds__(THREADS)
-state_gradient_kernel(const Args<T> a) {
-  const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
-  const int64_t s64 = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (c >= a.dim || s64 >= a.rows.count) return;
-  const int s = (int)s64;
-  const int64_t start = a.rows.start(s), len = a.rows.end(s) - start;
-  const Weights<T, V, W> wt(a, c);
-  T sum[W][V];
-#pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum[i][j] = 0;
-#pragma unroll
-  for (int q = 0; q < W - 1; ++q)
-    if (q < len) {
-      Pack<T, V> x[W];
-#pragma unroll
-      for (int k = 0; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, q - (W - 1) + k, c);
-      T g[V];
-      slope<T, V, W>(wt, x, load<T, V>(a.dy + (start + q) * a.ld_dy + c), a.swish, g);
-#pragma unroll
-      for (int i = q; i < W - 1; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum[i][j] += wt.w[i - q][j] * g[j];
-    }
-#pragma unroll
-  for (int i = 0; i < W - 1; ++i) {
-    Pack<T, V> o;
-#pragma unroll
-    for (int j = 0; j < V; ++j) o.v[j] = sum[i][j];
-    *reinterpret_cast<Pack<T, V>*>(a.dstate + ((int64_t)s * (W - 1) + i) * a.dim + c) = o;
-  }
-}
-
 // one new row of each sequence; state_out may be the state itself
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(THREADS)
@@ -314,64 +367,68 @@ step_kernel(const Args<T> a, int64_t batch) {
 // ---------------------------------------------------------------- launches
 enum class Pass { Forward, Backward, Step };
 
-template <typename T, int V, int W> static prad_status launch(prad_ctx* ctx, const Args<T>& a, Pass pass) {
+template <typename T, int V, int W, bool BACKWARD> static prad_status launch(prad_ctx* ctx, Args<T> a, Pass pass) {
   const unsigned across = (unsigned)ceil_div(a.dim, LANES * V);
-  if (pass == Pass::Step) {
+  if (!BACKWARD && pass == Pass::Step) {
     step_kernel<T, V, W><<<dim3((unsigned)ceil_div(a.rows.tokens, WARPS), across), THREADS, 0, ctx->stream>>>(a, a.rows.tokens);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
-  const int64_t blocks = ceil_div(a.rows.tokens, WARPS * RUN);
-  const dim3 grid((unsigned)blocks, across);
-  if (pass == Pass::Forward) {
-    if (blocks) {
-      forward_kernel<T, V, W><<<grid, THREADS, 0, ctx->stream>>>(a);
+  // Runs of 32 tokens, or shorter ones where those give less than two CTAs an SM (2047 tokens of 333 doubles, backward: 26 us with
+  // runs of 32, SHORT_US with runs of 8).
+  a.run = 32;
+  while (a.run > 8 && ceil_div(a.rows.tokens, WARPS * a.run) * across < 2 * ctx->sm_count) a.run /= 2;
+  a.blocks = (unsigned)ceil_div(a.rows.tokens, WARPS * a.run);
+  if constexpr (!BACKWARD) {
+    const int64_t rows = W > 1 && a.state_out ? (int64_t)a.rows.count * (W - 1) : 0;
+    const unsigned grid = a.blocks + (unsigned)ceil_div(rows, WARPS);
+    if (grid) {
+      forward_kernel<T, V, W><<<dim3(grid, across), THREADS, 0, ctx->stream>>>(a);
       PRAD_LAUNCHED(ctx);
     }
-    if (W > 1 && a.state_out && a.rows.count) {
-      state_kernel<T, V, W><<<dim3((unsigned)ceil_div((int64_t)a.rows.count * (W - 1), WARPS), across), THREADS, 0, ctx->stream>>>(a);
+    return PRAD_OK;
+  } else {
+    prad_status st = ensure_workspace(ctx, (size_t)(a.blocks ? a.blocks : 1) * (W + 1) * a.dim * sizeof(T));
+    if (st) return st;
+    const bool states = W > 1 && a.dstate && a.rows.count;
+    if (a.blocks) {
+      const unsigned grid = a.blocks + (states ? (unsigned)ceil_div(a.rows.count, WARPS) : 0);
+      backward_kernel<T, V, W><<<dim3(grid, across), THREADS, 0, ctx->stream>>>(a, (T*)ctx->ws);
+      PRAD_LAUNCHED(ctx);
+    } else if (states) {
+      PRAD_CUDA(cudaMemsetAsync(a.dstate, 0, (size_t)a.rows.count * (W - 1) * a.dim * sizeof(T), ctx->stream));
+    }
+    if (a.dw || a.dbias) {
+      totals_kernel<T><<<dim3((unsigned)ceil_div(a.dim, LANES), W + 1), THREADS, 0, ctx->stream>>>((const T*)ctx->ws, a.blocks, a.dim, W,
+                                                                                                a.dw, a.dbias);
       PRAD_LAUNCHED(ctx);
     }
     return PRAD_OK;
   }
-  prad_status st = ensure_workspace(ctx, (size_t)(blocks ? blocks : 1) * (W + 1) * a.dim * sizeof(T));
-  if (st) return st;
-  if (blocks) {
-    backward_kernel<T, V, W><<<grid, THREADS, 0, ctx->stream>>>(a, (T*)ctx->ws);
-    PRAD_LAUNCHED(ctx);
-  }
-  if (a.dw || a.dbias) {
-    totals_kernel<T><<<dim3((unsigned)ceil_div(a.dim, LANES), W + 1), THREADS, 0, ctx->stream>>>((const T*)ctx->ws, blocks, a.dim, W,
-                                                                                              a.dw, a.dbias);
-    PRAD_LAUNCHED(ctx);
-  }
-  if (W > 1 && a.dstate && a.rows.count && !blocks) {
-    PRAD_CUDA(cudaMemsetAsync(a.dstate, 0, (size_t)a.rows.count * (W - 1) * a.dim * sizeof(T), ctx->stream));
-  } else if (W > 1 && a.dstate && a.rows.count) {
-    state_gradient_kernel<T, V, W><<<dim3((unsigned)ceil_div(a.rows.count, WARPS), across), THREADS, 0, ctx->stream>>>(a);
-    PRAD_LAUNCHED(ctx);
-  }
-  return PRAD_OK;
 }
-template <typename T, int V> static prad_status pick(prad_ctx* ctx, const Args<T>& a, Pass pass, int width) {
+template <typename T, int V, bool BACKWARD> static prad_status pick(prad_ctx* ctx, const Args<T>& a, Pass pass, int width) {
   switch (width) {
-    case 1: return launch<T, V, 1>(ctx, a, pass);
-    case 2: return launch<T, V, 2>(ctx, a, pass);
-    case 3: return launch<T, V, 3>(ctx, a, pass);
-    case 4: return launch<T, V, 4>(ctx, a, pass);
-    case 5: return launch<T, V, 5>(ctx, a, pass);
-    case 6: return launch<T, V, 6>(ctx, a, pass);
-    case 7: return launch<T, V, 7>(ctx, a, pass);
-    default: return launch<T, V, 8>(ctx, a, pass);
+    case 1: return launch<T, V, 1, BACKWARD>(ctx, a, pass);
+    case 2: return launch<T, V, 2, BACKWARD>(ctx, a, pass);
+    case 3: return launch<T, V, 3, BACKWARD>(ctx, a, pass);
+    case 4: return launch<T, V, 4, BACKWARD>(ctx, a, pass);
+    case 5: return launch<T, V, 5, BACKWARD>(ctx, a, pass);
+    case 6: return launch<T, V, 6, BACKWARD>(ctx, a, pass);
+    case 7: return launch<T, V, 7, BACKWARD>(ctx, a, pass);
+    default: return launch<T, V, 8, BACKWARD>(ctx, a, pass);
   }
 }
 template <typename T> static prad_status run(prad_ctx* ctx, const Args<T>& a, Pass pass, int width) {
-  constexpr int V = 16 / sizeof(T);
+  // Eight bytes a thread in the backward pass: with sixteen its windows, sums and weights leave room for half of the threads.
+  const int bytes = pass == Pass::Backward ? 8 : 16;
   const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.dx | (uintptr_t)a.state |
                         (uintptr_t)a.state_out | (uintptr_t)a.dstate;
   const int64_t pitches = a.dim | a.ld_x | a.ld_y | a.ld_dy | a.ld_dx;
-  if ((all & 15) == 0 && pitches % V == 0) return pick<T, V>(ctx, a, pass, width);
-  return pick<T, 1>(ctx, a, pass, width);
+  const bool vector = all % bytes == 0 && pitches * (int64_t)sizeof(T) % bytes == 0;
+  Args<T> b = a;
+  b.wide_w = vector && (uintptr_t)a.w % bytes == 0;
+  if (pass == Pass::Backward) return vector ? pick<T, 8 / sizeof(T), true>(ctx, b, pass, width) : pick<T, 1, true>(ctx, b, pass, width);
+  return vector ? pick<T, 16 / sizeof(T), false>(ctx, b, pass, width) : pick<T, 1, false>(ctx, b, pass, width);
 }
 
 static prad_status check(const char* who, prad_dtype dt, int64_t tokens, int sequences, const void* offsets, int dim, int width) {

@@ -2,11 +2,14 @@
 // all positions of a sample,  xhat = (x - mean) rstd,  v = gamma xhat + beta,  y = v or swish(v).  Backward, with dv = dy swish'(v):
 //   dbeta = sum dv,  dgamma = sum dv xhat,  dx = rstd (gamma dv - mean(gamma dv) - xhat mean(gamma dv xhat)).
 //
-// Two shapes of work.  One position per sample (a norm per token): a group's values lie side by side and stay in the registers of
-// a few lanes, one pass over the memory each way.  Several positions: the rows of a sample are cut into blocks, sums of the blocks
-// first, then a pass that reads the values again.
+// Bound by memory; three shapes of work.  One position per sample (a norm per token): a group's values lie side by side and stay in
+// the registers of a few lanes, one pass over the memory each way.  Several positions: a cluster of CTAs takes a sample (or some of
+// its groups), each CTA a block of its positions; they sum, exchange the sums through each other's shared memory and read their
+// blocks again, now out of the L2.  Too few samples for that, or groups wider than a CTA: sums and results in launches of their own.
 // Means and variances are summed around a pivot out of the data (the average of the group's first values), so that a mean far
 // from zero takes nothing from the variance; sums go from float to double every few values.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "packed_sequences.cuh"
 
@@ -27,8 +30,12 @@ template <typename T> struct Args {
   int act;
 };
 
+__host__ __device__ inline int64_t ceil_rounds(int64_t n, int64_t by) { return (n + by - 1) / by; }
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+
+__device__ __forceinline__ float inverse_root(float x) { return rsqrtf(x); }
+__device__ __forceinline__ double inverse_root(double x) { return 1.0 / sqrt(x); }
 
 // ---------------------------------------------------------------- one position per sample
 // LW lanes share the values of a (sample, group), E packs of V values each; a lane keeps its channels for all its samples, so the
@@ -43,61 +50,72 @@ template <int LW, typename A> __device__ __forceinline__ A lanes_sum(A v) {
 template <typename T, int V, int LW, int E>
 __global__ void __launch_bounds__(THREADS)
 rows_forward_kernel(const Args<T> a, int64_t slots) {
+  constexpr int R = E == 1 ? 4 : E == 2 ? 2 : 1;       // samples whose values are on their way at a time
   const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
   const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
   const int64_t step = slots / a.groups;
   int c[E];
   bool on[E];
+  Pack<T, V> gamma[E], beta[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     c[e] = (l + e * LW) * V;
     on[e] = c[e] < a.per;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      gamma[e].v[j] = on[e] && a.gamma ? a.gamma[g * a.per + c[e] + j] : (T)1;
+      beta[e].v[j] = on[e] && a.beta ? a.beta[g * a.per + c[e] + j] : (T)0;
+    }
   }
   // all lanes of a warp take part in its sums: those beyond the last sample with nothing to add
   const int64_t first = slot < slots ? slot / a.groups : a.samples;
-  const int64_t rounds = (a.samples + step - 1) / step;
+  const int64_t rounds = ceil_rounds(a.samples, step * R);
   for (int64_t k = 0; k < rounds; ++k) {
-    const int64_t s = first + k * step;
-    const bool live = s < a.samples;
-    const T* row = a.x + s * a.channels + (int64_t)g * a.per;
-    Pack<T, V> x[E];
-    T sum = 0;
+    Pack<T, V> x[R][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[e].v[j] = 0;
-      if (live && on[e]) x[e] = load<T, V>(row + c[e]);
+      for (int e = 0; e < E; ++e) {
+        const int64_t s = first + (k * R + r) * step;
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum += x[e].v[j];
-    }
-    const T mean = lanes_sum<LW>(sum) / (T)a.per;
-    T sq = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const T d = x[e].v[j] - mean;
-        if (on[e]) sq += d * d;
+        for (int j = 0; j < V; ++j) x[r][e].v[j] = 0;
+        if (s < a.samples && on[e]) x[r][e] = load<T, V>(a.x + s * a.channels + (int64_t)g * a.per + c[e]);
       }
-    const T var = lanes_sum<LW>(sq) / (T)a.per;
-    const T rstd = (T)(1.0 / sqrt((double)var + a.eps));
-    if (!live) continue;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (on[e]) {
-        const int ch = g * a.per + c[e];
+    for (int r = 0; r < R; ++r) {
+      const int64_t s = first + (k * R + r) * step;
+      T sum = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += x[r][e].v[j];
+      const T mean = lanes_sum<LW>(sum) / (T)a.per;
+      T sq = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          T v = (x[e].v[j] - mean) * rstd;
-          if (a.gamma) v *= a.gamma[ch + j];
-          if (a.beta) v += a.beta[ch + j];
-          x[e].v[j] = a.act ? swish(v) : v;
+          const T d = x[r][e].v[j] - mean;
+          if (on[e]) sq += d * d;
         }
-        *reinterpret_cast<Pack<T, V>*>(a.y + s * a.channels + ch) = x[e];
+      const T var = lanes_sum<LW>(sq) / (T)a.per;
+      const T rstd = inverse_root(var + (T)a.eps);
+      if (s < a.samples) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (on[e]) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const T v = (x[r][e].v[j] - mean) * rstd * gamma[e].v[j] + beta[e].v[j];
+              x[r][e].v[j] = a.act ? swish(v) : v;
+            }
+            *reinterpret_cast<Pack<T, V>*>(a.y + s * a.channels + g * a.per + c[e]) = x[r][e];
+          }
+        if (l == 0) {
+          a.mean_out[s * a.groups + g] = mean;
+          a.rstd_out[s * a.groups + g] = rstd;
+        }
       }
-    if (l == 0) {
-      a.mean_out[s * a.groups + g] = mean;
-      a.rstd_out[s * a.groups + g] = rstd;
     }
   }
 }
@@ -181,10 +199,11 @@ rows_backward_kernel(const Args<T> a, int64_t slots, T* __restrict__ partial) {
 }
 
 // out[0][c], out[1][c] = sums over the blocks of partial[block][2][channels], in the order of the blocks within a warp's share
+constexpr int TOTALS = 1024;
 template <typename P, typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(TOTALS)
 column_totals_kernel(const P* __restrict__ partial, int64_t blocks, int channels, T* dgamma, T* dbeta) {
-  __shared__ double part[THREADS / 32][32];
+  __shared__ double part[TOTALS / 32][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   T* out = blockIdx.y ? dbeta : dgamma;
@@ -193,21 +212,21 @@ column_totals_kernel(const P* __restrict__ partial, int64_t blocks, int channels
   if (c < channels) {
     const P* p = partial + (int64_t)blockIdx.y * channels + c;
 #pragma unroll 8
-    for (int64_t b = w; b < blocks; b += THREADS / 32) sum += (double)p[b * 2 * channels];
+    for (int64_t b = w; b < blocks; b += TOTALS / 32) sum += (double)p[b * 2 * channels];
   }
   part[w][lane] = sum;
   __syncthreads();
   if (w == 0 && c < channels) {
     sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < THREADS / 32; ++k) sum += part[k][lane];
+    for (int k = 0; k < TOTALS / 32; ++k) sum += part[k][lane];
     out[c] = (T)sum;
   }
 }
 
 // ---------------------------------------------------------------- several positions per sample
 // A CTA takes a block of positions of one sample and a part of the channels: as many whole groups as THREADS packs of V channels
-// hold, the threads in rows of one position each; or one wide group, whose packs the threads walk.
+// hold (so at most THREADS), the threads in rows of one position each; or one wide group, whose packs the threads walk.
 struct Parts {
   int64_t blocks, rows;        // blocks of `rows` positions per sample
   int parts, groups_each;      // of the channels
@@ -231,31 +250,30 @@ template <typename T> struct Place {
   }
 };
 
+// the average of four values of a group
 template <typename T> __device__ __forceinline__ double pivot(const Args<T>& a, int64_t s, int g) {
   const T* x = a.x + s * a.positions * a.channels + (int64_t)g * a.per;
-  const int across = a.per < 32 ? a.per : 32;
-  const int down = (int)(32 / across < a.positions ? 32 / across : a.positions);
   double sum = 0.0;
-  for (int p = 0; p < down; ++p)
-    for (int c = 0; c < across; ++c) sum += (double)x[(int64_t)p * a.channels + c];
-  return (double)(T)(sum / (across * down));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sum += (double)x[(a.positions - 1) * k / 3 * a.channels + (a.per - 1) * k / 3];
+  return (double)(T)(sum * 0.25);
 }
 
 constexpr int RUN = 8;     // positions that are summed in T before they go into a double
 
-// sums[sample][block][group][2] = sums of x - pivot and of its square
-template <typename T, int V>
-__global__ void __launch_bounds__(THREADS)
-block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
-  __shared__ double part[THREADS][2];
-  __shared__ T piv[THREADS * V + 1];
-  const Place<T> w(a, k, V);
-  for (int g = threadIdx.x; g < w.g1 - w.g0; g += THREADS) piv[g] = (T)pivot(a, w.s, w.g0 + g);
+// sums of x - pivot and of its square over the CTA's block, for each of its groups, to `out(group, s1, s2)`
+template <typename T, int V> struct SumsShared {
+  double part[THREADS][2];
+  T piv[THREADS];
+};
+template <typename T, int V, typename Out>
+__device__ __forceinline__ void block_sums(const Args<T>& a, const Place<T>& w, SumsShared<T, V>& m, const Out& out) {
+  for (int g = threadIdx.x; g < w.g1 - w.g0; g += THREADS) m.piv[g] = (T)pivot(a, w.s, w.g0 + g);
   __syncthreads();
   double s1 = 0.0, s2 = 0.0;
   if (w.ty < w.rows)
     for (int q = w.tx; q < w.packs; q += THREADS) {
-      const T m = piv[q * V / a.per];
+      const T k = m.piv[q * V / a.per];
       const T* x = a.x + (w.s * a.positions) * a.channels + w.c0 + (int64_t)q * V;
       for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)RUN * w.rows) {
         T r1 = 0, r2 = 0;
@@ -264,14 +282,14 @@ block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
         for (int i = 0; i < RUN; ++i) {
           const int64_t at = p + (int64_t)i * w.rows;
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[i].v[j] = m;
+          for (int j = 0; j < V; ++j) v[i].v[j] = k;
           if (at < w.p1) v[i] = load<T, V>(x + at * a.channels);
         }
 #pragma unroll
         for (int i = 0; i < RUN; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const T d = v[i].v[j] - m;
+            const T d = v[i].v[j] - k;
             r1 += d;
             r2 += d * d;
           }
@@ -279,8 +297,8 @@ block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
         s2 += (double)r2;
       }
     }
-  part[threadIdx.x][0] = s1;
-  part[threadIdx.x][1] = s2;
+  m.part[threadIdx.x][0] = s1;
+  m.part[threadIdx.x][1] = s2;
   __syncthreads();
   // a warp adds up one group: its packs of every row of threads, lanes in a fixed order
   const int lane = threadIdx.x & 31, width = w.packs < THREADS ? w.packs : THREADS;
@@ -289,17 +307,34 @@ block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
     s1 = s2 = 0.0;
     for (int i = lane; i < each * w.rows; i += 32) {
       const int t = i / each * width + g * each + i % each;
-      s1 += part[t][0];
-      s2 += part[t][1];
+      s1 += m.part[t][0];
+      s2 += m.part[t][1];
     }
     s1 = lanes_sum<32>(s1);
     s2 = lanes_sum<32>(s2);
-    if (lane == 0) {
-      double* to = sums + ((w.s * k.blocks + w.block) * a.groups + w.g0 + g) * 2;
-      to[0] = s1;
-      to[1] = s2;
-    }
+    if (lane == 0) out(g, s1, s2);
   }
+}
+template <typename T>
+__device__ __forceinline__ void statistics(const Args<T>& a, double pivot, double s1, double s2, T& mean, T& rstd) {
+  const double n = (double)a.positions * a.per, m = s1 / n;
+  double var = s2 / n - m * m;
+  if (var < 0.0) var = 0.0;        // (a NaN stays)
+  mean = (T)(pivot + m);
+  rstd = (T)(1.0 / sqrt(var + a.eps));
+}
+
+// sums[sample][block][group][2]
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
+  __shared__ SumsShared<T, V> m;
+  const Place<T> w(a, k, V);
+  block_sums(a, w, m, [&](int g, double s1, double s2) {
+    double* to = sums + ((w.s * k.blocks + w.block) * a.groups + w.g0 + g) * 2;
+    to[0] = s1;
+    to[1] = s2;
+  });
 }
 
 template <typename T>
@@ -316,22 +351,18 @@ statistics_kernel(const Args<T> a, int64_t blocks, const double* __restrict__ su
     s1 += p[0];
     s2 += p[1];
   }
-  const double n = (double)a.positions * a.per, m = s1 / n;
-  double var = s2 / n - m * m;
-  if (var < 0.0) var = 0.0;        // (a NaN stays)
-  a.mean_out[i] = (T)(pivot(a, s, g) + m);
-  a.rstd_out[i] = (T)(1.0 / sqrt(var + a.eps));
+  statistics(a, pivot(a, s, g), s1, s2, a.mean_out[i], a.rstd_out[i]);
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(THREADS)
-apply_kernel(const Args<T> a, const Parts k) {
-  const Place<T> w(a, k, V);
+// y of the CTA's block; stats(group of the CTA, mean, rstd)
+template <typename T, int V, typename Stats>
+__device__ __forceinline__ void apply(const Args<T>& a, const Place<T>& w, const Stats& stats) {
   if (w.ty >= w.rows) return;
   for (int q = w.tx; q < w.packs; q += THREADS) {
     const int c = w.c0 + q * V;
-    const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
-    const T mean = a.mean[i], rstd = a.rstd[i];
+    const int64_t at = w.s * a.positions * a.channels + c;
+    T mean, rstd;
+    stats(q * V / a.per, mean, rstd);
     T gamma[V], beta[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -356,76 +387,128 @@ apply_kernel(const Args<T> a, const Parts k) {
     }
   }
 }
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+apply_kernel(const Args<T> a, const Parts k) {
+  const Place<T> w(a, k, V);
+  apply<T, V>(a, w, [&](int g, T& mean, T& rstd) {
+    mean = a.mean[w.s * a.groups + w.g0 + g];
+    rstd = a.rstd[w.s * a.groups + w.g0 + g];
+  });
+}
 
-// sums[sample][block][2][channels] = sums of dv xhat and of dv over the block
+// both by one cluster per sample and part: the CTAs' sums through each other's shared memory
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+cluster_forward_kernel(const Args<T> a, const Parts k) {
+  __shared__ union { SumsShared<T, V> sums; T stats[THREADS][2]; } m;
+  __shared__ double own[THREADS][2];
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const Place<T> w(a, k, V);
+  block_sums(a, w, m.sums, [&](int g, double s1, double s2) {
+    own[g][0] = s1;
+    own[g][1] = s2;
+  });
+  cluster.sync();
+  for (int g = threadIdx.x; g < w.g1 - w.g0; g += THREADS) {
+    double s1 = 0.0, s2 = 0.0;
+    for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
+      const double* p = cluster.map_shared_rank(&own[g][0], r);
+      s1 += p[0];
+      s2 += p[1];
+    }
+    T mean, rstd;
+    statistics(a, pivot(a, w.s, w.g0 + g), s1, s2, mean, rstd);
+    m.stats[g][0] = mean;
+    m.stats[g][1] = rstd;
+    if (w.block == 0) {
+      a.mean_out[w.s * a.groups + w.g0 + g] = mean;
+      a.rstd_out[w.s * a.groups + w.g0 + g] = rstd;
+    }
+  }
+  cluster.sync();                  // (no CTA may end while another reads its sums)
+  apply<T, V>(a, w, [&](int g, T& mean, T& rstd) {
+    mean = m.stats[g][0];
+    rstd = m.stats[g][1];
+  });
+}
+
+// Sums of dv xhat and of dv over the CTA's block, per channel of packs q0 .. q0 + THREADS - 1, by the thread of each pack and row.
+template <typename T, int V>
+__device__ __forceinline__ void thread_gradients(const Args<T>& a, const Place<T>& w, int q, double (&sg)[V], double (&sb)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) sg[j] = sb[j] = 0.0;
+  if (w.ty >= w.rows || q >= w.packs) return;
+  const int c = w.c0 + q * V;
+  const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
+  const T mean = a.mean[i], rstd = a.rstd[i];
+  T gamma[V], beta[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
+    beta[j] = a.beta ? a.beta[c + j] : (T)0;
+  }
+  for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
+    Pack<T, V> x[4], d[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (p + (int64_t)r * w.rows < w.p1) {
+        x[r] = load<T, V>(a.x + at + (p + (int64_t)r * w.rows) * a.channels);
+        d[r] = load<T, V>(a.dy + at + (p + (int64_t)r * w.rows) * a.channels);
+      }
+    T rg[V], rb[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) rg[j] = rb[j] = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (p + (int64_t)r * w.rows < w.p1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const T xh = (x[r].v[j] - mean) * rstd;
+          T dv = d[r].v[j];
+          if (a.act) dv *= swish_slope(xh * gamma[j] + beta[j]);
+          rg[j] += dv * xh;
+          rb[j] += dv;
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      sg[j] += (double)rg[j];
+      sb[j] += (double)rb[j];
+    }
+  }
+}
+// Of packs q0 .. q0 + THREADS - 1: the rows of threads added up, part[0 / 1][channel] and sums[sample][block][2][channels].
+template <typename T, int V>
+__device__ __forceinline__ void block_gradients(const Args<T>& a, const Parts& k, const Place<T>& w, int q0, double (*part)[THREADS * V],
+                                                double* __restrict__ sums) {
+  const int width = w.packs < THREADS ? w.packs : THREADS;
+  double sg[V], sb[V];
+  thread_gradients<T, V>(a, w, q0 + w.tx, sg, sb);
+  __syncthreads();
+  if (w.ty < w.rows)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      part[0][(w.ty * width + w.tx) * V + j] = sg[j];
+      part[1][(w.ty * width + w.tx) * V + j] = sb[j];
+    }
+  __syncthreads();
+  const int here = (w.packs - q0 < THREADS ? w.packs - q0 : THREADS) * V;
+  for (int e = threadIdx.x; e < 2 * here; e += THREADS) {
+    const int c = e % here;
+    double sum = 0.0;
+    for (int r = 0; r < w.rows; ++r) sum += part[e / here][r * width * V + c];
+    sums[((w.s * k.blocks + w.block) * 2 + e / here) * a.channels + w.c0 + q0 * V + c] = sum;
+    part[e / here][c] = sum;       // (this thread alone reads and writes row 0 of channel c)
+  }
+  __syncthreads();
+}
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS)
 block_gradients_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
   __shared__ double part[2][THREADS * V];
   const Place<T> w(a, k, V);
-  const int width = w.packs < THREADS ? w.packs : THREADS;
-  for (int q0 = 0; q0 < w.packs; q0 += THREADS) {
-    const int q = q0 + w.tx;
-    const bool on = w.ty < w.rows && q < w.packs;
-    double sg[V], sb[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) sg[j] = sb[j] = 0.0;
-    if (on) {
-      const int c = w.c0 + q * V;
-      const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
-      const T mean = a.mean[i], rstd = a.rstd[i];
-      T gamma[V], beta[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
-        beta[j] = a.beta ? a.beta[c + j] : (T)0;
-      }
-      for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
-        Pack<T, V> x[4], d[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (p + (int64_t)r * w.rows < w.p1) {
-            x[r] = load<T, V>(a.x + at + (p + (int64_t)r * w.rows) * a.channels);
-            d[r] = load<T, V>(a.dy + at + (p + (int64_t)r * w.rows) * a.channels);
-          }
-        T rg[V], rb[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) rg[j] = rb[j] = 0;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (p + (int64_t)r * w.rows < w.p1) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const T xh = (x[r].v[j] - mean) * rstd;
-              T dv = d[r].v[j];
-              if (a.act) dv *= swish_slope(xh * gamma[j] + beta[j]);
-              rg[j] += dv * xh;
-              rb[j] += dv;
-            }
-          }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          sg[j] += (double)rg[j];
-          sb[j] += (double)rb[j];
-        }
-      }
-    }
-    __syncthreads();
-    if (on)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        part[0][(w.ty * width + w.tx) * V + j] = sg[j];
-        part[1][(w.ty * width + w.tx) * V + j] = sb[j];
-      }
-    __syncthreads();
-    const int here = (w.packs - q0 < THREADS ? w.packs - q0 : THREADS) * V;
-    for (int e = threadIdx.x; e < 2 * here; e += THREADS) {
-      const int c = e % here;
-      double sum = 0.0;
-      for (int r = 0; r < w.rows; ++r) sum += part[e / here][r * width * V + c];
-      sums[((w.s * k.blocks + w.block) * 2 + e / here) * a.channels + w.c0 + q0 * V + c] = sum;
-    }
-  }
+  for (int q0 = 0; q0 < w.packs; q0 += THREADS) block_gradients<T, V>(a, k, w, q0, part, sums);
 }
 
 // Per sample and group: mean(gamma dv) and mean(gamma dv xhat) of the whole sample; a warp each.
@@ -454,15 +537,16 @@ group_gradients_kernel(const Args<T> a, int64_t blocks, const double* __restrict
   }
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(THREADS)
-input_gradients_kernel(const Args<T> a, const Parts k, const double* __restrict__ means) {
-  const Place<T> w(a, k, V);
+// dx of the CTA's block; means(group of the CTA, mean(gamma dv), mean(gamma dv xhat))
+template <typename T, int V, typename Means>
+__device__ __forceinline__ void input_gradients(const Args<T>& a, const Place<T>& w, const Means& means) {
   if (w.ty >= w.rows) return;
   for (int q = w.tx; q < w.packs; q += THREADS) {
     const int c = w.c0 + q * V;
     const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
-    const T mean = a.mean[i], rstd = a.rstd[i], s1 = (T)means[i * 2], s2 = (T)means[i * 2 + 1];
+    const T mean = a.mean[i], rstd = a.rstd[i];
+    T s1, s2;
+    means(q * V / a.per, s1, s2);
     T gamma[V], beta[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -492,6 +576,60 @@ input_gradients_kernel(const Args<T> a, const Parts k, const double* __restrict_
     }
   }
 }
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+input_gradients_kernel(const Args<T> a, const Parts k, const double* __restrict__ means) {
+  const Place<T> w(a, k, V);
+  input_gradients<T, V>(a, w, [&](int g, T& s1, T& s2) {
+    const double* p = means + (w.s * a.groups + w.g0 + g) * 2;
+    s1 = (T)p[0];
+    s2 = (T)p[1];
+  });
+}
+
+// both by one cluster per sample and part; sums as above, for dgamma and dbeta
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+cluster_backward_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
+  __shared__ double part[2][THREADS * V];
+  __shared__ double own[THREADS][2];
+  __shared__ T mine[THREADS][2];
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const Place<T> w(a, k, V);
+  block_gradients<T, V>(a, k, w, 0, part, sums);
+  const int lane = threadIdx.x & 31;
+  for (int g = threadIdx.x >> 5; g < w.g1 - w.g0; g += THREADS / 32) {
+    double s1 = 0.0, s2 = 0.0;
+    for (int c = lane; c < a.per; c += 32) {
+      const double gamma = a.gamma ? (double)a.gamma[w.c0 + g * a.per + c] : 1.0;
+      s2 += gamma * part[0][g * a.per + c];
+      s1 += gamma * part[1][g * a.per + c];
+    }
+    s1 = lanes_sum<32>(s1);
+    s2 = lanes_sum<32>(s2);
+    if (lane == 0) {
+      own[g][0] = s1;
+      own[g][1] = s2;
+    }
+  }
+  cluster.sync();
+  const double n = (double)a.positions * a.per;
+  for (int g = threadIdx.x; g < w.g1 - w.g0; g += THREADS) {
+    double s1 = 0.0, s2 = 0.0;
+    for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
+      const double* p = cluster.map_shared_rank(&own[g][0], r);
+      s1 += p[0];
+      s2 += p[1];
+    }
+    mine[g][0] = (T)(s1 / n);
+    mine[g][1] = (T)(s2 / n);
+  }
+  cluster.sync();                  // (no CTA may end while another reads its sums)
+  input_gradients<T, V>(a, w, [&](int g, T& s1, T& s2) {
+    s1 = mine[g][0];
+    s2 = mine[g][1];
+  });
+}
 
 // ---------------------------------------------------------------- launches
 template <typename T, int V> constexpr int most_in_registers() { return 32 * 8 * V; }
@@ -515,7 +653,7 @@ template <typename T, int V, int LW, int E> static prad_status rows(prad_ctx* ct
   rows_backward_kernel<T, V, LW, E><<<(unsigned)grid, THREADS, 0, ctx->stream>>>(a, slots, (T*)ctx->ws);
   PRAD_LAUNCHED(ctx);
   if (a.dgamma || a.dbeta) {
-    column_totals_kernel<T, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), THREADS, 0, ctx->stream>>>((const T*)ctx->ws, per_group,
+    column_totals_kernel<T, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream>>>((const T*)ctx->ws, per_group,
                                                                                                       a.channels, a.dgamma, a.dbeta);
     PRAD_LAUNCHED(ctx);
   }
@@ -532,8 +670,63 @@ template <typename T, int V> static prad_status pick_rows(prad_ctx* ctx, const A
   return rows<T, V, 32, 8>(ctx, a, backward);
 }
 
+// A cluster's CTAs on the device's SMs at the same time (grid.x: a multiple of `ctas`).
+template <typename... P, typename... A>
+static void launch_clusters(void (*kernel)(P...), dim3 grid, unsigned ctas, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = THREADS;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);     // (PRAD_LAUNCHED looks at the error)
+}
+
+// By clusters: up to eight CTAs a sample and part, each with at least 16 values a thread; parts of fewer groups where the CTAs would
+// not fill the device and a row of the part stays 128 bytes or more.  Returns the CTAs of a cluster, or 0 where launches of their own
+// are better: groups wider than a CTA, or so few samples that the clusters leave most of a large input to few SMs.
+template <typename T> static int by_clusters(prad_ctx* ctx, const Args<T>& a, int V, Parts& k) {
+  if (a.per / V > THREADS) return 0;
+  int groups = THREADS * V / a.per < a.groups ? THREADS * V / a.per : a.groups, ctas = 8;
+  while (ctas > 1 && a.positions * groups * a.per < (int64_t)ctas * THREADS * 16) ctas /= 2;
+  while (groups > 1 && a.samples * ctas * ceil_div(a.groups, groups) < 2 * ctx->sm_count &&
+         (int64_t)groups * a.per * (int64_t)sizeof(T) >= 256)
+    groups = (groups + 1) / 2;
+  k.groups_each = groups;
+  k.parts = (int)ceil_div(a.groups, groups);
+  const int64_t total = a.samples * ctas * k.parts;
+  if (total < ctx->sm_count && a.samples * a.positions * a.channels > 1 << 20) return 0;
+  k.rows = ceil_div(a.positions, ctas);
+  k.blocks = ctas;
+  return ctas;
+}
+
 template <typename T, int V> static prad_status blocks(prad_ctx* ctx, Args<T> a, bool backward) {
   Parts k;
+  const int ctas = by_clusters(ctx, a, V, k);
+  if (ctas) {
+    PRAD_REQUIRE(a.samples * ctas <= 0x7fffffff && k.parts <= 65535, PRAD_ERR_UNSUPPORTED, "group norm: too many samples or channels");
+    const dim3 grid((unsigned)(a.samples * ctas), (unsigned)k.parts);
+    if (!backward) {
+      launch_clusters(cluster_forward_kernel<T, V>, grid, ctas, ctx->stream, a, k);
+      PRAD_LAUNCHED(ctx);
+      return PRAD_OK;
+    }
+    prad_status st = ensure_workspace(ctx, (size_t)(a.samples * ctas) * 2 * a.channels * sizeof(double));
+    if (st) return st;
+    launch_clusters(cluster_backward_kernel<T, V>, grid, ctas, ctx->stream, a, k, (double*)ctx->ws);
+    PRAD_LAUNCHED(ctx);
+    if (a.dgamma || a.dbeta) {
+      column_totals_kernel<double, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream>>>(
+          (const double*)ctx->ws, a.samples * ctas, a.channels, a.dgamma, a.dbeta);
+      PRAD_LAUNCHED(ctx);
+    }
+    return PRAD_OK;
+  }
   k.groups_each = THREADS * V / a.per;
   if (k.groups_each < 1) k.groups_each = 1;
   if (k.groups_each > a.groups) k.groups_each = a.groups;
@@ -574,7 +767,7 @@ template <typename T, int V> static prad_status blocks(prad_ctx* ctx, Args<T> a,
   input_gradients_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k, means);
   PRAD_LAUNCHED(ctx);
   if (a.dgamma || a.dbeta) {
-    column_totals_kernel<double, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), THREADS, 0, ctx->stream>>>(
+    column_totals_kernel<double, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream>>>(
         sums, a.samples * k.blocks, a.channels, a.dgamma, a.dbeta);
     PRAD_LAUNCHED(ctx);
   }

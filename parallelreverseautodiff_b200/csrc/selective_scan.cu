@@ -34,7 +34,7 @@ template <typename T> struct Args {
   int64_t span;                 // tokens of a span
   int spans, dim, state, groups, per, blocks;   // per: channels of a group, in `blocks` CTAs
   int softplus;
-  int wide, wide_B, wide_C;     // the token matrices, B and C can be read and written 16 bytes at a time
+  int wide, wide_B, wide_C, wide_h;     // the token matrices, B, C and the matrices of states: 16 bytes at a time
   int64_t ld_u, ld_delta, ld_z, ld_B, ld_C, ld_y, ld_dy, ld_du, ld_ddelta, ld_dz, ld_dB, ld_dC;
   const T *u, *delta, *z, *A, *B, *C, *D, *bias, *h0, *dy;
   T *y, *h_last, *saved;
@@ -176,6 +176,45 @@ template <int L> struct Lanes {
   }
 };
 
+// States n0 .. n0 + S - 1 of a channel in a [dim][state] matrix; those that do not exist are zero.
+template <int S, typename T>
+__device__ __forceinline__ void read_states(const T* m, int channel, int n0, bool on, const Args<T>& a, T (&h)[S]) {
+  constexpr int V = S * sizeof(T) < 16 ? S : 16 / sizeof(T);
+  m += (int64_t)channel * a.state + n0;
+  if (a.wide_h) {
+#pragma unroll
+    for (int j = 0; j < S; j += V) {
+      Pack<T, V> w;
+#pragma unroll
+      for (int i = 0; i < V; ++i) w.v[i] = 0;
+      if (on && n0 + j < a.state) w = *reinterpret_cast<const Pack<T, V>*>(m + j);
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[j + i] = w.v[i];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < S; ++j) h[j] = on && n0 + j < a.state ? m[j] : (T)0;
+  }
+}
+template <int S, typename T>
+__device__ __forceinline__ void write_states(T* m, int channel, int n0, bool on, const Args<T>& a, const T (&h)[S]) {
+  constexpr int V = S * sizeof(T) < 16 ? S : 16 / sizeof(T);
+  m += (int64_t)channel * a.state + n0;
+  if (a.wide_h) {
+#pragma unroll
+    for (int j = 0; j < S; j += V) {
+      Pack<T, V> w;
+#pragma unroll
+      for (int i = 0; i < V; ++i) w.v[i] = h[j + i];
+      if (on && n0 + j < a.state) *reinterpret_cast<Pack<T, V>*>(m + j) = w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+      if (on && n0 + j < a.state) m[j] = h[j];
+  }
+}
+
 // A CTA's channels and a thread's place among them.
 template <typename T, int L, int S> struct Place {
   static constexpr int CH = THREADS / L;
@@ -192,15 +231,8 @@ template <typename T, int L, int S> struct Place {
     on = ch < channels;
   }
   // S states of this thread in a [dim][state] matrix
-  __device__ __forceinline__ void load(const Args<T>& a, const T* m, T (&h)[S]) const {
-#pragma unroll
-    for (int j = 0; j < S; ++j) h[j] = on && n0 + j < a.state ? m[(int64_t)(c0 + ch) * a.state + n0 + j] : (T)0;
-  }
-  __device__ __forceinline__ void store(const Args<T>& a, T* m, const T (&h)[S]) const {
-#pragma unroll
-    for (int j = 0; j < S; ++j)
-      if (on && n0 + j < a.state) m[(int64_t)(c0 + ch) * a.state + n0 + j] = h[j];
-  }
+  __device__ __forceinline__ void load(const Args<T>& a, const T* m, T (&h)[S]) const { read_states<S>(m, c0 + ch, n0, on, a, h); }
+  __device__ __forceinline__ void store(const Args<T>& a, T* m, const T (&h)[S]) const { write_states<S>(m, c0 + ch, n0, on, a, h); }
 };
 
 // Four values a lane, one for each of four tokens, summed over the L lanes of a channel: afterwards lane l holds the sum of token
@@ -352,7 +384,7 @@ template <typename T, int L, int S> struct Forward {
 
 // EDGES: only the state that the span ends in when it begins with zero, and the sum of its time steps.
 template <typename T, int L, int S, bool EDGES>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 4)
 forward_kernel(const Args<T> a) {
   constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -470,13 +502,14 @@ forward_kernel(const Args<T> a) {
       };
 #pragma unroll 2
       for (int t0 = 0; t0 < TT; t0 += 4) {
-        T part[4];
+        T part[4] = {0, 0, 0, 0};
         if (!EDGES && t0 % POINT == 0 && a.saved && t0 >= from && t0 < to) keep(a.saved + (tile0 + t0) / POINT * states);
         if ((starts >> t0 & 15) == 0) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) part[k] = token(t0 + k);
         } else {
-#pragma unroll
+          // (a loop that is not unrolled: what tokens that begin sequences need is little used, and long)
+#pragma unroll 1
           for (int k = 0; k < 4; ++k) {
             if (starts >> (t0 + k) & 1) {
               // the sequence that ends here, and the ones without a token behind it
@@ -489,7 +522,11 @@ forward_kernel(const Args<T> a) {
               end = a.rows.end(s);
               sum = 0;
             }
-            part[k] = token(t0 + k);
+            const T r = token(t0 + k);
+            part[0] = k == 0 ? r : part[0];
+            part[1] = k == 1 ? r : part[1];
+            part[2] = k == 2 ? r : part[2];
+            part[3] = k == 3 ? r : part[3];
           }
         }
         if (!EDGES) {
@@ -567,7 +604,7 @@ template <typename T, int L, int S> struct Edges {
   typename StepOf<T>::type step[TT][CH];        // dt and v
 };
 template <typename T, int L, int S>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 4)
 backward_edges_kernel(const Args<T> a) {
   constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -698,7 +735,7 @@ __device__ __forceinline__ void read_step(const double* m, Two<double>& dt, Two<
 }
 
 template <typename T, int L, int S>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 backward_kernel(const Args<T> a) {
   using K = Backward<T, L, S>;
   constexpr int CC = K::CC, HALF = K::HALF, CH = K::CH, TT = K::TT, N = K::N, P = K::P, FT = K::FT;
@@ -718,7 +755,7 @@ backward_kernel(const Args<T> a) {
   const int64_t begin = span.begin, finish = span.finish;
   const auto load = [&](const T* from, int k, Two<T>(&h)[P]) {       // null: zero
     const int ch = ch0 + k * HALF;
-    T w[S];
+    T w[S];      // (value by value: with the checkpoints read 16 bytes at a time the kernel took 590 us for 540)
 #pragma unroll
     for (int j = 0; j < S; ++j) w[j] = from && ch < channels && n0 + j < a.state ? from[(int64_t)(c0 + ch) * a.state + n0 + j] : (T)0;
 #pragma unroll
@@ -726,14 +763,10 @@ backward_kernel(const Args<T> a) {
   };
   const auto store = [&](T* to, int k, const Two<T>(&h)[P]) {
     const int ch = ch0 + k * HALF;
+    T w[S];
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      T w[2];
-      h[j].get(w[0], w[1]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (ch < channels && n0 + 2 * j + i < a.state) to[(int64_t)(c0 + ch) * a.state + n0 + 2 * j + i] = w[i];
-    }
+    for (int j = 0; j < P; ++j) h[j].get(w[2 * j], w[2 * j + 1]);
+    write_states<S>(to, c0 + ch, n0, ch < channels, a, w);
   };
   Two<T> A[CC][P], e[CC][P], dA[CC][P];
 #pragma unroll
@@ -839,8 +872,7 @@ backward_kernel(const Args<T> a) {
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += 4) {
         T part[CC][4];
-        const auto token = [&](int i) {
-          const int t = t0 + i;
+        const auto token = [&](int t, T(&sums)[CC]) {
           Two<T> B[P], C[P];
           read(&rows_B[t][n0], B);
           read(&rows_C[t][n0], C);
@@ -856,19 +888,29 @@ backward_kernel(const Args<T> a) {
               r = j ? fma(C[j], h[k][j], r) : mul(C[j], h[k][j]);
             }
             m.h[k][t + 1][threadIdx.x] = now;
-            part[k][i] = total(r);
+            sums[k] = total(r);
           }
         };
         if ((starts >> t0 & 15) == 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) token(i);
-        } else {
+          for (int i = 0; i < 4; ++i) {
+            T sums[CC];
+            token(t0 + i, sums);
 #pragma unroll
+            for (int k = 0; k < CC; ++k) part[k][i] = sums[k];
+          }
+        } else {
+#pragma unroll 1
           for (int i = 0; i < 4; ++i) {
             if (starts >> (t0 + i) & 1)
 #pragma unroll
               for (int k = 0; k < CC; ++k) load(initial(t0 + i), k, h[k]);
-            token(i);
+            T sums[CC];
+            token(t0 + i, sums);
+#pragma unroll
+            for (int k = 0; k < CC; ++k)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) part[k][j] = i == j ? sums[k] : part[k][j];
           }
         }
 #pragma unroll
@@ -889,10 +931,9 @@ backward_kernel(const Args<T> a) {
       for (int f = TT - FT; f >= 0; f -= FT) {
 #pragma unroll 1
         for (int t0 = f + FT - 2; t0 >= f; t0 -= 2) {
-          T two[CC][4];
+          T two[CC][4] = {};
           // one token: its gradients from the state in front of it
-          const auto token = [&](int i, const Two<T>(&before)[CC][P]) {
-            const int t = t0 + i;
+          const auto token = [&](int t, const Two<T>(&before)[CC][P], T(&sums)[CC][2]) {
             Two<T> B[P], C[P], dB[P], dC[P];
             read(&rows_B[t][n0], B);
             read(&rows_C[t][n0], C);
@@ -913,8 +954,8 @@ backward_kernel(const Args<T> a) {
                 dB[j] = k ? fma(g, x, dB[j]) : mul(g, x);
                 dC[j] = k ? fma(now[k][j], v, dC[j]) : mul(now[k][j], v);
               }
-              two[k][2 * i] = total(gB);
-              two[k][2 * i + 1] = total(gA);
+              sums[k][0] = total(gB);
+              sums[k][1] = total(gA);
             }
             T rows[2 * S];
 #pragma unroll
@@ -938,31 +979,39 @@ backward_kernel(const Args<T> a) {
           in_front(t0 + 1, one);
           in_front(t0, zero);
           if ((starts >> t0 & 3) == 0) {
-            token(1, one);
+            T sums[2][CC][2];
+            token(t0 + 1, one, sums[1]);
 #pragma unroll
             for (int k = 0; k < CC; ++k)
 #pragma unroll
               for (int j = 0; j < P; ++j) now[k][j] = one[k][j];
-            token(0, zero);
-          } else {
+            token(t0, zero, sums[0]);
 #pragma unroll
+            for (int k = 0; k < CC; ++k)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) two[k][j] = sums[j / 2][k][j % 2];
+          } else {
+#pragma unroll 1
             for (int i = 1; i >= 0; --i) {
               const bool begins = starts >> (t0 + i) & 1;
               Two<T> before[CC][P];
+              T sums[CC][2];
 #pragma unroll
               for (int k = 0; k < CC; ++k) {
 #pragma unroll
                 for (int j = 0; j < P; ++j) before[k][j] = i ? one[k][j] : zero[k][j];
                 if (begins) load(initial(t0 + i), k, before[k]);
               }
-              token(i, before);
+              token(t0 + i, before, sums);
 #pragma unroll
               for (int k = 0; k < CC; ++k) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) two[k][j] = j / 2 == i ? sums[k][j % 2] : two[k][j];
                 if (begins && a.dh0) store(a.dh0 + a.rows.at(tile0 + t0 + i) * states, k, e[k]);
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
                   if (begins) e[k][j] = {(T)0, (T)0};
-                  if (i) now[k][j] = one[k][j];
+                  now[k][j] = one[k][j];
                 }
               }
             }
@@ -1102,35 +1151,53 @@ row_totals_kernel(const Args<T> a) {
 }
 
 // ---------------------------------------------------------------- one token
-// one new token for each row of a batch; h_last may be h0
-template <typename T, int L, int S>
+// One new token for each row of a batch; h_last may be h0.  A thread takes R rows, whose states are all on their way at a time.
+template <typename T, int L, int S, int R>
 __global__ void __launch_bounds__(THREADS)
 step_kernel(const Args<T> a) {
   const Place<T, L, S> me(a);
-  const int64_t row = blockIdx.y;
   const int c = me.c0 + me.ch;
-  T A[S], h[S], sum = 0;
-  me.load(a, a.A, A);
-  me.load(a, a.h0 + row * a.dim * a.state, h);
-  const T u = me.on ? a.u[row * a.ld_u + c] : (T)0;
-  T dt = me.on ? a.delta[row * a.ld_delta + c] : (T)0;
-  if (a.bias && me.on) dt += a.bias[c];
-  if (a.softplus) dt = softplus(dt);
+  const int64_t row0 = (int64_t)blockIdx.y * R, states = (int64_t)a.dim * a.state;
+  T A[S], h[R][S], B[R][S], C[R][S], u[R], dt[R], z[R];
 #pragma unroll
-  for (int j = 0; j < S; ++j) {
-    const bool live = me.on && me.n0 + j < a.state;
-    const T B = live ? a.B[row * a.ld_B + me.q * a.state + me.n0 + j] : (T)0;
-    const T C = live ? a.C[row * a.ld_C + me.q * a.state + me.n0 + j] : (T)0;
-    h[j] = decay(dt * rate(A[j])) * h[j] + dt * u * B;
-    sum += C * h[j];
+  for (int k = 0; k < R; ++k) {
+    const int64_t row = row0 + k;
+    const bool on = me.on && row < a.rows.tokens;
+    read_states<S>(a.h0 + row * states, c, me.n0, on, a, h[k]);
+    u[k] = on ? a.u[row * a.ld_u + c] : (T)0;
+    dt[k] = on ? a.delta[row * a.ld_delta + c] : (T)0;
+    z[k] = on && a.z ? a.z[row * a.ld_z + c] : (T)0;
+    const T *b = a.B + row * a.ld_B + me.q * a.state + me.n0, *g = a.C + row * a.ld_C + me.q * a.state + me.n0;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      const bool live = on && me.n0 + j < a.state;
+      B[k][j] = live ? b[j] : (T)0;
+      C[k][j] = live ? g[j] : (T)0;
+    }
   }
-  me.store(a, a.h_last + row * a.dim * a.state, h);
+  me.load(a, a.A, A);
+  const T bias = a.bias && me.on ? a.bias[c] : (T)0, D = a.D && me.on ? a.D[c] : (T)0;
 #pragma unroll
-  for (int i = 0; i < Lanes<L>::STATE_BITS; ++i) sum += __shfl_xor_sync(0xffffffffu, sum, 1 << Lanes<L>::state_bit(i));
-  if (me.on && me.lane == 0) {
-    if (a.D) sum += a.D[c] * u;
-    if (a.z) sum *= swish(a.z[row * a.ld_z + c]);
-    a.y[row * a.ld_y + c] = sum;
+  for (int k = 0; k < R; ++k) {
+    const int64_t row = row0 + k;
+    const bool on = me.on && row < a.rows.tokens;
+    dt[k] += bias;
+    if (a.softplus) dt[k] = softplus(dt[k]);
+    const T x = dt[k] * u[k];
+    T sum = 0;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      h[k][j] = decay(dt[k] * rate(A[j])) * h[k][j] + x * B[k][j];
+      sum += C[k][j] * h[k][j];
+    }
+    write_states<S>(a.h_last + row * states, c, me.n0, on, a, h[k]);
+#pragma unroll
+    for (int i = 0; i < Lanes<L>::STATE_BITS; ++i) sum += __shfl_xor_sync(0xffffffffu, sum, 1 << Lanes<L>::state_bit(i));
+    if (on && me.lane == 0) {
+      sum += D * u[k];
+      if (a.z) sum *= swish(z[k]);
+      a.y[row * a.ld_y + c] = sum;
+    }
   }
 }
 
@@ -1207,13 +1274,18 @@ template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Arg
   const int64_t across = (int64_t)a.groups * a.blocks;
   PRAD_REQUIRE(across <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many channels");
   if (pass == Pass::Step) {
-    for (int64_t r0 = 0; r0 < a.rows.tokens; r0 += 65535) {      // (the grid's second dimension)
+    // four rows a thread where that still gives every SM eight CTAs
+    const int R = sizeof(T) == 4 && a.rows.tokens * across >= (int64_t)ctx->sm_count * 32 ? 4 : 1;
+    const int64_t most = (int64_t)65535 * R, states = (int64_t)a.dim * a.state;      // (the grid's second dimension)
+    for (int64_t r0 = 0; r0 < a.rows.tokens; r0 += most) {
       Args<T> b = a;
-      const int64_t n = a.rows.tokens - r0 < 65535 ? a.rows.tokens - r0 : 65535, states = (int64_t)a.dim * a.state;
+      b.rows.tokens = a.rows.tokens - r0 < most ? a.rows.tokens - r0 : most;
       b.u += r0 * a.ld_u, b.delta += r0 * a.ld_delta, b.B += r0 * a.ld_B, b.C += r0 * a.ld_C, b.y += r0 * a.ld_y;
       if (b.z) b.z += r0 * a.ld_z;
       b.h0 += r0 * states, b.h_last += r0 * states;
-      step_kernel<T, L, S><<<dim3((unsigned)across, (unsigned)n), THREADS, 0, ctx->stream>>>(b);
+      const dim3 grid((unsigned)across, (unsigned)ceil_div(b.rows.tokens, R));
+      if (R == 1) step_kernel<T, L, S, 1><<<grid, THREADS, 0, ctx->stream>>>(b);
+      else step_kernel<T, L, S, 4><<<grid, THREADS, 0, ctx->stream>>>(b);
       PRAD_LAUNCHED(ctx);
     }
     return PRAD_OK;
@@ -1267,6 +1339,8 @@ template <typename T> static prad_status pick(prad_ctx* ctx, Args<T> a, Pass pas
                         (uintptr_t)a.ddelta | (uintptr_t)a.dz;
   const int64_t pitches = a.ld_u | a.ld_delta | a.ld_z | a.ld_y | a.ld_dy | a.ld_du | a.ld_ddelta | a.ld_dz;
   a.wide = (all & 15) == 0 && pitches % V == 0 && (a.groups == 1 || a.per % V == 0);
+  const uintptr_t matrices = (uintptr_t)a.A | (uintptr_t)a.h0 | (uintptr_t)a.h_last | (uintptr_t)a.saved | (uintptr_t)a.dh0;
+  a.wide_h = (matrices & 15) == 0 && a.state % V == 0;
   if (a.state <= 8) return launch<T, 4, 2>(ctx, a, pass);
   if (a.state <= 16) return launch<T, 4, 4>(ctx, a, pass);
   if (a.state <= 32) return launch<T, 8, 4>(ctx, a, pass);

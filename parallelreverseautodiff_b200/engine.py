@@ -51,8 +51,8 @@ class DeviceMatrix:
     def __init__(self, engine: "Engine", ptr: int, shape: Sequence[int], dtype, owned=True):
         self.engine = engine
         self.ptr = ptr
-        self.shape = tuple(int(s) for s in shape)
-        self.dtype = np.dtype(dtype)
+        self.shape = tuple(map(int, shape))
+        self.dtype = dtype if isinstance(dtype, np.dtype) else np.dtype(dtype)
         self._owned = owned
 
     @property
@@ -98,7 +98,8 @@ class DeviceMatrix:
 
     def __del__(self):
         try:
-            self.free()
+            if self._owned:
+                self.free()
         except Exception:
             pass
 
