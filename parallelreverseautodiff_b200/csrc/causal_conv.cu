@@ -3,8 +3,9 @@
 // where the W - 1 rows before a sequence's first token come from its state (zero without one).  Backward, with g = dy swish'(p):
 //   dx_t = sum_k w[c][k] g_(t + W - 1 - k)  over the tokens of the sequence,  dw[c][k] = sum_t g_t x_(t - (W - 1) + k),  dbias = sum g.
 //
-// Bound by memory: a thread takes V neighbouring channels and walks down a run of tokens with the last W rows in registers and the
-// next four on their way, so that a row is read once per run and W - 1 rows twice.
+// Bound by memory: a thread takes V neighbouring channels and walks down a run of tokens with the last W rows in registers, so that a
+// row is read once per run and W - 1 rows twice.  The next rows are on their way into a ring of its own in shared memory: in
+// registers, four rows ahead took the room of the warps that are to keep the memory busy.
 #include "common.cuh"
 #include "packed_sequences.cuh"
 
@@ -16,7 +17,7 @@ using seq::swish;
 using seq::swish_slope;
 
 constexpr int LANES = 32, WARPS = 8, THREADS = LANES * WARPS;
-constexpr int AHEAD = 4;         // rows on their way
+constexpr int AHEAD = 8;         // rows on their way
 
 template <typename T> struct Args {
   Sequences rows;
@@ -30,6 +31,21 @@ template <typename T> struct Args {
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+
+// A thread's ring of rows: rows go in by asynchronous copies, one group of copies a row, and come out in their order.
+template <typename T, int V> struct Ring {
+  Pack<T, V>* at;                // of this thread's first slot; slots are THREADS packs apart
+  __device__ __forceinline__ Ring(void* shared, int which) : at((Pack<T, V>*)shared + which * AHEAD * THREADS + threadIdx.x) {}
+  __device__ __forceinline__ void put(int slot, const T* from) const {
+    constexpr int bytes = sizeof(T) * V;
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(at + slot * THREADS);
+    if constexpr (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(from), "n"(bytes) : "memory");
+  }
+  __device__ __forceinline__ Pack<T, V> get(int slot) const { return at[slot * THREADS]; }
+};
+__device__ __forceinline__ void end_of_row() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void oldest_landed() { asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory"); }
 
 // the row at place `p` of sequence s, which begins at row `start`: a token, or below zero a row of its state
 template <typename T, int V, int W>
@@ -101,22 +117,21 @@ forward_kernel(const Args<T> a) {
   Pack<T, V> x[W];              // x[W - 1]: the newest row
 #pragma unroll
   for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, t - start - (W - k), c);
-  Pack<T, V> next[AHEAD];
+  extern __shared__ __align__(16) unsigned char raw[];
+  const Ring<T, V> ring(raw, 0);
   const T* px = a.x + t * a.ld_x + c;
   T* py = a.y + t * a.ld_y + c;
+  const int rows = (int)(last - t);
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (t + i < last) next[i] = load<T, V>(px + i * a.ld_x);
-  while (t < last) {
-    Pack<T, V> now[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) now[i] = next[i];
-    px += AHEAD * a.ld_x;
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (t + AHEAD + i < last) next[i] = load<T, V>(px + i * a.ld_x);
+  for (int i = 0; i < AHEAD; ++i) {
+    if (i < rows) ring.put(i, px + i * a.ld_x);
+    end_of_row();
+  }
+  px += AHEAD * a.ld_x;
+  for (int i0 = 0;; i0 += AHEAD)
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
+      if (i0 + i >= rows) return;
       if (t == end) {
         do ++s; while (s < a.rows.count && a.rows.end(s) <= t);
         if (s >= a.rows.count) return;
@@ -127,7 +142,11 @@ forward_kernel(const Args<T> a) {
       }
 #pragma unroll
       for (int k = 0; k + 1 < W; ++k) x[k] = x[k + 1];
-      x[W - 1] = now[i];
+      oldest_landed();
+      x[W - 1] = ring.get(i);
+      if (i0 + i + AHEAD < rows) ring.put(i, px);
+      end_of_row();
+      px += a.ld_x;
       Pack<T, V> y;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -138,9 +157,8 @@ forward_kernel(const Args<T> a) {
       }
       *reinterpret_cast<Pack<T, V>*>(py) = y;
       py += a.ld_y;
-      if (++t == last) return;
+      ++t;
     }
-  }
 }
 
 // g at place q of a sequence
@@ -204,6 +222,7 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
     return;
   }
   __shared__ T part[WARPS][LANES * V];
+  extern __shared__ __align__(16) unsigned char raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = (blockIdx.y * LANES + lane) * V;
   const bool on = c < a.dim;
@@ -220,6 +239,7 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
   }
   if (on && t < last) {
     const Weights<T, V, W> wt(a, c);
+    const Ring<T, V> ring_x(raw, 0), ring_d(raw, 1);
     int s = a.rows.at(t);
     while (t < last && s < a.rows.count) {
       int64_t start = a.rows.start(s);
@@ -239,25 +259,17 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
       const T *px = a.x + t * a.ld_x + c, *pd = a.dy + t * a.ld_dy + c;
       T* po = a.dx + t * a.ld_dx + c;
       const int all = (int)(stop - t) + W - 1, taken = (int)(ahead - t), own = (int)(stop - t);
-      Pack<T, V> nx[AHEAD], nd[AHEAD];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i)
+      for (int i = 0; i < AHEAD; ++i) {
         if (i < taken) {
-          nx[i] = load<T, V>(px + i * a.ld_x);
-          nd[i] = load<T, V>(pd + i * a.ld_dy);
+          ring_x.put(i, px + i * a.ld_x);
+          ring_d.put(i, pd + i * a.ld_dy);
         }
+        end_of_row();
+      }
+      px += AHEAD * a.ld_x;
+      pd += AHEAD * a.ld_dy;
       for (int q0 = 0; q0 < all; q0 += AHEAD) {
-        Pack<T, V> cx[AHEAD], cd[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) cx[i] = nx[i], cd[i] = nd[i];
-        px += AHEAD * a.ld_x;
-        pd += AHEAD * a.ld_dy;
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-          if (q0 + AHEAD + i < taken) {
-            nx[i] = load<T, V>(px + i * a.ld_x);
-            nd[i] = load<T, V>(pd + i * a.ld_dy);
-          }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           const int q = q0 + i;
@@ -268,9 +280,10 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
 #pragma unroll
             for (int j = 0; j < V; ++j) g[k][j] = g[k + 1][j];
           }
+          oldest_landed();
           if (q < taken) {
-            x[W - 1] = cx[i];
-            slope<T, V, W>(wt, x, cd[i], a.swish, g[W - 1]);
+            x[W - 1] = ring_x.get(i);
+            slope<T, V, W>(wt, x, ring_d.get(i), a.swish, g[W - 1]);
             if (q < own)
 #pragma unroll
               for (int j = 0; j < V; ++j) {
@@ -282,6 +295,13 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
 #pragma unroll
             for (int j = 0; j < V; ++j) g[W - 1][j] = 0;
           }
+          if (q + AHEAD < taken) {
+            ring_x.put(i, px);
+            ring_d.put(i, pd);
+          }
+          end_of_row();
+          px += a.ld_x;
+          pd += a.ld_dy;
           if (q >= W - 1) {                                    // g[k] belongs to the token W - 1 - k before q
             Pack<T, V> dx;
 #pragma unroll
@@ -383,7 +403,10 @@ template <typename T, int V, int W, bool BACKWARD> static prad_status launch(pra
     const int64_t rows = W > 1 && a.state_out ? (int64_t)a.rows.count * (W - 1) : 0;
     const unsigned grid = a.blocks + (unsigned)ceil_div(rows, WARPS);
     if (grid) {
-      forward_kernel<T, V, W><<<dim3(grid, across), THREADS, 0, ctx->stream>>>(a);
+      constexpr int bytes = AHEAD * THREADS * V * (int)sizeof(T);
+      prad_status st = allow_smem<forward_kernel<T, V, W>>(ctx, bytes);
+      if (st) return st;
+      forward_kernel<T, V, W><<<dim3(grid, across), THREADS, bytes, ctx->stream>>>(a);
       PRAD_LAUNCHED(ctx);
     }
     return PRAD_OK;
@@ -393,7 +416,10 @@ template <typename T, int V, int W, bool BACKWARD> static prad_status launch(pra
     const bool states = W > 1 && a.dstate && a.rows.count;
     if (a.blocks) {
       const unsigned grid = a.blocks + (states ? (unsigned)ceil_div(a.rows.count, WARPS) : 0);
-      backward_kernel<T, V, W><<<dim3(grid, across), THREADS, 0, ctx->stream>>>(a, (T*)ctx->ws);
+      constexpr int bytes = 2 * AHEAD * THREADS * V * (int)sizeof(T);
+      st = allow_smem<backward_kernel<T, V, W>>(ctx, bytes);
+      if (st) return st;
+      backward_kernel<T, V, W><<<dim3(grid, across), THREADS, bytes, ctx->stream>>>(a, (T*)ctx->ws);
       PRAD_LAUNCHED(ctx);
     } else if (states) {
       PRAD_CUDA(cudaMemsetAsync(a.dstate, 0, (size_t)a.rows.count * (W - 1) * a.dim * sizeof(T), ctx->stream));

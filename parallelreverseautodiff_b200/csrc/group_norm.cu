@@ -70,6 +70,7 @@ rows_forward_kernel(const Args<T> a, int64_t slots) {
   // all lanes of a warp take part in its sums: those beyond the last sample with nothing to add
   const int64_t first = slot < slots ? slot / a.groups : a.samples;
   const int64_t rounds = ceil_rounds(a.samples, step * R);
+  const T inv = (T)1 / (T)a.per, eps = (T)a.eps;
   for (int64_t k = 0; k < rounds; ++k) {
     Pack<T, V> x[R][E];
 #pragma unroll
@@ -89,7 +90,7 @@ rows_forward_kernel(const Args<T> a, int64_t slots) {
       for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int j = 0; j < V; ++j) sum += x[r][e].v[j];
-      const T mean = lanes_sum<LW>(sum) / (T)a.per;
+      const T mean = lanes_sum<LW>(sum) * inv;
       T sq = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e)
@@ -98,8 +99,7 @@ rows_forward_kernel(const Args<T> a, int64_t slots) {
           const T d = x[r][e].v[j] - mean;
           if (on[e]) sq += d * d;
         }
-      const T var = lanes_sum<LW>(sq) / (T)a.per;
-      const T rstd = inverse_root(var + (T)a.eps);
+      const T rstd = inverse_root(lanes_sum<LW>(sq) * inv + eps);
       if (s < a.samples) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -448,10 +448,10 @@ __device__ __forceinline__ void thread_gradients(const Args<T>& a, const Place<T
     gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
     beta[j] = a.beta ? a.beta[c + j] : (T)0;
   }
-  for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
-    Pack<T, V> x[4], d[4];
+  for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)2 * w.rows) {
+    Pack<T, V> x[2], d[2];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 2; ++r)
       if (p + (int64_t)r * w.rows < w.p1) {
         x[r] = load<T, V>(a.x + at + (p + (int64_t)r * w.rows) * a.channels);
         d[r] = load<T, V>(a.dy + at + (p + (int64_t)r * w.rows) * a.channels);
@@ -460,7 +460,7 @@ __device__ __forceinline__ void thread_gradients(const Args<T>& a, const Place<T
 #pragma unroll
     for (int j = 0; j < V; ++j) rg[j] = rb[j] = 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 2; ++r)
       if (p + (int64_t)r * w.rows < w.p1) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -553,16 +553,16 @@ __device__ __forceinline__ void input_gradients(const Args<T>& a, const Place<T>
       gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
       beta[j] = a.beta ? a.beta[c + j] : (T)0;
     }
-    for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
-      Pack<T, V> x[4], d[4];
+    for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)2 * w.rows) {
+      Pack<T, V> x[2], d[2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 2; ++r)
         if (p + (int64_t)r * w.rows < w.p1) {
           x[r] = load<T, V>(a.x + at + (p + (int64_t)r * w.rows) * a.channels);
           d[r] = load<T, V>(a.dy + at + (p + (int64_t)r * w.rows) * a.channels);
         }
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 2; ++r)
         if (p + (int64_t)r * w.rows < w.p1) {
 #pragma unroll
           for (int j = 0; j < V; ++j) {
@@ -589,7 +589,7 @@ input_gradients_kernel(const Args<T> a, const Parts k, const double* __restrict_
 
 // both by one cluster per sample and part; sums as above, for dgamma and dbeta
 template <typename T, int V>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 4 : 2)
 cluster_backward_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
   __shared__ double part[2][THREADS * V];
   __shared__ double own[THREADS][2];
@@ -634,9 +634,24 @@ cluster_backward_kernel(const Args<T> a, const Parts k, double* __restrict__ sum
 // ---------------------------------------------------------------- launches
 template <typename T, int V> constexpr int most_in_registers() { return 32 * 8 * V; }
 
+// CTAs of a kernel that an SM holds (the same for every device this library is built for)
+template <auto Kernel> static int resident() {
+  static std::atomic<int> each{0};
+  int n = each.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, THREADS, 0) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = 1;
+    }
+    each.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 template <typename T, int V, int LW, int E> static prad_status rows(prad_ctx* ctx, const Args<T>& a, bool backward) {
-  // as many slots as fill the device, and a whole number of them per group
-  const int64_t fill = (int64_t)ctx->sm_count * (2048 / 2) / LW;
+  // as many slots as fill the device once, and a whole number of them per group
+  const int held = backward ? resident<rows_backward_kernel<T, V, LW, E>>() : resident<rows_forward_kernel<T, V, LW, E>>();
+  const int64_t fill = (int64_t)ctx->sm_count * held * THREADS / LW;
   int64_t per_group = fill / a.groups;
   if (per_group < 1) per_group = 1;
   if (per_group > a.samples) per_group = a.samples;
