@@ -6,6 +6,8 @@
 // Bound by memory: a thread takes V neighbouring channels and walks down a run of tokens with the last W rows in registers, so that a
 // row is read once per run and W - 1 rows twice.  The next rows are on their way into a ring of its own in shared memory: in
 // registers, four rows ahead took the room of the warps that are to keep the memory busy.
+#include <type_traits>
+
 #include "common.cuh"
 #include "packed_sequences.cuh"
 
@@ -221,6 +223,8 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
     if constexpr (W > 1) state_gradients<T, V, W>(a, blockIdx.x - a.blocks);
     return;
   }
+  using F = seq::Few<T, V>;
+  using Unit = typename F::type;
   __shared__ T part[WARPS][LANES * V];
   extern __shared__ __align__(16) unsigned char raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -230,15 +234,21 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
   int64_t t = ((int64_t)blockIdx.x * WARPS + warp) * a.run, last = t + a.run;
   if (t < lo) t = lo;
   if (last > hi) last = hi;
-  T dw[W][V], db[V];
+  T zeros[V], ones[V], minuses[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    db[j] = 0;
+  for (int j = 0; j < V; ++j) zeros[j] = 0, ones[j] = 1, minuses[j] = -1;
+  const Unit zero = F::from(zeros), one = F::from(ones), minus = F::from(minuses);
+  Unit dw[W], db = zero;
 #pragma unroll
-    for (int k = 0; k < W; ++k) dw[k][j] = 0;
-  }
+  for (int k = 0; k < W; ++k) dw[k] = zero;
   if (on && t < last) {
-    const Weights<T, V, W> wt(a, c);
+    Unit w[W], bias;
+    {
+      const Weights<T, V, W> wt(a, c);
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = F::from(wt.w[k]);
+      bias = F::from(wt.bias);
+    }
     const Ring<T, V> ring_x(raw, 0), ring_d(raw, 1);
     int s = a.rows.at(t);
     while (t < last && s < a.rows.count) {
@@ -248,14 +258,14 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
       const int64_t stop = end < last ? end : last;            // of the tokens whose dx is this thread's
       int64_t ahead = stop + W - 1;                            // of the tokens whose g they take
       if (ahead > end) ahead = end;
-      Pack<T, V> x[W];
+      Unit x[W], g[W];                                         // x[W - 1], g[W - 1]: the newest token's
 #pragma unroll
-      for (int k = 1; k < W; ++k) x[k] = row_at<T, V, W>(a, s, start, t - start - (W - k), c);
-      T g[W][V];                                               // g[W - 1]: the newest token's
+      for (int k = 1; k < W; ++k) {
+        const Pack<T, V> r = row_at<T, V, W>(a, s, start, t - start - (W - k), c);
+        x[k] = F::from(r.v);
+      }
 #pragma unroll
-      for (int k = 0; k < W; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) g[k][j] = 0;
+      for (int k = 0; k < W; ++k) g[k] = zero;
       const T *px = a.x + t * a.ld_x + c, *pd = a.dy + t * a.ld_dy + c;
       T* po = a.dx + t * a.ld_dx + c;
       const int all = (int)(stop - t) + W - 1, taken = (int)(ahead - t), own = (int)(stop - t);
@@ -269,49 +279,61 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
       }
       px += AHEAD * a.ld_x;
       pd += AHEAD * a.ld_dy;
+      // one row; INNER: its dx and the row AHEAD behind it are this run's
+      const auto row = [&](auto inner, int q, int i) {
+        constexpr bool INNER = decltype(inner)::value;
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) {
+          x[k] = x[k + 1];
+          g[k] = g[k + 1];
+        }
+        oldest_landed();
+        g[W - 1] = zero;
+        if (INNER || q < taken) {
+          const Pack<T, V> rx = ring_x.get(i), rd = ring_d.get(i);
+          x[W - 1] = F::from(rx.v);
+          g[W - 1] = F::from(rd.v);
+          if (a.swish) {
+            Unit p = bias;
+#pragma unroll
+            for (int k = 0; k < W; ++k) p = seq::fma(w[k], x[k], p);
+            // s (1 + p (1 - s)) = s + s p - s (s p)
+            const Unit sig = seq::each<T>(p, seq::sigmoid), sp = seq::mul(sig, p);
+            const Unit rest = seq::fma(seq::mul(sig, minus), sp, sp);
+            g[W - 1] = seq::mul(g[W - 1], seq::fma(sig, one, rest));
+          }
+          if (INNER || q < own) {
+            db = seq::fma(g[W - 1], one, db);
+#pragma unroll
+            for (int k = 0; k < W; ++k) dw[k] = seq::fma(g[W - 1], x[k], dw[k]);
+          }
+        }
+        if (INNER || q + AHEAD < taken) {
+          ring_x.put(i, px);
+          ring_d.put(i, pd);
+        }
+        end_of_row();
+        px += a.ld_x;
+        pd += a.ld_dy;
+        if (INNER || q >= W - 1) {                             // g[k] belongs to the token W - 1 - k before q
+          Unit dx = seq::mul(w[W - 1], g[0]);
+#pragma unroll
+          for (int k = 1; k < W; ++k) dx = seq::fma(w[W - 1 - k], g[k], dx);
+          Pack<T, V> out;
+          F::to(dx, out.v);
+          *reinterpret_cast<Pack<T, V>*>(po) = out;
+          po += a.ld_dx;
+        }
+      };
       for (int q0 = 0; q0 < all; q0 += AHEAD) {
+        if (q0 >= W - 1 && q0 + 2 * AHEAD <= own) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const int q = q0 + i;
-          if (q >= all) break;
+          for (int i = 0; i < AHEAD; ++i) row(std::true_type(), q0 + i, i);
+        } else {
 #pragma unroll
-          for (int k = 0; k + 1 < W; ++k) {
-            x[k] = x[k + 1];
-#pragma unroll
-            for (int j = 0; j < V; ++j) g[k][j] = g[k + 1][j];
-          }
-          oldest_landed();
-          if (q < taken) {
-            x[W - 1] = ring_x.get(i);
-            slope<T, V, W>(wt, x, ring_d.get(i), a.swish, g[W - 1]);
-            if (q < own)
-#pragma unroll
-              for (int j = 0; j < V; ++j) {
-                db[j] += g[W - 1][j];
-#pragma unroll
-                for (int k = 0; k < W; ++k) dw[k][j] += g[W - 1][j] * x[k].v[j];
-              }
-          } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) g[W - 1][j] = 0;
-          }
-          if (q + AHEAD < taken) {
-            ring_x.put(i, px);
-            ring_d.put(i, pd);
-          }
-          end_of_row();
-          px += a.ld_x;
-          pd += a.ld_dy;
-          if (q >= W - 1) {                                    // g[k] belongs to the token W - 1 - k before q
-            Pack<T, V> dx;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              dx.v[j] = 0;
-#pragma unroll
-              for (int k = 0; k < W; ++k) dx.v[j] += wt.w[W - 1 - k][j] * g[k][j];
-            }
-            *reinterpret_cast<Pack<T, V>*>(po) = dx;
-            po += a.ld_dx;
+          for (int i = 0; i < AHEAD; ++i) {
+            if (q0 + i >= all) break;
+            row(std::false_type(), q0 + i, i);
           }
         }
       }
@@ -323,8 +345,10 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
 #pragma unroll
   for (int k = 0; k <= W; ++k) {
     __syncthreads();
+    T sums[V];
+    F::to(k < W ? dw[k < W ? k : 0] : db, sums);
 #pragma unroll
-    for (int j = 0; j < V; ++j) part[warp][lane * V + j] = k < W ? dw[k < W ? k : 0][j] : db[j];
+    for (int j = 0; j < V; ++j) part[warp][lane * V + j] = sums[j];
     __syncthreads();
     for (int e = threadIdx.x; e < LANES * V; e += THREADS) {
       const int ch = blockIdx.y * LANES * V + e;
@@ -394,9 +418,9 @@ template <typename T, int V, int W, bool BACKWARD> static prad_status launch(pra
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
-  // Runs of 32 tokens, or shorter ones where those give less than two CTAs an SM (2047 tokens of 333 doubles, backward: 26 us with
-  // runs of 32, SHORT_US with runs of 8).
-  a.run = 32;
+  // Runs of 32 tokens, of 64 backward (16384 tokens of 2048 floats: forward 45 us, 51 with 64; backward 93 us, 85 with 64), or shorter
+  // ones where those give less than two CTAs an SM (2047 tokens of 333 doubles, backward: 26 us with runs of 32, 13 with runs of 8).
+  a.run = BACKWARD ? 64 : 32;
   while (a.run > 8 && ceil_div(a.rows.tokens, WARPS * a.run) * across < 2 * ctx->sm_count) a.run /= 2;
   a.blocks = (unsigned)ceil_div(a.rows.tokens, WARPS * a.run);
   if constexpr (!BACKWARD) {

@@ -54,5 +54,62 @@ template <typename T> __device__ __forceinline__ T swish_slope(T x) {
   return s * ((T)1 + x * ((T)1 - s));
 }
 
+// two values side by side: float works on both with one instruction
+template <typename T> struct Two;
+template <> struct Two<float> {
+  unsigned long long v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+template <> struct Two<double> {
+  double a_, b_;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(double a, double b) : a_(a), b_(b) {}
+  __device__ __forceinline__ void get(double& a, double& b) const { a = a_, b = b_; }
+};
+__device__ __forceinline__ Two<float> mul(Two<float> a, Two<float> b) {
+  Two<float> r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) {
+  Two<float> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two<double> mul(Two<double> a, Two<double> b) { return {a.a_ * b.a_, a.b_ * b.b_}; }
+__device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) {
+  return {::fma(a.a_, b.a_, c.a_), ::fma(a.b_, b.b_, c.b_)};
+}
+// one value, with the same functions
+template <typename T> struct One {
+  T v;
+  __device__ __forceinline__ One() {}
+  __device__ __forceinline__ explicit One(T a) : v(a) {}
+};
+__device__ __forceinline__ One<float> mul(One<float> a, One<float> b) { return One<float>(a.v * b.v); }
+__device__ __forceinline__ One<float> fma(One<float> a, One<float> b, One<float> c) { return One<float>(fmaf(a.v, b.v, c.v)); }
+__device__ __forceinline__ One<double> mul(One<double> a, One<double> b) { return One<double>(a.v * b.v); }
+__device__ __forceinline__ One<double> fma(One<double> a, One<double> b, One<double> c) { return One<double>(::fma(a.v, b.v, c.v)); }
+template <typename T> __device__ __forceinline__ Two<T> each(const Two<T>& x, T (*f)(T)) {
+  T a, b;
+  x.get(a, b);
+  return {f(a), f(b)};
+}
+template <typename T> __device__ __forceinline__ One<T> each(const One<T>& x, T (*f)(T)) { return One<T>(f(x.v)); }
+// V = 1 or 2 neighbouring values
+template <typename T, int V> struct Few;
+template <typename T> struct Few<T, 1> {
+  using type = One<T>;
+  __device__ static __forceinline__ type from(const T* v) { return One<T>(v[0]); }
+  __device__ static __forceinline__ void to(const type& x, T* v) { v[0] = x.v; }
+};
+template <typename T> struct Few<T, 2> {
+  using type = Two<T>;
+  __device__ static __forceinline__ type from(const T* v) { return {v[0], v[1]}; }
+  __device__ static __forceinline__ void to(const type& x, T* v) { x.get(v[0], v[1]); }
+};
+
 }  // namespace seq
 }  // namespace prad

@@ -23,6 +23,9 @@ namespace ssm {
 using seq::Sequences;
 using seq::swish;
 using seq::swish_slope;
+using seq::Two;
+using seq::fma;
+using seq::mul;
 
 constexpr int THREADS = 128;
 template <typename T> constexpr int tile() { return sizeof(T) == 8 ? 16 : 32; }     // TT of the passes without a history
@@ -80,34 +83,6 @@ __device__ __forceinline__ double softplus(double x, double& slope) {
 }
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
-// two values side by side: float works on both with one instruction
-template <typename T> struct Two;
-template <> struct Two<float> {
-  unsigned long long v;
-  __device__ __forceinline__ Two() {}
-  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-template <> struct Two<double> {
-  double a_, b_;
-  __device__ __forceinline__ Two() {}
-  __device__ __forceinline__ Two(double a, double b) : a_(a), b_(b) {}
-  __device__ __forceinline__ void get(double& a, double& b) const { a = a_, b = b_; }
-};
-__device__ __forceinline__ Two<float> mul(Two<float> a, Two<float> b) {
-  Two<float> r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) {
-  Two<float> r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Two<double> mul(Two<double> a, Two<double> b) { return {a.a_ * b.a_, a.b_ * b.b_}; }
-__device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) {
-  return {::fma(a.a_, b.a_, c.a_), ::fma(a.b_, b.b_, c.b_)};
-}
 template <typename T> __device__ __forceinline__ Two<T> decay(Two<T> x) {
   T a, b;
   x.get(a, b);
