@@ -28,7 +28,9 @@ using seq::fma;
 using seq::mul;
 
 constexpr int THREADS = 128;
-template <typename T> constexpr int tile() { return sizeof(T) == 8 ? 16 : 32; }     // TT of the passes without a history
+// TT of the passes without a history: 16 where a CTA has 64 channels (or doubles), so that what it fetches stays in registers
+template <typename T, int L> constexpr int tile() { return sizeof(T) == 8 || L == 2 ? 16 : 32; }
+constexpr int SPAN = 32;         // spans are multiples of this many tokens
 constexpr int POINT = 16;        // tokens per checkpoint, and TT of the main backward pass
 constexpr int MAX_STATE = 128;
 
@@ -95,12 +97,15 @@ template <typename T> __device__ __forceinline__ T total(Two<T> x) {
 }
 // S values of shared memory (16-byte aligned for float) as pairs
 template <int P> __device__ __forceinline__ void read(const float* m, Two<float> (&v)[P]) {
-  if constexpr (P == 2) {
-    const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(m);
-    v[0].v = q.x;
-    v[1].v = q.y;
-  } else {
+  if constexpr (P == 1) {
     v[0].v = *reinterpret_cast<const unsigned long long*>(m);
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; j += 2) {
+      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(m + 2 * j);
+      v[j].v = q.x;
+      v[j + 1].v = q.y;
+    }
   }
 }
 template <int P> __device__ __forceinline__ void read(const double* m, Two<double> (&v)[P]) {
@@ -134,9 +139,9 @@ template <typename T, int S> struct alignas(sizeof(T) * S) Pack { T v[S]; };
 // many as L needs), its channel's number of the others.  A 128-bit read of shared memory takes two cycles if its address does not
 // depend on bit 0 or does not depend on bit 1 of the lane, and four otherwise: so the reads by channel and those by state both take two.
 template <int L> struct Lanes {
-  static constexpr int STATE_BITS = L == 4 ? 2 : L == 8 ? 3 : L == 16 ? 4 : 5;
+  static constexpr int STATE_BITS = L == 2 ? 1 : L == 4 ? 2 : L == 8 ? 3 : L == 16 ? 4 : 5;
   __host__ __device__ static constexpr int state_bit(int i) { return i == 0 ? 1 : i == 4 ? 0 : 5 - i; }
-  __host__ __device__ static constexpr int channel_bit(int i) { return i == 0 ? 0 : i + 1; }
+  __host__ __device__ static constexpr int channel_bit(int i) { return i == 0 ? 0 : i + 1; }      // 0, 2, 3, 4
   __device__ static __forceinline__ int state(int lane) {
     int l = 0;
 #pragma unroll
@@ -211,17 +216,27 @@ template <typename T, int L, int S> struct Place {
 };
 
 // Four values a lane, one for each of four tokens, summed over the L lanes of a channel: afterwards lane l holds the sum of token
-// l mod 4.  Half of the values change hands in each of the first two steps.
-template <int L, typename T> __device__ __forceinline__ T sum4(const T (&v)[4], int lane) {
-  const bool hi = lane & 2, odd = lane & 1;
-  T a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
-  a += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 1 << Lanes<L>::state_bit(1));
-  b += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 1 << Lanes<L>::state_bit(1));
-  T c = odd ? b : a;
-  c += __shfl_xor_sync(0xffffffffu, odd ? a : b, 1 << Lanes<L>::state_bit(0));
+// l mod 4 (with two lanes: lane l the sums of tokens 2 l and 2 l + 1).  Half of the values change hands in each of the first steps.
+template <int L, typename T> __device__ __forceinline__ void sum4(const T (&v)[4], int lane, T& a, T& b) {
+  const bool hi = L == 2 ? lane & 1 : lane & 2;
+  constexpr int over = 1 << Lanes<L>::state_bit(L == 2 ? 0 : 1);
+  a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
+  a += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], over);
+  b += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], over);
+  if constexpr (L > 2) {
+    const bool odd = lane & 1;
+    const T give = odd ? a : b;
+    a = odd ? b : a;
+    a += __shfl_xor_sync(0xffffffffu, give, 1 << Lanes<L>::state_bit(0));
 #pragma unroll
-  for (int i = 2; i < Lanes<L>::STATE_BITS; ++i) c += __shfl_xor_sync(0xffffffffu, c, 1 << Lanes<L>::state_bit(i));
-  return c;
+    for (int i = 2; i < Lanes<L>::STATE_BITS; ++i) a += __shfl_xor_sync(0xffffffffu, a, 1 << Lanes<L>::state_bit(i));
+  }
+}
+template <int L, typename T> __device__ __forceinline__ T sum4(const T (&v)[4], int lane) {
+  static_assert(L > 2, "one sum a lane");
+  T a, b;
+  sum4<L>(v, lane, a, b);
+  return a;
 }
 
 // bits of the tile's tokens that begin a sequence; `s` is the sequence of the tile's first token or a later one's that begins in it
@@ -351,7 +366,7 @@ template <int V, typename T> __device__ __forceinline__ void pick(const T* m, T 
 
 // ---------------------------------------------------------------- forward
 template <typename T, int L, int S> struct Forward {
-  static constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S;
+  static constexpr int CH = THREADS / L, TT = tile<T, L>(), N = L * S;
   alignas(16) T B[2][TT][N], C[2][TT][N];
   typename StepOf<T>::type step[TT][CH];
   alignas(16) T y[TT][CH + 8];  // (four tokens of eight channels at a time: no two in one bank)
@@ -361,7 +376,7 @@ template <typename T, int L, int S> struct Forward {
 template <typename T, int L, int S, bool EDGES>
 __global__ void __launch_bounds__(THREADS, 4)
 forward_kernel(const Args<T> a) {
-  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2;
+  constexpr int CH = THREADS / L, TT = tile<T, L>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
   Forward<T, L, S>& m = *reinterpret_cast<Forward<T, L, S>*>(raw);
   const Place<T, L, S> me(a);
@@ -505,8 +520,14 @@ forward_kernel(const Args<T> a) {
           }
         }
         if (!EDGES) {
-          const T r = sum4<L>(part, me.lane);
-          if (me.lane < 4) m.y[t0 + me.lane][me.ch] = r;
+          T one, two;
+          sum4<L>(part, me.lane, one, two);
+          if (L == 2) {
+            m.y[t0 + 2 * me.lane][me.ch] = one;
+            m.y[t0 + 2 * me.lane + 1][me.ch] = two;
+          } else if (me.lane < 4) {
+            m.y[t0 + me.lane][me.ch] = one;
+          }
         }
       }
       __syncthreads();
@@ -539,49 +560,66 @@ forward_kernel(const Args<T> a) {
 
 // Strings the spans together: edge[p] becomes the state that span p begins with.  FORWARD: edge[p + 1] holds what span p ends in
 // from zero; otherwise edge[p] holds what span p hands up from zero, and becomes what it is handed from below.
+// A span takes what it is given, x, to own + through x.  A CTA has JOINED neighbouring states and 32 spans at a time, a warp each
+// state: the lanes' maps are composed in five steps (one thread for all spans of a state took 12 us for 18 spans of 16384 states).
+constexpr int JOINED = 8;
 template <typename T, bool FORWARD>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(32 * JOINED)
 join_kernel(const Args<T> a) {
-  const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x, each = (int64_t)a.dim * a.state;
-  if (i >= each) return;
-  const T A = rate(a.A[i]);
-  const int c = (int)(i / a.state);
-  T carry = 0;
+  __shared__ T s_own[JOINED][33], s_through[JOINED][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int k = threadIdx.x / JOINED;                  // of the reading and writing: span k, state i
+  const int64_t i0 = (int64_t)blockIdx.x * JOINED, i = i0 + threadIdx.x % JOINED, each = (int64_t)a.dim * a.state;
+  const bool on = i < each;
+  const T A = on ? rate(a.A[i]) : (T)0;
+  const int c = on ? (int)(i / a.state) : 0;
   const int spans = FORWARD ? a.spans - 1 : a.spans;
-  constexpr int AHEAD = 8;             // spans whose values are on their way at the same time
-  for (int k0 = 0; k0 < spans; k0 += AHEAD) {
-    T own[AHEAD], through[AHEAD];
+  T carry = 0;                                         // of this warp's state
+  for (int k0 = 0; k0 < spans; k0 += 32) {
+    const int p = FORWARD ? k0 + k : spans - 1 - k0 - k;
+    const bool live = on && k0 + k < spans;
+    T own = 0, through = 1;
+    if (live) {
+      own = a.edge[(p + FORWARD) * each + i];
+      through = a.passes[p] ? decay(A * a.sum[(int64_t)p * a.dim + c]) : (T)-1;       // (a decay is never negative)
+    }
+    s_own[threadIdx.x % JOINED][k] = own;
+    s_through[threadIdx.x % JOINED][k] = through;
+    __syncthreads();
+    own = s_own[warp][lane];
+    through = s_through[warp][lane];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int p = FORWARD ? k0 + k : spans - 1 - k0 - k;
-      own[k] = through[k] = 0;
-      if (k0 + k < spans) {
-        own[k] = a.edge[(p + FORWARD) * each + i];
-        through[k] = a.passes[p] ? decay(A * a.sum[(int64_t)p * a.dim + c]) : (T)-1;
+    for (int o = 1; o < 32; o <<= 1) {
+      const T before = __shfl_up_sync(0xffffffffu, own, o), pass = __shfl_up_sync(0xffffffffu, through, o);
+      if (lane >= o && !(through < (T)0)) {            // (what a map that passes nothing is given, NaN or not, leaves no trace)
+        own += through * before;
+        through = pass < (T)0 ? pass : through * pass;
       }
     }
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int p = FORWARD ? k0 + k : spans - 1 - k0 - k;
-      if (k0 + k >= spans) break;
-      if (!FORWARD) a.edge[p * each + i] = carry;
-      carry = through[k] < (T)0 ? own[k] : own[k] + through[k] * carry;      // (a decay is never negative)
-      if (FORWARD) a.edge[(p + 1) * each + i] = carry;
-    }
+    // behind span k0 + lane, and in front of it
+    const T behind = through < (T)0 ? own : own + through * carry;
+    T front = __shfl_up_sync(0xffffffffu, behind, 1);
+    if (lane == 0) front = carry;
+    carry = __shfl_sync(0xffffffffu, behind, 31);
+    __syncthreads();
+    s_own[warp][lane] = FORWARD ? behind : front;
+    __syncthreads();
+    if (live) a.edge[(p + FORWARD) * each + i] = s_own[threadIdx.x % JOINED][k];
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------- backward
 // What a span hands to the one above it when it is handed zero: a_n g_n of its first token.
 template <typename T, int L, int S> struct Edges {
-  static constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S;
+  static constexpr int CH = THREADS / L, TT = tile<T, L>(), N = L * S;
   alignas(16) T C[2][TT][N];
   typename StepOf<T>::type step[TT][CH];        // dt and v
 };
 template <typename T, int L, int S>
 __global__ void __launch_bounds__(THREADS, 4)
 backward_edges_kernel(const Args<T> a) {
-  constexpr int CH = THREADS / L, TT = tile<T>(), N = L * S, P = S / 2;
+  constexpr int CH = THREADS / L, TT = tile<T, L>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
   Edges<T, L, S>& m = *reinterpret_cast<Edges<T, L, S>*>(raw);
   const Place<T, L, S> me(a);
@@ -1197,7 +1235,7 @@ template <auto Kernel> static int64_t resident(prad_ctx* ctx, int smem) {
 // about half of the work again), else into spans of whole tiles, as many as the device holds at a time: one CTA more takes as long
 // as twice as many.
 template <typename T> static void cut(Args<T>& a, int64_t across, int64_t full) {
-  if (!a.rows.offsets && a.rows.count > 0 && a.rows.count <= 65535 && (a.rows.count * across >= full / 2 || a.rows.each <= 2 * tile<T>())) {
+  if (!a.rows.offsets && a.rows.count > 0 && a.rows.count <= 65535 && (a.rows.count * across >= full / 2 || a.rows.each <= 2 * SPAN)) {
     a.span = a.rows.each > 0 ? a.rows.each : 1;
     a.spans = a.rows.count;
     return;
@@ -1205,8 +1243,8 @@ template <typename T> static void cut(Args<T>& a, int64_t across, int64_t full) 
   int64_t spans = full / across;
   if (spans < 1) spans = 1;
   if (spans > 65535) spans = 65535;
-  int64_t span = ceil_div(ceil_div(a.rows.tokens, spans), tile<T>()) * tile<T>();
-  if (span < 2 * tile<T>()) span = 2 * tile<T>();
+  int64_t span = ceil_div(ceil_div(a.rows.tokens, spans), SPAN) * SPAN;
+  if (span < 2 * SPAN) span = 2 * SPAN;
   a.span = span;
   a.spans = (int)ceil_div(a.rows.tokens, span);
   if (a.spans < 1) a.spans = 1;
@@ -1240,12 +1278,13 @@ template <typename T> static size_t carve(Args<T>& a, bool backward, void* ws) {
   return c.used;
 }
 
-template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Args<T> a, Pass pass) {
+// FL lanes of FS states a channel in the forward passes, L of S backward and for single tokens
+template <typename T, int L, int S, int FL, int FS> static prad_status launch(prad_ctx* ctx, Args<T> a, Pass pass) {
   using Main = Backward<T, L, S>;
   const bool backward = pass == Pass::Backward;
   // the edges' pass has THREADS / L channels a CTA, the main backward pass CC times as many
   const int edge_blocks = (int)ceil_div(a.per, THREADS / L);
-  a.blocks = backward ? (int)ceil_div(a.per, Main::CH) : edge_blocks;
+  a.blocks = backward ? (int)ceil_div(a.per, Main::CH) : pass == Pass::Forward ? (int)ceil_div(a.per, THREADS / FL) : edge_blocks;
   const int64_t across = (int64_t)a.groups * a.blocks;
   PRAD_REQUIRE(across <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many channels");
   if (pass == Pass::Step) {
@@ -1266,12 +1305,12 @@ template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Arg
     return PRAD_OK;
   }
   using Shared = typename Main::Shared;
-  constexpr int bytes = (int)sizeof(Forward<T, L, S>);
-  prad_status st = backward ? allow_smem<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : allow_smem<forward_kernel<T, L, S, false>>(ctx, bytes);
+  constexpr int bytes = (int)sizeof(Forward<T, FL, FS>);
+  prad_status st = backward ? allow_smem<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : allow_smem<forward_kernel<T, FL, FS, false>>(ctx, bytes);
   constexpr int edge_bytes = (int)sizeof(Edges<T, L, S>);
-  if (!st) st = backward ? allow_smem<backward_edges_kernel<T, L, S>>(ctx, edge_bytes) : allow_smem<forward_kernel<T, L, S, true>>(ctx, bytes);
+  if (!st) st = backward ? allow_smem<backward_edges_kernel<T, L, S>>(ctx, edge_bytes) : allow_smem<forward_kernel<T, FL, FS, true>>(ctx, bytes);
   if (st) return st;
-  cut(a, across, backward ? resident<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : resident<forward_kernel<T, L, S, false>>(ctx, bytes));
+  cut(a, across, backward ? resident<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : resident<forward_kernel<T, FL, FS, false>>(ctx, bytes));
   st = ensure_workspace(ctx, carve(a, backward, nullptr));
   if (st) return st;
   carve(a, backward, ctx->ws);
@@ -1279,12 +1318,12 @@ template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Arg
   const unsigned x = (unsigned)across;
   if (!backward) {
     if (joined(a)) {
-      forward_kernel<T, L, S, true><<<dim3(x, (unsigned)a.spans - 1), THREADS, bytes, ctx->stream>>>(a);
+      forward_kernel<T, FL, FS, true><<<dim3(x, (unsigned)a.spans - 1), THREADS, bytes, ctx->stream>>>(a);
       PRAD_LAUNCHED(ctx);
-      join_kernel<T, true><<<(unsigned)ceil_div(states, THREADS), THREADS, 0, ctx->stream>>>(a);
+      join_kernel<T, true><<<(unsigned)ceil_div(states, JOINED), 32 * JOINED, 0, ctx->stream>>>(a);
       PRAD_LAUNCHED(ctx);
     }
-    forward_kernel<T, L, S, false><<<dim3(x, (unsigned)a.spans), THREADS, bytes, ctx->stream>>>(a);
+    forward_kernel<T, FL, FS, false><<<dim3(x, (unsigned)a.spans), THREADS, bytes, ctx->stream>>>(a);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
@@ -1294,7 +1333,7 @@ template <typename T, int L, int S> static prad_status launch(prad_ctx* ctx, Arg
     b.blocks = edge_blocks;
     backward_edges_kernel<T, L, S><<<dim3((unsigned)(a.groups * edge_blocks), (unsigned)a.spans), THREADS, edge_bytes, ctx->stream>>>(b);
     PRAD_LAUNCHED(ctx);
-    join_kernel<T, false><<<(unsigned)ceil_div(states, THREADS), THREADS, 0, ctx->stream>>>(a);
+    join_kernel<T, false><<<(unsigned)ceil_div(states, JOINED), 32 * JOINED, 0, ctx->stream>>>(a);
     PRAD_LAUNCHED(ctx);
   }
   backward_kernel<T, L, S><<<dim3(x, (unsigned)a.spans), THREADS, sizeof(Shared), ctx->stream>>>(a);
@@ -1316,11 +1355,20 @@ template <typename T> static prad_status pick(prad_ctx* ctx, Args<T> a, Pass pas
   a.wide = (all & 15) == 0 && pitches % V == 0 && (a.groups == 1 || a.per % V == 0);
   const uintptr_t matrices = (uintptr_t)a.A | (uintptr_t)a.h0 | (uintptr_t)a.h_last | (uintptr_t)a.saved | (uintptr_t)a.dh0;
   a.wide_h = (matrices & 15) == 0 && a.state % V == 0;
-  if (a.state <= 8) return launch<T, 4, 2>(ctx, a, pass);
-  if (a.state <= 16) return launch<T, 4, 4>(ctx, a, pass);
-  if (a.state <= 32) return launch<T, 8, 4>(ctx, a, pass);
-  if (a.state <= 64) return launch<T, 16, 4>(ctx, a, pass);
-  return launch<T, 32, 4>(ctx, a, pass);
+  // Forward, eight states of a float channel to a lane: half of the sums over lanes and of the reads of dt that four take.
+  if constexpr (sizeof(T) == 4) {
+    if (a.state <= 8) return launch<T, 4, 2, 2, 4>(ctx, a, pass);
+    if (a.state <= 16) return launch<T, 4, 4, 2, 8>(ctx, a, pass);
+    if (a.state <= 32) return launch<T, 8, 4, 4, 8>(ctx, a, pass);
+    if (a.state <= 64) return launch<T, 16, 4, 8, 8>(ctx, a, pass);
+    return launch<T, 32, 4, 16, 8>(ctx, a, pass);
+  } else {
+    if (a.state <= 8) return launch<T, 4, 2, 4, 2>(ctx, a, pass);
+    if (a.state <= 16) return launch<T, 4, 4, 4, 4>(ctx, a, pass);
+    if (a.state <= 32) return launch<T, 8, 4, 8, 4>(ctx, a, pass);
+    if (a.state <= 64) return launch<T, 16, 4, 16, 4>(ctx, a, pass);
+    return launch<T, 32, 4, 32, 4>(ctx, a, pass);
+  }
 }
 
 static prad_status check(const char* who, prad_dtype dt, const prad_scan_t* s) {

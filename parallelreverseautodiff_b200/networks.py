@@ -927,3 +927,123 @@ class SwinBlock:
         self.d_x = e.layernorm_backward_add(self.x, self.mu1, self.sd1, d_ln1, d_r1, out=B_("d_x", (T, d)))
         self.d_qkv, self.d_attn = d_qkv, d_attn
         return self.d_x
+
+
+class StateSpaceBlock:
+    """One state space layer over packed sequences, forward, backward and token by token:
+
+        uz = x Win;  c = swish(causal convolution of u);  dbc = c Wx;  delta = dbc[rank] Wdt
+        y = selective scan of (c, delta + bdt, A, B = dbc[...], C = dbc[...], D) times swish(z)
+        out = x + dropout(groupnorm(y) Wout)
+
+    Not in the reference, whose sequence models are the LSTM examples (see LstmNetwork) and attention (SwinBlock).  u and z are
+    the halves of one product, delta's factor, B and C the columns of another: the operators read them where they are.
+    """
+
+    def __init__(self, eng: E.Engine, dtype, dim, inner=None, state=16, groups=1, rank=None, width=4, norm_groups=1, dropout=0.0,
+                 seed=0):
+        self.eng, self.dtype = eng, np.dtype(dtype)
+        self.dim, self.inner, self.state, self.groups, self.width = dim, inner or 2 * dim, state, groups, width
+        self.rank, self.norm_groups, self.p_drop, self.seed = rank or max(1, dim // 16), norm_groups, dropout, seed
+        d, n = self.inner, state
+        self.columns = self.rank + 2 * groups * n                 # of dbc
+        z = lambda *s: eng.zeros(s, dtype)  # noqa: E731
+        self.p = {"Win": z(dim, 2 * d), "Wc": z(d, width), "bc": z(d), "Wx": z(d, self.columns), "Wdt": z(self.rank, d), "bdt": z(d),
+                  "A": z(d, n), "D": z(d), "gamma": z(d), "beta": z(d), "Wout": z(d, dim)}
+        self.g = {k: z(*v.shape) for k, v in self.p.items()}
+        self._cache = {}
+
+    _buf = SwinBlock._buf
+    set_parameters = SwinBlock.set_parameters
+
+    def new_states(self, sequences):
+        """The states in front of `sequences` empty sequences: the convolution's last rows and the scan's state."""
+        z = lambda *s: self.eng.zeros(s, self.dtype)  # noqa: E731
+        return {"conv": z(sequences, (self.width - 1) * self.inner), "h": z(sequences, self.inner * self.state)}
+
+    def _parts(self, uz, dbc):
+        """Columns of the two products, and the pitches they are read with."""
+        T, d, n = uz.shape[0], self.inner, self.groups * self.state
+        parts = {"u": uz.view((T, d)), "z": uz.view((T, d), d), "factor": dbc.view((T, self.rank)),
+                 "B": dbc.view((T, n), self.rank), "C": dbc.view((T, n), self.rank + n)}
+        return parts, {"z": 2 * d, "B": self.columns, "C": self.columns}
+
+    def _mix(self, x, T, convolve):
+        """x -> uz, c, dbc, delta; `convolve` is the convolution of a prompt or of single tokens."""
+        e, p, d, B_ = self.eng, self.p, self.inner, self._buf
+        uz, dbc, delta = B_("uz", (T, 2 * d)), B_("dbc", (T, self.columns)), B_("delta", (T, d))
+        e.matmul_forward(x, p["Win"], Y=uz)
+        c = convolve(uz.view((T, d)), B_("c", (T, d)))
+        e.matmul_forward(c, p["Wx"], Y=dbc)
+        e.gemm(dbc, p["Wdt"], delta, M=T, N=d, K=self.rank, lda=self.columns)
+        return uz, c, dbc, delta
+
+    def _project(self, x, y, T, drop, step):
+        """y -> x + dropout(groupnorm(y) Wout)."""
+        e, p, d, B_ = self.eng, self.p, self.inner, self._buf
+        self.norm = e.group_norm_forward(y, self.norm_groups, p["gamma"], p["beta"], out=(B_("v", (T, d)), B_("mean", (T, self.norm_groups)),
+                                                                                       B_("rstd", (T, self.norm_groups))))
+        proj = e.matmul_forward(self.norm[0], p["Wout"], Y=B_("proj", (T, self.dim)))
+        return e.dropout(proj, self.p_drop if drop else 0.0, self.seed, 0, residual=x, step=step, out=B_("out", (T, self.dim)))
+
+    def forward(self, x: E.DeviceMatrix, offsets=None, sequences=1, states=None, states_out=None, training=True, step=None):
+        """x [tokens x dim].  `states`: in front of the sequences (new_states or an earlier states_out), `states_out`: to take those
+        behind them; `step`: a device counter that draws another dropout mask at each value (Engine.dropout_step)."""
+        e, p, B_, T = self.eng, self.p, self._buf, x.shape[0]
+        self.x, self.rows, self.step_counter, self.training = x, dict(offsets=offsets, sequences=sequences), step, training
+        before = states or {"conv": None, "h": None}
+        after = states_out or {"conv": None, "h": None}
+        self.before = before
+        conv = lambda u, out: e.causal_conv_forward(u, p["Wc"], p["bc"], before["conv"], **self.rows, out=out,  # noqa: E731
+                                                    state_out=after["conv"], ld_x=2 * self.inner)[0]
+        self.uz, self.c, self.dbc, self.delta = self._mix(x, T, conv)
+        parts, pitches = self._parts(self.uz, self.dbc)
+        saved = B_("saved", (max(1, (T + 15) // 16 * self.inner * self.state),)) if training else False
+        self.y, _, self.saved = e.selective_scan_forward(
+            self.c, self.delta, p["A"], parts["B"], parts["C"], p["D"], parts["z"], p["bdt"], before["h"], groups=self.groups, **self.rows,
+            out=B_("y", (T, self.inner)), h_last=after["h"], save=saved, pitches=pitches)
+        self.out = self._project(x, self.y, T, training, step)
+        return self.out
+
+    def backward(self, d_out: E.DeviceMatrix):
+        """Gradients of the parameters into `g` (and of the states into d_states, where there were any); returns d_x."""
+        e, p, g, d, T, B_ = self.eng, self.p, self.g, self.inner, d_out.shape[0], self._buf
+        parts, pitches = self._parts(self.uz, self.dbc)
+        d_proj = e.dropout(d_out, self.p_drop if self.training else 0.0, self.seed, 0, step=self.step_counter, out=B_("d_proj", (T, self.dim)))
+        v, mean, rstd = self.norm
+        d_v, _ = e.matmul_backward(v, p["Wout"], d_proj, dA=B_("d_v", (T, d)), dB=g["Wout"])
+        d_y, _, _ = e.group_norm_backward(self.y, mean, rstd, d_v, self.norm_groups, p["gamma"], p["beta"],
+                                          out=(B_("d_y", (T, d)), g["gamma"], g["beta"]))
+        d_uz, d_dbc = B_("d_uz", (T, 2 * d)), B_("d_dbc", (T, self.columns))
+        d_parts, _ = self._parts(d_uz, d_dbc)
+        d_c, d_delta = B_("d_c", (T, d)), B_("d_delta", (T, d))
+        out = {"u": d_c, "delta": d_delta, "z": d_parts["z"], "A": g["A"], "B": d_parts["B"], "C": d_parts["C"], "D": g["D"],
+               "delta_bias": g["bdt"]}
+        self.d_states = {}
+        if self.before["h"] is not None:
+            out["h0"] = self.d_states["h"] = B_("d_h", self.before["h"].shape)
+        e.selective_scan_backward(self.c, self.delta, p["A"], parts["B"], parts["C"], self.saved, d_y, p["D"], parts["z"], p["bdt"],
+                                  self.before["h"], groups=self.groups, **self.rows, out=out, pitches=pitches, gradient_pitches=pitches)
+        # delta = factor Wdt, factor the first columns of dbc
+        e.gemm(d_delta, p["Wdt"], d_dbc, transB=True, M=T, N=self.rank, K=d, lda=d, ldb=d, ldc=self.columns)
+        e.gemm(self.dbc, d_delta, g["Wdt"], transA=True, M=self.rank, N=d, K=T, lda=self.columns, ldb=d, ldc=d)
+        d_c2, _ = e.matmul_backward(self.c, p["Wx"], d_dbc, dA=B_("d_c2", (T, d)), dB=g["Wx"])
+        e.accumulate(d_c, d_c2)                                   # c feeds the scan and Wx
+        out = {"x": d_parts["u"], "w": g["Wc"], "bias": g["bc"]}
+        if self.before["conv"] is not None and self.width > 1:
+            out["state"] = self.d_states["conv"] = B_("d_conv", self.before["conv"].shape)
+        e.causal_conv_backward(parts["u"], p["Wc"], d_c, p["bc"], self.before["conv"], **self.rows, out=out, ld_x=2 * d, ld_dx=2 * d)
+        d_x, _ = e.matmul_backward(self.x, p["Win"], d_uz, dA=B_("d_x", (T, self.dim)), dB=g["Win"])
+        e.accumulate(d_x, d_out)                                  # the residual
+        self.d_x = d_x
+        return d_x
+
+    def step(self, x: E.DeviceMatrix, states):
+        """One new token [sequences x dim] for each sequence; `states` are replaced."""
+        e, p, T = self.eng, self.p, x.shape[0]
+        conv = lambda u, out: e.causal_conv_step(u, p["Wc"], states["conv"], p["bc"], out=out, ld_x=2 * self.inner)  # noqa: E731
+        uz, c, dbc, delta = self._mix(x, T, conv)
+        parts, pitches = self._parts(uz, dbc)
+        y = e.selective_scan_step(c, delta, p["A"], parts["B"], parts["C"], states["h"], p["D"], parts["z"], p["bdt"], groups=self.groups,
+                                  out=self._buf("y", (T, self.inner)), pitches=pitches)
+        return self._project(x, y, T, False, None)
