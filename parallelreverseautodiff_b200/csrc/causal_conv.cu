@@ -100,6 +100,7 @@ __device__ __forceinline__ void final_states(const Args<T>& a, int64_t block) {
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(THREADS)
 forward_kernel(const Args<T> a) {
+  chain_begin();
   if (blockIdx.x >= a.blocks) {
     if constexpr (W > 1) final_states<T, V, W>(a, blockIdx.x - a.blocks);
     return;
@@ -219,6 +220,7 @@ __device__ __forceinline__ void state_gradients(const Args<T>& a, int64_t block)
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(THREADS)
 backward_kernel(const Args<T> a, T* __restrict__ partial) {
+  chain_begin();
   if (blockIdx.x >= a.blocks) {
     if constexpr (W > 1) state_gradients<T, V, W>(a, blockIdx.x - a.blocks);
     return;
@@ -363,6 +365,7 @@ backward_kernel(const Args<T> a, T* __restrict__ partial) {
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 totals_kernel(const T* __restrict__ partial, int64_t blocks, int dim, int width, T* dw, T* dbias) {
+  chain_begin();
   __shared__ double part[WARPS][LANES];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * LANES + lane, k = blockIdx.y;
@@ -387,6 +390,7 @@ totals_kernel(const T* __restrict__ partial, int64_t blocks, int dim, int width,
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(THREADS)
 step_kernel(const Args<T> a, int64_t batch) {
+  chain_begin();
   const int c = (blockIdx.y * LANES + (threadIdx.x & 31)) * V;
   const int64_t s = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
   if (c >= a.dim || s >= batch) return;
@@ -414,7 +418,7 @@ enum class Pass { Forward, Backward, Step };
 template <typename T, int V, int W, bool BACKWARD> static prad_status launch(prad_ctx* ctx, Args<T> a, Pass pass) {
   const unsigned across = (unsigned)ceil_div(a.dim, LANES * V);
   if (!BACKWARD && pass == Pass::Step) {
-    step_kernel<T, V, W><<<dim3((unsigned)ceil_div(a.rows.tokens, WARPS), across), THREADS, 0, ctx->stream>>>(a, a.rows.tokens);
+    launch_chained(step_kernel<T, V, W>, dim3((unsigned)ceil_div(a.rows.tokens, WARPS), across), THREADS, 0, ctx->stream, a, a.rows.tokens);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
@@ -430,7 +434,7 @@ template <typename T, int V, int W, bool BACKWARD> static prad_status launch(pra
       constexpr int bytes = AHEAD * THREADS * V * (int)sizeof(T);
       prad_status st = allow_smem<forward_kernel<T, V, W>>(ctx, bytes);
       if (st) return st;
-      forward_kernel<T, V, W><<<dim3(grid, across), THREADS, bytes, ctx->stream>>>(a);
+      launch_chained(forward_kernel<T, V, W>, dim3(grid, across), THREADS, bytes, ctx->stream, a);
       PRAD_LAUNCHED(ctx);
     }
     return PRAD_OK;
@@ -443,13 +447,13 @@ template <typename T, int V, int W, bool BACKWARD> static prad_status launch(pra
       constexpr int bytes = 2 * AHEAD * THREADS * V * (int)sizeof(T);
       st = allow_smem<backward_kernel<T, V, W>>(ctx, bytes);
       if (st) return st;
-      backward_kernel<T, V, W><<<dim3(grid, across), THREADS, bytes, ctx->stream>>>(a, (T*)ctx->ws);
+      launch_chained(backward_kernel<T, V, W>, dim3(grid, across), THREADS, bytes, ctx->stream, a, (T*)ctx->ws);
       PRAD_LAUNCHED(ctx);
     } else if (states) {
       PRAD_CUDA(cudaMemsetAsync(a.dstate, 0, (size_t)a.rows.count * (W - 1) * a.dim * sizeof(T), ctx->stream));
     }
     if (a.dw || a.dbias) {
-      totals_kernel<T><<<dim3((unsigned)ceil_div(a.dim, LANES), W + 1), THREADS, 0, ctx->stream>>>((const T*)ctx->ws, a.blocks, a.dim, W,
+      launch_chained(totals_kernel<T>, dim3((unsigned)ceil_div(a.dim, LANES), W + 1), THREADS, 0, ctx->stream, (const T*)ctx->ws, a.blocks, a.dim, W,
                                                                                                 a.dw, a.dbias);
       PRAD_LAUNCHED(ctx);
     }

@@ -63,6 +63,7 @@ template <typename T, bool VECTOR, bool RESIDUAL>
 __global__ void __launch_bounds__(THREADS)
 dropout_kernel(const T* x, const T* residual, T* y, int64_t n, uint64_t keep, T scale, uint64_t seed, uint64_t offset,
                const uint64_t* step) {
+  chain_begin();
   if (step) offset += *step;
   const int64_t blocks = (n + 3) / 4, stride = (int64_t)gridDim.x * THREADS;
   for (int64_t b = (int64_t)blockIdx.x * THREADS + threadIdx.x; b < blocks; b += stride) {
@@ -88,7 +89,7 @@ static prad_status run(prad_ctx* ctx, const void* x, const void* residual, void*
   const int grid = stream_grid(ctx, (n + 3) / 4, THREADS, 8);
   auto kernel = vector ? (residual ? dropout_kernel<T, true, true> : dropout_kernel<T, true, false>)
                        : (residual ? dropout_kernel<T, false, true> : dropout_kernel<T, false, false>);
-  kernel<<<grid, THREADS, 0, ctx->stream>>>((const T*)x, (const T*)residual, (T*)y, n, keep, (T)scale, seed, offset, step);
+  launch_chained(kernel, grid, THREADS, 0, ctx->stream, (const T*)x, (const T*)residual, (T*)y, n, keep, (T)scale, seed, offset, step);
   PRAD_LAUNCHED(ctx);
   return PRAD_OK;
 }

@@ -50,6 +50,7 @@ template <int LW, typename A> __device__ __forceinline__ A lanes_sum(A v) {
 template <typename T, int V, int LW, int E>
 __global__ void __launch_bounds__(THREADS)
 rows_forward_kernel(const Args<T> a, int64_t slots) {
+  chain_begin();
   constexpr int R = E == 1 ? 4 : E == 2 ? 2 : 1;       // samples whose values are on their way at a time
   const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
   const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
@@ -124,6 +125,7 @@ rows_forward_kernel(const Args<T> a, int64_t slots) {
 template <typename T, int V, int LW, int E>
 __global__ void __launch_bounds__(THREADS)
 rows_backward_kernel(const Args<T> a, int64_t slots, T* __restrict__ partial) {
+  chain_begin();
   const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
   const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
   const int64_t step = slots / a.groups;
@@ -203,6 +205,7 @@ constexpr int TOTALS = 1024;
 template <typename P, typename T>
 __global__ void __launch_bounds__(TOTALS)
 column_totals_kernel(const P* __restrict__ partial, int64_t blocks, int channels, T* dgamma, T* dbeta) {
+  chain_begin();
   __shared__ double part[TOTALS / 32][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
@@ -328,6 +331,7 @@ __device__ __forceinline__ void statistics(const Args<T>& a, double pivot, doubl
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS)
 block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
+  chain_begin();
   __shared__ SumsShared<T, V> m;
   const Place<T> w(a, k, V);
   block_sums(a, w, m, [&](int g, double s1, double s2) {
@@ -340,6 +344,7 @@ block_sums_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 statistics_kernel(const Args<T> a, int64_t blocks, const double* __restrict__ sums) {
+  chain_begin();
   const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   if (i >= a.samples * a.groups) return;
   const int64_t s = i / a.groups;
@@ -390,6 +395,7 @@ __device__ __forceinline__ void apply(const Args<T>& a, const Place<T>& w, const
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS)
 apply_kernel(const Args<T> a, const Parts k) {
+  chain_begin();
   const Place<T> w(a, k, V);
   apply<T, V>(a, w, [&](int g, T& mean, T& rstd) {
     mean = a.mean[w.s * a.groups + w.g0 + g];
@@ -401,6 +407,7 @@ apply_kernel(const Args<T> a, const Parts k) {
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS)
 cluster_forward_kernel(const Args<T> a, const Parts k) {
+  chain_begin();
   __shared__ union { SumsShared<T, V> sums; T stats[THREADS][2]; } m;
   __shared__ double own[THREADS][2];
   cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
@@ -506,6 +513,7 @@ __device__ __forceinline__ void block_gradients(const Args<T>& a, const Parts& k
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS)
 block_gradients_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
+  chain_begin();
   __shared__ double part[2][THREADS * V];
   const Place<T> w(a, k, V);
   for (int q0 = 0; q0 < w.packs; q0 += THREADS) block_gradients<T, V>(a, k, w, q0, part, sums);
@@ -515,6 +523,7 @@ block_gradients_kernel(const Args<T> a, const Parts k, double* __restrict__ sums
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 group_gradients_kernel(const Args<T> a, int64_t blocks, const double* __restrict__ sums, double* __restrict__ means) {
+  chain_begin();
   const int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (i >= a.samples * a.groups) return;
@@ -579,6 +588,7 @@ __device__ __forceinline__ void input_gradients(const Args<T>& a, const Place<T>
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS)
 input_gradients_kernel(const Args<T> a, const Parts k, const double* __restrict__ means) {
+  chain_begin();
   const Place<T> w(a, k, V);
   input_gradients<T, V>(a, w, [&](int g, T& s1, T& s2) {
     const double* p = means + (w.s * a.groups + w.g0 + g) * 2;
@@ -591,6 +601,7 @@ input_gradients_kernel(const Args<T> a, const Parts k, const double* __restrict_
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 4 : 2)
 cluster_backward_kernel(const Args<T> a, const Parts k, double* __restrict__ sums) {
+  chain_begin();
   __shared__ double part[2][THREADS * V];
   __shared__ double own[THREADS][2];
   __shared__ T mine[THREADS][2];
@@ -659,16 +670,16 @@ template <typename T, int V, int LW, int E> static prad_status rows(prad_ctx* ct
   const int64_t grid = ceil_div(slots * LW, THREADS);
   PRAD_REQUIRE(grid <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "group norm: too many groups");
   if (!backward) {
-    rows_forward_kernel<T, V, LW, E><<<(unsigned)grid, THREADS, 0, ctx->stream>>>(a, slots);
+    launch_chained(rows_forward_kernel<T, V, LW, E>, (unsigned)grid, THREADS, 0, ctx->stream, a, slots);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
   prad_status st = ensure_workspace(ctx, (size_t)per_group * 2 * a.channels * sizeof(T));
   if (st) return st;
-  rows_backward_kernel<T, V, LW, E><<<(unsigned)grid, THREADS, 0, ctx->stream>>>(a, slots, (T*)ctx->ws);
+  launch_chained(rows_backward_kernel<T, V, LW, E>, (unsigned)grid, THREADS, 0, ctx->stream, a, slots, (T*)ctx->ws);
   PRAD_LAUNCHED(ctx);
   if (a.dgamma || a.dbeta) {
-    column_totals_kernel<T, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream>>>((const T*)ctx->ws, per_group,
+    launch_chained(column_totals_kernel<T, T>, dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream, (const T*)ctx->ws, per_group,
                                                                                                       a.channels, a.dgamma, a.dbeta);
     PRAD_LAUNCHED(ctx);
   }
@@ -685,19 +696,21 @@ template <typename T, int V> static prad_status pick_rows(prad_ctx* ctx, const A
   return rows<T, V, 32, 8>(ctx, a, backward);
 }
 
-// A cluster's CTAs on the device's SMs at the same time (grid.x: a multiple of `ctas`).
+// launch_chained with clusters of `ctas` CTAs (grid.x: a multiple of them).
 template <typename... P, typename... A>
 static void launch_clusters(void (*kernel)(P...), dim3 grid, unsigned ctas, cudaStream_t stream, A&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = ctas;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = grid;
   cfg.blockDim = THREADS;
   cfg.stream = stream;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);     // (PRAD_LAUNCHED looks at the error)
 }
 
@@ -736,7 +749,7 @@ template <typename T, int V> static prad_status blocks(prad_ctx* ctx, Args<T> a,
     launch_clusters(cluster_backward_kernel<T, V>, grid, ctas, ctx->stream, a, k, (double*)ctx->ws);
     PRAD_LAUNCHED(ctx);
     if (a.dgamma || a.dbeta) {
-      column_totals_kernel<double, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream>>>(
+      launch_chained(column_totals_kernel<double, T>, dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream,
           (const double*)ctx->ws, a.samples * ctas, a.channels, a.dgamma, a.dbeta);
       PRAD_LAUNCHED(ctx);
     }
@@ -761,13 +774,13 @@ template <typename T, int V> static prad_status blocks(prad_ctx* ctx, Args<T> a,
   if (!backward) {
     prad_status st = ensure_workspace(ctx, (size_t)(a.samples * k.blocks * a.groups) * 2 * sizeof(double));
     if (st) return st;
-    block_sums_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k, (double*)ctx->ws);
+    launch_chained(block_sums_kernel<T, V>, grid, THREADS, 0, ctx->stream, a, k, (double*)ctx->ws);
     PRAD_LAUNCHED(ctx);
-    statistics_kernel<T><<<(unsigned)ceil_div(each, THREADS), THREADS, 0, ctx->stream>>>(a, k.blocks, (const double*)ctx->ws);
+    launch_chained(statistics_kernel<T>, (unsigned)ceil_div(each, THREADS), THREADS, 0, ctx->stream, a, k.blocks, (const double*)ctx->ws);
     PRAD_LAUNCHED(ctx);
     a.mean = a.mean_out;
     a.rstd = a.rstd_out;
-    apply_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k);
+    launch_chained(apply_kernel<T, V>, grid, THREADS, 0, ctx->stream, a, k);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
@@ -775,14 +788,14 @@ template <typename T, int V> static prad_status blocks(prad_ctx* ctx, Args<T> a,
   prad_status st = ensure_workspace(ctx, (columns + (size_t)each * 2) * sizeof(double));
   if (st) return st;
   double *sums = (double*)ctx->ws, *means = sums + columns;
-  block_gradients_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k, sums);
+  launch_chained(block_gradients_kernel<T, V>, grid, THREADS, 0, ctx->stream, a, k, sums);
   PRAD_LAUNCHED(ctx);
-  group_gradients_kernel<T><<<(unsigned)ceil_div(each * 32, THREADS), THREADS, 0, ctx->stream>>>(a, k.blocks, sums, means);
+  launch_chained(group_gradients_kernel<T>, (unsigned)ceil_div(each * 32, THREADS), THREADS, 0, ctx->stream, a, k.blocks, sums, means);
   PRAD_LAUNCHED(ctx);
-  input_gradients_kernel<T, V><<<grid, THREADS, 0, ctx->stream>>>(a, k, means);
+  launch_chained(input_gradients_kernel<T, V>, grid, THREADS, 0, ctx->stream, a, k, means);
   PRAD_LAUNCHED(ctx);
   if (a.dgamma || a.dbeta) {
-    column_totals_kernel<double, T><<<dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream>>>(
+    launch_chained(column_totals_kernel<double, T>, dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream,
         sums, a.samples * k.blocks, a.channels, a.dgamma, a.dbeta);
     PRAD_LAUNCHED(ctx);
   }

@@ -250,34 +250,43 @@ template <int TT> __device__ __forceinline__ uint32_t starts_in(const Sequences&
   return mask;
 }
 
-// B or C rows of a tile, by asynchronous copies; rows without a token are zero
-template <typename T, int N, int TT>
-__device__ __forceinline__ void fetch_rows(T (*to)[N], const T* from, int64_t ld, int first, int state, int wide, int64_t tile0, int begin,
-                                           int finish) {
-  constexpr int V = 16 / sizeof(T);
-  from += tile0 * ld + first;
-  if (wide && N % V == 0) {
+// B or C rows of tiles, by asynchronous copies; rows without a token are zero
+template <typename T, int N, int TT> struct Rows {
+  static constexpr int V = 16 / sizeof(T), ACROSS = N / V, AT_ONCE = THREADS / ACROSS;
+  const T *at, *valid;
+  int64_t ld;
+  int row, n, state;
+  bool wide;
+  __device__ __forceinline__ Rows(const T* from, int64_t ld, int first, int state, int wide, int64_t tile0)
+      : valid(from), ld(ld), row(threadIdx.x / ACROSS), n(threadIdx.x % ACROSS * V), state(state), wide(wide) {
+    at = from + tile0 * ld + first;
+  }
+  // rows [begin, finish) of the tile that `at` is at
+  __device__ __forceinline__ void fetch(T (*to)[N], int begin, int finish) const {
+    if (wide) {
+      if (ACROSS * AT_ONCE != THREADS && row >= AT_ONCE) return;
 #pragma unroll
-    for (int i = 0; i < (TT * N / V + THREADS - 1) / THREADS; ++i) {
-      const int e = threadIdx.x + i * THREADS, t = e / (N / V), n = e % (N / V) * V;
-      if (TT * N / V % THREADS != 0 && e >= TT * N / V) break;
-      const bool live = t >= begin && t < finish && n < state;
-      const uint32_t d = (uint32_t)__cvta_generic_to_shared(&to[t][n]);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from + (live ? t * ld + n : begin * ld)), "r"(live ? 16 : 0)
+      for (int t0 = 0; t0 < TT; t0 += AT_ONCE) {
+        const int t = t0 + row;
+        if (TT % AT_ONCE != 0 && t >= TT) break;
+        const bool live = t >= begin && t < finish && n < state;
+        const uint32_t d = (uint32_t)__cvta_generic_to_shared(&to[t][n]);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(live ? at + t * ld + n : valid), "r"(live ? 16 : 0)
+                     : "memory");
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int e = threadIdx.x; e < TT * N; e += THREADS) {
+      const int t = e / N, k = e % N;
+      const bool live = t >= begin && t < finish && k < state;
+      const uint32_t d = (uint32_t)__cvta_generic_to_shared(&to[t][k]);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(live ? at + t * ld + k : valid), "n"((int)sizeof(T)),
+                   "r"(live ? (int)sizeof(T) : 0)
                    : "memory");
     }
-    return;
   }
-#pragma unroll 1
-  for (int e = threadIdx.x; e < TT * N; e += THREADS) {
-    const int t = e / N, n = e % N;
-    const bool live = t >= begin && t < finish && n < state;
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(&to[t][n]);
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(from + (live ? t * ld + n : begin * ld)),
-                 "n"((int)sizeof(T)), "r"(live ? (int)sizeof(T) : 0)
-                 : "memory");
-  }
-}
+};
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void landed() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
@@ -306,40 +315,43 @@ template <typename T, int CH, int TT> struct Cells {
   }
   // whether row e of this thread lies in the tile
   __device__ __forceinline__ bool in(int e) const { return ROWS <= TT || row < TT; }
+  // this thread's first value of a tile
+  __device__ __forceinline__ int64_t first(int64_t ld, int64_t tile0) const { return (tile0 + row) * ld + col; }
   // rows [from, to) of the tile; what lies outside, and channels that do not exist, as zero
-  __device__ __forceinline__ void load(const T* tile, int64_t ld, int from, int to, T (&v)[E][V]) const {
-    const T* at = tile + row * ld + col;
+  __device__ __forceinline__ void load(const T* at, int64_t ld, int from, int to, T (&v)[E][V]) const {
+    if (wide && to - from == TT && ROWS <= TT) {
 #pragma unroll
-    for (int e = 0; e < E; ++e, at += ROWS * ld) {
-      const bool live = row + e * ROWS >= from && row + e * ROWS < to;
-      if (wide) {
-        Pack<T, V> w;
-#pragma unroll
-        for (int j = 0; j < V; ++j) w.v[j] = 0;
-        if (live) w = *reinterpret_cast<const Pack<T, V>*>(at);
+      for (int e = 0; e < E; ++e, at += ROWS * ld) {
+        const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(at);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[e][j] = w.v[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[e][j] = live && j < mine ? at[j] : (T)0;
       }
+      return;
     }
-  }
-  __device__ __forceinline__ void store(T* tile, int64_t ld, int from, int to, const T (&v)[E][V]) const {
-    T* at = tile + row * ld + col;
 #pragma unroll
     for (int e = 0; e < E; ++e, at += ROWS * ld) {
       const bool live = row + e * ROWS >= from && row + e * ROWS < to;
-      if (wide) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[e][j] = live && j < mine ? at[j] : (T)0;
+    }
+  }
+  __device__ __forceinline__ void store(T* at, int64_t ld, int from, int to, const T (&v)[E][V]) const {
+    if (wide && to - from == TT && ROWS <= TT) {
+#pragma unroll
+      for (int e = 0; e < E; ++e, at += ROWS * ld) {
         Pack<T, V> w;
 #pragma unroll
         for (int j = 0; j < V; ++j) w.v[j] = v[e][j];
-        if (live) *reinterpret_cast<Pack<T, V>*>(at) = w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (live && j < mine) at[j] = v[e][j];
+        *reinterpret_cast<Pack<T, V>*>(at) = w;
       }
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e, at += ROWS * ld) {
+      const bool live = row + e * ROWS >= from && row + e * ROWS < to;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (live && j < mine) at[j] = v[e][j];
     }
   }
   // one value per channel
@@ -351,6 +363,8 @@ template <typename T, int CH, int TT> struct Cells {
 // Where channel c's entry of 16 bytes lies in a row of shared memory: threads that write V channels each, and warps that read eight,
 // spread over all banks.
 template <typename T> __device__ __forceinline__ int spot(int c) { return c ^ (c >> 3 & (16 / (int)sizeof(T) - 1)); }
+// the same of channel col + j, j < V, for a thread's first channel
+template <typename T> __device__ __forceinline__ int spot(int col, int j) { return col + (j ^ (col >> 3 & (16 / (int)sizeof(T) - 1))); }
 // V values side by side in shared memory
 template <int V, typename T> __device__ __forceinline__ void put(T* m, const T (&v)[V]) {
   Pack<T, V> w;
@@ -376,6 +390,7 @@ template <typename T, int L, int S> struct Forward {
 template <typename T, int L, int S, bool EDGES>
 __global__ void __launch_bounds__(THREADS, 4)
 forward_kernel(const Args<T> a) {
+  chain_begin();
   constexpr int CH = THREADS / L, TT = tile<T, L>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
   Forward<T, L, S>& m = *reinterpret_cast<Forward<T, L, S>*>(raw);
@@ -436,13 +451,28 @@ forward_kernel(const Args<T> a) {
     T u[E][V], d[E][V], z[E][V], bias[V], D[V];
     mine.per_channel(a.bias ? a.bias + me.c0 : nullptr, bias);
     mine.per_channel(!EDGES && a.D ? a.D + me.c0 : nullptr, D);
-    const auto fetch = [&](int64_t tile0) {
+    const T* pu = a.u + me.c0 + mine.first(a.ld_u, tiles0);
+    const T* pd = a.delta + me.c0 + mine.first(a.ld_delta, tiles0);
+    const T* pz = a.z ? a.z + me.c0 + mine.first(a.ld_z, tiles0) : nullptr;
+    T* py = EDGES ? nullptr : a.y + me.c0 + mine.first(a.ld_y, tiles0);
+    Rows<T, N, TT> B_rows(a.B, a.ld_B, me.q * a.state, a.state, a.wide_B, tiles0);
+    Rows<T, N, TT> C_rows(a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, tiles0);
+    const auto fetch = [&](int64_t tile0) {      // of the tiles in turn
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      mine.load(a.u + tile0 * a.ld_u + me.c0, a.ld_u, from, to, u);
-      mine.load(a.delta + tile0 * a.ld_delta + me.c0, a.ld_delta, from, to, d);
-      if (!EDGES && a.z) mine.load(a.z + tile0 * a.ld_z + me.c0, a.ld_z, from, to, z);
-      fetch_rows<T, N, TT>(m.B[tile0 / TT & 1], a.B, a.ld_B, me.q * a.state, a.state, a.wide_B, tile0, from, to);
-      if (!EDGES) fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, tile0, from, to);
+      mine.load(pu, a.ld_u, from, to, u);
+      mine.load(pd, a.ld_delta, from, to, d);
+      pu += TT * a.ld_u;
+      pd += TT * a.ld_delta;
+      B_rows.fetch(m.B[tile0 / TT & 1], from, to);
+      B_rows.at += TT * a.ld_B;
+      if (!EDGES) {
+        if (a.z) {
+          mine.load(pz, a.ld_z, from, to, z);
+          pz += TT * a.ld_z;
+        }
+        C_rows.fetch(m.C[tile0 / TT & 1], from, to);
+        C_rows.at += TT * a.ld_C;
+      }
     };
     fetch(tiles0);
     commit();
@@ -459,7 +489,7 @@ forward_kernel(const Args<T> a) {
           T dt = d[e][j] + bias[j];
           if (a.softplus) dt = softplus(dt);
           if (!live) dt = 0;
-          if (mine.in(e)) write(&m.step[r][spot<T>(mine.col + j)], dt, dt * u[e][j]);
+          if (mine.in(e)) write(&m.step[r][spot<T>(mine.col, j)], dt, dt * u[e][j]);
           kept_u[e][j] = u[e][j];
           if (!EDGES) kept_z[e][j] = z[e][j];
         }
@@ -542,7 +572,8 @@ forward_kernel(const Args<T> a) {
             if (a.z) y[e][j] *= swish(kept_z[e][j]);
           }
         }
-        mine.store(a.y + tile0 * a.ld_y + me.c0, a.ld_y, from, to, y);
+        mine.store(py, a.ld_y, from, to, y);
+        py += TT * a.ld_y;
       }
     }
     landed<0>();
@@ -566,6 +597,7 @@ constexpr int JOINED = 8;
 template <typename T, bool FORWARD>
 __global__ void __launch_bounds__(32 * JOINED)
 join_kernel(const Args<T> a) {
+  chain_begin();
   __shared__ T s_own[JOINED][33], s_through[JOINED][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int k = threadIdx.x / JOINED;                  // of the reading and writing: span k, state i
@@ -619,6 +651,7 @@ template <typename T, int L, int S> struct Edges {
 template <typename T, int L, int S>
 __global__ void __launch_bounds__(THREADS, 4)
 backward_edges_kernel(const Args<T> a) {
+  chain_begin();
   constexpr int CH = THREADS / L, TT = tile<T, L>(), N = L * S, P = S / 2;
   extern __shared__ __align__(16) unsigned char raw[];
   Edges<T, L, S>& m = *reinterpret_cast<Edges<T, L, S>*>(raw);
@@ -644,14 +677,24 @@ backward_edges_kernel(const Args<T> a) {
     constexpr int E = Cells<T, CH, TT>::E, V = Cells<T, CH, TT>::V, ROWS = Cells<T, CH, TT>::ROWS;
     T d[E][V], v[E][V], z[E][V], bias[V];
     mine.per_channel(a.bias ? a.bias + me.c0 : nullptr, bias);
-    const auto fetch = [&](int64_t tile0) {
-      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      mine.load(a.delta + tile0 * a.ld_delta + me.c0, a.ld_delta, from, to, d);
-      mine.load(a.dy + tile0 * a.ld_dy + me.c0, a.ld_dy, from, to, v);
-      if (a.z) mine.load(a.z + tile0 * a.ld_z + me.c0, a.ld_z, from, to, z);
-      fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, tile0, from, to);
-    };
     const int64_t top = (finish - 1) / TT * TT, bottom = begin / TT * TT;
+    const T* pd = a.delta + me.c0 + mine.first(a.ld_delta, top);
+    const T* pv = a.dy + me.c0 + mine.first(a.ld_dy, top);
+    const T* pz = a.z ? a.z + me.c0 + mine.first(a.ld_z, top) : nullptr;
+    Rows<T, N, TT> C_rows(a.C, a.ld_C, me.q * a.state, a.state, a.wide_C, top);
+    const auto fetch = [&](int64_t tile0) {      // of the tiles in turn, from the last one
+      const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
+      mine.load(pd, a.ld_delta, from, to, d);
+      mine.load(pv, a.ld_dy, from, to, v);
+      pd -= TT * a.ld_delta;
+      pv -= TT * a.ld_dy;
+      if (a.z) {
+        mine.load(pz, a.ld_z, from, to, z);
+        pz -= TT * a.ld_z;
+      }
+      C_rows.fetch(m.C[tile0 / TT & 1], from, to);
+      C_rows.at -= TT * a.ld_C;
+    };
     fetch(top);
     commit();
     for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT) {
@@ -665,7 +708,7 @@ backward_edges_kernel(const Args<T> a) {
           T dt = d[e0][j] + bias[j];
           if (a.softplus) dt = softplus(dt);
           if (!live) dt = 0;
-          if (mine.in(e0)) write(&m.step[r][spot<T>(mine.col + j)], dt, a.z ? v[e0][j] * swish(z[e0][j]) : v[e0][j]);
+          if (mine.in(e0)) write(&m.step[r][spot<T>(mine.col, j)], dt, a.z ? v[e0][j] * swish(z[e0][j]) : v[e0][j]);
         }
       }
       if (tile0 > bottom) fetch(tile0 - TT);
@@ -750,6 +793,7 @@ __device__ __forceinline__ void read_step(const double* m, Two<double>& dt, Two<
 template <typename T, int L, int S>
 __global__ void __launch_bounds__(THREADS, 2)
 backward_kernel(const Args<T> a) {
+  chain_begin();
   using K = Backward<T, L, S>;
   constexpr int CC = K::CC, HALF = K::HALF, CH = K::CH, TT = K::TT, N = K::N, P = K::P, FT = K::FT;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -807,14 +851,31 @@ backward_kernel(const Args<T> a) {
     const int64_t top = (finish - 1) / TT * TT, bottom = begin / TT * TT;
     T u[E][V], d[E][V], z[E][V], dy[E][V];
     Two<T> next[CC][P];                         // the checkpoint of the tile that is fetched
-    const auto fetch = [&](int64_t tile0) {
+    const T* pu = a.u + c0 + mine.first(a.ld_u, top);
+    const T* pd = a.delta + c0 + mine.first(a.ld_delta, top);
+    const T* pv = a.dy + c0 + mine.first(a.ld_dy, top);
+    const T* pz = a.z ? a.z + c0 + mine.first(a.ld_z, top) : nullptr;
+    T* to_u = a.du + c0 + mine.first(a.ld_du, top);
+    T* to_d = a.ddelta + c0 + mine.first(a.ld_ddelta, top);
+    T* to_z = a.z ? a.dz + c0 + mine.first(a.ld_dz, top) : nullptr;
+    Rows<T, N, TT> B_rows(a.B, a.ld_B, q * a.state, a.state, a.wide_B, top);
+    Rows<T, N, TT> C_rows(a.C, a.ld_C, q * a.state, a.state, a.wide_C, top);
+    const auto fetch = [&](int64_t tile0) {      // of the tiles in turn, from the last one
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      mine.load(a.u + tile0 * a.ld_u + c0, a.ld_u, from, to, u);
-      mine.load(a.delta + tile0 * a.ld_delta + c0, a.ld_delta, from, to, d);
-      mine.load(a.dy + tile0 * a.ld_dy + c0, a.ld_dy, from, to, dy);
-      if (a.z) mine.load(a.z + tile0 * a.ld_z + c0, a.ld_z, from, to, z);
-      fetch_rows<T, N, TT>(m.B[tile0 / TT & 1], a.B, a.ld_B, q * a.state, a.state, a.wide_B, tile0, from, to);
-      fetch_rows<T, N, TT>(m.C[tile0 / TT & 1], a.C, a.ld_C, q * a.state, a.state, a.wide_C, tile0, from, to);
+      mine.load(pu, a.ld_u, from, to, u);
+      mine.load(pd, a.ld_delta, from, to, d);
+      mine.load(pv, a.ld_dy, from, to, dy);
+      pu -= TT * a.ld_u;
+      pd -= TT * a.ld_delta;
+      pv -= TT * a.ld_dy;
+      if (a.z) {
+        mine.load(pz, a.ld_z, from, to, z);
+        pz -= TT * a.ld_z;
+      }
+      B_rows.fetch(m.B[tile0 / TT & 1], from, to);
+      C_rows.fetch(m.C[tile0 / TT & 1], from, to);
+      B_rows.at -= TT * a.ld_B;
+      C_rows.at -= TT * a.ld_C;
 #pragma unroll
       for (int k = 0; k < CC; ++k) load(from == 0 ? a.saved + tile0 / TT * states : nullptr, k, next[k]);
     };
@@ -845,7 +906,7 @@ backward_kernel(const Args<T> a) {
             v[j] *= z[i][j] * g;
           }
           const typename K::Step st = {dt, dt, dt * u[i][j], dt * u[i][j]};
-          if (mine.in(i)) m.step[r][spot<T>(mine.col + j)] = st;
+          if (mine.in(i)) m.step[r][spot<T>(mine.col, j)] = st;
         }
         if (mine.in(i)) {
           put(&m.v[r][mine.col], v);
@@ -942,11 +1003,11 @@ backward_kernel(const Args<T> a) {
           now[k][j] = h[k][j];
         }
       for (int f = TT - FT; f >= 0; f -= FT) {
-#pragma unroll 1
+#pragma unroll 2
         for (int t0 = f + FT - 2; t0 >= f; t0 -= 2) {
-          T two[CC][4] = {};
+          T two[CC][4];
           // one token: its gradients from the state in front of it
-          const auto token = [&](int t, const Two<T>(&before)[CC][P], T(&sums)[CC][2]) {
+          const auto token = [&](int t, const Two<T>(&behind)[CC][P], const Two<T>(&before)[CC][P], T(&sums)[CC][2]) {
             Two<T> B[P], C[P], dB[P], dC[P];
             read(&rows_B[t][n0], B);
             read(&rows_C[t][n0], C);
@@ -965,7 +1026,7 @@ backward_kernel(const Args<T> a) {
                 gA = j ? fma(w, A[k][j], gA) : mul(w, A[k][j]);
                 tile_dA[k][j] = fma(w, dt, tile_dA[k][j]);
                 dB[j] = k ? fma(g, x, dB[j]) : mul(g, x);
-                dC[j] = k ? fma(now[k][j], v, dC[j]) : mul(now[k][j], v);
+                dC[j] = k ? fma(behind[k][j], v, dC[j]) : mul(behind[k][j], v);
               }
               sums[k][0] = total(gB);
               sums[k][1] = total(gA);
@@ -993,17 +1054,17 @@ backward_kernel(const Args<T> a) {
           in_front(t0, zero);
           if ((starts >> t0 & 3) == 0) {
             T sums[2][CC][2];
-            token(t0 + 1, one, sums[1]);
-#pragma unroll
-            for (int k = 0; k < CC; ++k)
-#pragma unroll
-              for (int j = 0; j < P; ++j) now[k][j] = one[k][j];
-            token(t0, zero, sums[0]);
+            token(t0 + 1, now, one, sums[1]);
+            token(t0, one, zero, sums[0]);
 #pragma unroll
             for (int k = 0; k < CC; ++k)
 #pragma unroll
               for (int j = 0; j < 4; ++j) two[k][j] = sums[j / 2][k][j % 2];
           } else {
+#pragma unroll
+            for (int k = 0; k < CC; ++k)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) two[k][j] = 0;
 #pragma unroll 1
             for (int i = 1; i >= 0; --i) {
               const bool begins = starts >> (t0 + i) & 1;
@@ -1015,7 +1076,7 @@ backward_kernel(const Args<T> a) {
                 for (int j = 0; j < P; ++j) before[k][j] = i ? one[k][j] : zero[k][j];
                 if (begins) load(initial(t0 + i), k, before[k]);
               }
-              token(t0 + i, before, sums);
+              token(t0 + i, now, before, sums);
 #pragma unroll
               for (int k = 0; k < CC; ++k) {
 #pragma unroll
@@ -1075,8 +1136,9 @@ backward_kernel(const Args<T> a) {
       T du[E][V], dd[E][V], dz[E][V];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int r = mine.in(i) ? mine.row + i * ROWS : 0;
-        const bool live = mine.in(i) && r >= from && r < to;
+        if (!mine.in(i)) break;
+        const int r = mine.row + i * ROWS;
+        const bool live = r >= from && r < to;
         T ut[V], v[V], slope[V], w[V], rt[V];
         pick(&m.u[r][mine.col], ut);
         pick(&m.v[r][mine.col], v);
@@ -1085,7 +1147,7 @@ backward_kernel(const Args<T> a) {
         pick(&m.r[r][mine.col], rt);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const typename K::Step st = m.step[r][spot<T>(mine.col + j)];
+          const typename K::Step st = m.step[r][spot<T>(mine.col, j)];
           du[i][j] = st.dt * st.gB + D[j] * v[j];
           dd[i][j] = (ut[j] * st.gB + per_rate<T>() * st.gA) * slope[j];
           dz[i][j] = w[j] * (rt[j] + D[j] * ut[j]);
@@ -1095,10 +1157,15 @@ backward_kernel(const Args<T> a) {
           }
         }
       }
-      mine.store(a.du + tile0 * a.ld_du + c0, a.ld_du, from, to, du);
-      mine.store(a.ddelta + tile0 * a.ld_ddelta + c0, a.ld_ddelta, from, to, dd);
-      if (a.z) mine.store(a.dz + tile0 * a.ld_dz + c0, a.ld_dz, from, to, dz);
-      __syncthreads();
+      mine.store(to_u, a.ld_du, from, to, du);
+      mine.store(to_d, a.ld_ddelta, from, to, dd);
+      to_u -= TT * a.ld_du;
+      to_d -= TT * a.ld_ddelta;
+      if (a.z) {
+        mine.store(to_z, a.ld_dz, from, to, dz);
+        to_z -= TT * a.ld_dz;
+      }
+      // (no barrier: a thread alone reads and writes its cells of the tile, here and where the next tile's go in)
     }
     landed<0>();
   }
@@ -1126,6 +1193,7 @@ backward_kernel(const Args<T> a) {
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 span_totals_kernel(const Args<T> a) {
+  chain_begin();
   int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   const int64_t states = (int64_t)a.dim * a.state;
   const T* from = a.part_A;
@@ -1151,6 +1219,7 @@ span_totals_kernel(const Args<T> a) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 row_totals_kernel(const Args<T> a) {
+  chain_begin();
   const int64_t lo = a.rows.begin(), hi = a.rows.finish(), each = (int64_t)a.groups * 2 * a.state;
   const int64_t i = lo * each + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= hi * each) return;
@@ -1168,6 +1237,7 @@ row_totals_kernel(const Args<T> a) {
 template <typename T, int L, int S, int R>
 __global__ void __launch_bounds__(THREADS)
 step_kernel(const Args<T> a) {
+  chain_begin();
   const Place<T, L, S> me(a);
   const int c = me.c0 + me.ch;
   const int64_t row0 = (int64_t)blockIdx.y * R, states = (int64_t)a.dim * a.state;
@@ -1298,8 +1368,8 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
       if (b.z) b.z += r0 * a.ld_z;
       b.h0 += r0 * states, b.h_last += r0 * states;
       const dim3 grid((unsigned)across, (unsigned)ceil_div(b.rows.tokens, R));
-      if (R == 1) step_kernel<T, L, S, 1><<<grid, THREADS, 0, ctx->stream>>>(b);
-      else step_kernel<T, L, S, 4><<<grid, THREADS, 0, ctx->stream>>>(b);
+      if (R == 1) launch_chained(step_kernel<T, L, S, 1>, grid, THREADS, 0, ctx->stream, b);
+      else launch_chained(step_kernel<T, L, S, 4>, grid, THREADS, 0, ctx->stream, b);
       PRAD_LAUNCHED(ctx);
     }
     return PRAD_OK;
@@ -1318,12 +1388,12 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   const unsigned x = (unsigned)across;
   if (!backward) {
     if (joined(a)) {
-      forward_kernel<T, FL, FS, true><<<dim3(x, (unsigned)a.spans - 1), THREADS, bytes, ctx->stream>>>(a);
+      launch_chained(forward_kernel<T, FL, FS, true>, dim3(x, (unsigned)a.spans - 1), THREADS, bytes, ctx->stream, a);
       PRAD_LAUNCHED(ctx);
-      join_kernel<T, true><<<(unsigned)ceil_div(states, JOINED), 32 * JOINED, 0, ctx->stream>>>(a);
+      launch_chained(join_kernel<T, true>, (unsigned)ceil_div(states, JOINED), 32 * JOINED, 0, ctx->stream, a);
       PRAD_LAUNCHED(ctx);
     }
-    forward_kernel<T, FL, FS, false><<<dim3(x, (unsigned)a.spans), THREADS, bytes, ctx->stream>>>(a);
+    launch_chained(forward_kernel<T, FL, FS, false>, dim3(x, (unsigned)a.spans), THREADS, bytes, ctx->stream, a);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
@@ -1331,18 +1401,18 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   if (joined(a)) {
     Args<T> b = a;
     b.blocks = edge_blocks;
-    backward_edges_kernel<T, L, S><<<dim3((unsigned)(a.groups * edge_blocks), (unsigned)a.spans), THREADS, edge_bytes, ctx->stream>>>(b);
+    launch_chained(backward_edges_kernel<T, L, S>, dim3((unsigned)(a.groups * edge_blocks), (unsigned)a.spans), THREADS, edge_bytes, ctx->stream, b);
     PRAD_LAUNCHED(ctx);
-    join_kernel<T, false><<<(unsigned)ceil_div(states, JOINED), 32 * JOINED, 0, ctx->stream>>>(a);
+    launch_chained(join_kernel<T, false>, (unsigned)ceil_div(states, JOINED), 32 * JOINED, 0, ctx->stream, a);
     PRAD_LAUNCHED(ctx);
   }
-  backward_kernel<T, L, S><<<dim3(x, (unsigned)a.spans), THREADS, sizeof(Shared), ctx->stream>>>(a);
+  launch_chained(backward_kernel<T, L, S>, dim3(x, (unsigned)a.spans), THREADS, sizeof(Shared), ctx->stream, a);
   PRAD_LAUNCHED(ctx);
-  span_totals_kernel<T><<<(unsigned)ceil_div(states + 2 * (int64_t)a.dim, THREADS), THREADS, 0, ctx->stream>>>(a);
+  launch_chained(span_totals_kernel<T>, (unsigned)ceil_div(states + 2 * (int64_t)a.dim, THREADS), THREADS, 0, ctx->stream, a);
   PRAD_LAUNCHED(ctx);
   if (a.blocks > 1 && a.rows.tokens) {
     const int64_t n = a.rows.tokens * a.groups * 2 * a.state;
-    row_totals_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, ctx->stream>>>(a);
+    launch_chained(row_totals_kernel<T>, (unsigned)ceil_div(n, 256), 256, 0, ctx->stream, a);
     PRAD_LAUNCHED(ctx);
   }
   return PRAD_OK;
