@@ -27,12 +27,21 @@ template <typename T> struct Args {
   int64_t samples, positions;
   int channels, groups, per;     // per: channels of a group
   double eps;
-  int act;
+  int act, wide;                 // wide: gamma and beta can be read as many values at a time as x
 };
 
 __host__ __device__ inline int64_t ceil_rounds(int64_t n, int64_t by) { return (n + by - 1) / by; }
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+
+// V values of gamma or beta from channel c on; `none` without any
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> parameters(const Args<T>& a, const T* p, int c, T none) {
+  Pack<T, V> r;
+  if (p && a.wide) return load<T, V>(p + c);
+#pragma unroll
+  for (int j = 0; j < V; ++j) r.v[j] = p ? p[c + j] : none;
+  return r;
+}
 
 __device__ __forceinline__ float inverse_root(float x) { return rsqrtf(x); }
 __device__ __forceinline__ double inverse_root(double x) { return 1.0 / sqrt(x); }
@@ -47,11 +56,13 @@ template <int LW, typename A> __device__ __forceinline__ A lanes_sum(A v) {
   return v;
 }
 
+// samples of a slot in the forward pass, whose values are on their way at the same time
+template <int E> constexpr int rows_at_once() { return E == 1 ? 4 : E == 2 ? 2 : 1; }
 template <typename T, int V, int LW, int E>
 __global__ void __launch_bounds__(THREADS)
 rows_forward_kernel(const Args<T> a, int64_t slots) {
   chain_begin();
-  constexpr int R = E == 1 ? 4 : E == 2 ? 2 : 1;       // samples whose values are on their way at a time
+  constexpr int R = rows_at_once<E>();
   const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
   const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
   const int64_t step = slots / a.groups;
@@ -62,60 +73,56 @@ rows_forward_kernel(const Args<T> a, int64_t slots) {
   for (int e = 0; e < E; ++e) {
     c[e] = (l + e * LW) * V;
     on[e] = c[e] < a.per;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      gamma[e].v[j] = on[e] && a.gamma ? a.gamma[g * a.per + c[e] + j] : (T)1;
-      beta[e].v[j] = on[e] && a.beta ? a.beta[g * a.per + c[e] + j] : (T)0;
+    if (on[e]) {
+      gamma[e] = parameters<T, V>(a, a.gamma, g * a.per + c[e], (T)1);
+      beta[e] = parameters<T, V>(a, a.beta, g * a.per + c[e], (T)0);
     }
   }
   // all lanes of a warp take part in its sums: those beyond the last sample with nothing to add
   const int64_t first = slot < slots ? slot / a.groups : a.samples;
-  const int64_t rounds = ceil_rounds(a.samples, step * R);
   const T inv = (T)1 / (T)a.per, eps = (T)a.eps;
-  for (int64_t k = 0; k < rounds; ++k) {
-    Pack<T, V> x[R][E];
+  Pack<T, V> x[R][E];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int64_t s = first + (k * R + r) * step;
+    for (int e = 0; e < E; ++e) {
+      const int64_t s = first + r * step;
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[r][e].v[j] = 0;
-        if (s < a.samples && on[e]) x[r][e] = load<T, V>(a.x + s * a.channels + (int64_t)g * a.per + c[e]);
+      for (int j = 0; j < V; ++j) x[r][e].v[j] = 0;
+      if (s < a.samples && on[e]) x[r][e] = load<T, V>(a.x + s * a.channels + (int64_t)g * a.per + c[e]);
+    }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t s = first + r * step;
+    T sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += x[r][e].v[j];
+    const T mean = lanes_sum<LW>(sum) * inv;
+    T sq = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const T d = x[r][e].v[j] - mean;
+        if (on[e]) sq += d * d;
       }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t s = first + (k * R + r) * step;
-      T sum = 0;
+    const T rstd = inverse_root(lanes_sum<LW>(sq) * inv + eps);
+    if (s < a.samples) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
+        if (on[e]) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum += x[r][e].v[j];
-      const T mean = lanes_sum<LW>(sum) * inv;
-      T sq = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const T d = x[r][e].v[j] - mean;
-          if (on[e]) sq += d * d;
-        }
-      const T rstd = inverse_root(lanes_sum<LW>(sq) * inv + eps);
-      if (s < a.samples) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (on[e]) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const T v = (x[r][e].v[j] - mean) * rstd * gamma[e].v[j] + beta[e].v[j];
-              x[r][e].v[j] = a.act ? swish(v) : v;
-            }
-            *reinterpret_cast<Pack<T, V>*>(a.y + s * a.channels + g * a.per + c[e]) = x[r][e];
+          for (int j = 0; j < V; ++j) {
+            const T v = (x[r][e].v[j] - mean) * rstd * gamma[e].v[j] + beta[e].v[j];
+            x[r][e].v[j] = a.act ? swish(v) : v;
           }
-        if (l == 0) {
-          a.mean_out[s * a.groups + g] = mean;
-          a.rstd_out[s * a.groups + g] = rstd;
+          *reinterpret_cast<Pack<T, V>*>(a.y + s * a.channels + g * a.per + c[e]) = x[r][e];
         }
+      if (l == 0) {
+        a.mean_out[s * a.groups + g] = mean;
+        a.rstd_out[s * a.groups + g] = rstd;
       }
     }
   }
@@ -368,12 +375,9 @@ __device__ __forceinline__ void apply(const Args<T>& a, const Place<T>& w, const
     const int64_t at = w.s * a.positions * a.channels + c;
     T mean, rstd;
     stats(q * V / a.per, mean, rstd);
-    T gamma[V], beta[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
-      beta[j] = a.beta ? a.beta[c + j] : (T)0;
-    }
+    const Pack<T, V> gammas = parameters<T, V>(a, a.gamma, c, (T)1), betas = parameters<T, V>(a, a.beta, c, (T)0);
+    const T(&gamma)[V] = gammas.v;
+    const T(&beta)[V] = betas.v;
     for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
       Pack<T, V> v[4];
 #pragma unroll
@@ -449,12 +453,9 @@ __device__ __forceinline__ void thread_gradients(const Args<T>& a, const Place<T
   const int c = w.c0 + q * V;
   const int64_t i = w.s * a.groups + c / a.per, at = w.s * a.positions * a.channels + c;
   const T mean = a.mean[i], rstd = a.rstd[i];
-  T gamma[V], beta[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
-    beta[j] = a.beta ? a.beta[c + j] : (T)0;
-  }
+  const Pack<T, V> gammas = parameters<T, V>(a, a.gamma, c, (T)1), betas = parameters<T, V>(a, a.beta, c, (T)0);
+  const T(&gamma)[V] = gammas.v;
+  const T(&beta)[V] = betas.v;
   for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)2 * w.rows) {
     Pack<T, V> x[2], d[2];
 #pragma unroll
@@ -556,12 +557,9 @@ __device__ __forceinline__ void input_gradients(const Args<T>& a, const Place<T>
     const T mean = a.mean[i], rstd = a.rstd[i];
     T s1, s2;
     means(q * V / a.per, s1, s2);
-    T gamma[V], beta[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      gamma[j] = a.gamma ? a.gamma[c + j] : (T)1;
-      beta[j] = a.beta ? a.beta[c + j] : (T)0;
-    }
+    const Pack<T, V> gammas = parameters<T, V>(a, a.gamma, c, (T)1), betas = parameters<T, V>(a, a.beta, c, (T)0);
+    const T(&gamma)[V] = gammas.v;
+    const T(&beta)[V] = betas.v;
     for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)2 * w.rows) {
       Pack<T, V> x[2], d[2];
 #pragma unroll
@@ -660,12 +658,14 @@ template <auto Kernel> static int resident() {
 }
 
 template <typename T, int V, int LW, int E> static prad_status rows(prad_ctx* ctx, const Args<T>& a, bool backward) {
-  // as many slots as fill the device once, and a whole number of them per group
-  const int held = backward ? resident<rows_backward_kernel<T, V, LW, E>>() : resident<rows_forward_kernel<T, V, LW, E>>();
-  const int64_t fill = (int64_t)ctx->sm_count * held * THREADS / LW;
-  int64_t per_group = fill / a.groups;
-  if (per_group < 1) per_group = 1;
-  if (per_group > a.samples) per_group = a.samples;
+  // Forward a slot for every R samples of a group.  Backward as many slots as the device holds: each leaves sums of its own.
+  int64_t per_group = ceil_div(a.samples, rows_at_once<E>());
+  if (backward) {
+    const int64_t fill = (int64_t)ctx->sm_count * resident<rows_backward_kernel<T, V, LW, E>>() * THREADS / LW;
+    per_group = fill / a.groups;
+    if (per_group < 1) per_group = 1;
+    if (per_group > a.samples) per_group = a.samples;
+  }
   const int64_t slots = per_group * a.groups;
   const int64_t grid = ceil_div(slots * LW, THREADS);
   PRAD_REQUIRE(grid <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "group norm: too many groups");
@@ -802,8 +802,9 @@ template <typename T, int V> static prad_status blocks(prad_ctx* ctx, Args<T> a,
   return PRAD_OK;
 }
 
-template <typename T> static prad_status run(prad_ctx* ctx, const Args<T>& a, bool backward) {
+template <typename T> static prad_status run(prad_ctx* ctx, Args<T> a, bool backward) {
   constexpr int V = 16 / sizeof(T);
+  a.wide = (((uintptr_t)a.gamma | (uintptr_t)a.beta) & 15) == 0;
   const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.y | (uintptr_t)a.dx;
   const bool vector = a.per % V == 0 && (all & 15) == 0;
   if (a.positions == 1 && a.per <= (vector ? most_in_registers<T, V>() : most_in_registers<T, 1>()))
