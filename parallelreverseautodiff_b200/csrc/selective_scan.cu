@@ -30,7 +30,8 @@ using seq::mul;
 constexpr int THREADS = 128;
 // TT of the passes without a history: 16 where a CTA has 64 channels (or doubles), so that what it fetches stays in registers
 template <typename T, int L> constexpr int tile() { return sizeof(T) == 8 || L == 2 ? 16 : 32; }
-constexpr int SPAN = 32;         // spans are multiples of this many tokens
+// spans are multiples of this many tokens, and two of them at least
+template <typename T> constexpr int span_unit() { return sizeof(T) == 8 ? 16 : 32; }
 constexpr int POINT = 16;        // tokens per checkpoint, and TT of the main backward pass
 constexpr int MAX_STATE = 128;
 
@@ -768,16 +769,18 @@ template <int L, int S, typename T> __device__ __forceinline__ void channel_sums
 template <typename T, int L, int S> struct Backward {
   static constexpr int CC = sizeof(T) == 8 && L < 32 ? 1 : 2, HALF = THREADS / L, CH = CC * HALF, TT = POINT, N = L * S, P = S / 2;
   static constexpr int WARPS = THREADS / 32;
+  // In double what a thread keeps for itself stays in registers, and fewer tokens are gathered at a time: two CTAs fit an SM.
+  static constexpr bool OWN = sizeof(T) == 8;
   // tokens whose dB and dC are gathered at a time
-  static constexpr int FT = 8 * 16 / N < 2 ? 2 : 8 * 16 / N < 8 ? 8 * 16 / N : 8;
+  static constexpr int MOST = OWN ? 4 : 8, FT = 8 * 16 / N < 2 ? 2 : 8 * 16 / N < MOST ? 8 * 16 / N : MOST;
   struct alignas(16) Step { T dt, gB, x, gA; };                       // in float first {dt, dt, x, x}
   struct Shared {
     Pack<T, S> h[CC][TT + 1][THREADS];                                // the state in front of each token, and behind the last
     alignas(16) T B[2][TT][N], C[2][TT][N];
     Step step[TT][CH];
     T red[WARPS][FT][2 * N];
-    alignas(16) T v[TT][CH], u[TT][CH], slope[TT][CH], w[TT][CH];      // slope: d dt / d delta, w: dz / r
-    alignas(16) T r[TT][CH + 8];
+    alignas(16) T v[TT][CH], u[TT][CH], slope[TT][CH], w[OWN ? 1 : TT][CH];      // slope: d dt / d delta, w: dz / r
+    alignas(16) T r[TT][CH + (OWN ? 4 : 8)];
   };
 };
 __device__ __forceinline__ void read_step(const float* m, Two<float>& dt, Two<float>& x) {
@@ -886,6 +889,7 @@ backward_kernel(const Args<T> a) {
     for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT) {
       const int buf = (int)(tile0 / TT & 1);
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
+      T own_w[E][V];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int r = mine.row + i * ROWS;
@@ -912,8 +916,11 @@ backward_kernel(const Args<T> a) {
           put(&m.v[r][mine.col], v);
           put(&m.u[r][mine.col], u[i]);
           put(&m.slope[r][mine.col], slope);
-          put(&m.w[r][mine.col], w);
+          if constexpr (!K::OWN) put(&m.w[r][mine.col], w);
         }
+        if constexpr (K::OWN)
+#pragma unroll
+          for (int j = 0; j < V; ++j) own_w[i][j] = w[j];
       }
       Two<T> h[CC][P];
 #pragma unroll
@@ -1143,7 +1150,12 @@ backward_kernel(const Args<T> a) {
         pick(&m.u[r][mine.col], ut);
         pick(&m.v[r][mine.col], v);
         pick(&m.slope[r][mine.col], slope);
-        pick(&m.w[r][mine.col], w);
+        if constexpr (!K::OWN) {
+          pick(&m.w[r][mine.col], w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) w[j] = own_w[i][j];
+        }
         pick(&m.r[r][mine.col], rt);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -1305,7 +1317,7 @@ template <auto Kernel> static int64_t resident(prad_ctx* ctx, int smem) {
 // about half of the work again), else into spans of whole tiles, as many as the device holds at a time: one CTA more takes as long
 // as twice as many.
 template <typename T> static void cut(Args<T>& a, int64_t across, int64_t full) {
-  if (!a.rows.offsets && a.rows.count > 0 && a.rows.count <= 65535 && (a.rows.count * across >= full / 2 || a.rows.each <= 2 * SPAN)) {
+  if (!a.rows.offsets && a.rows.count > 0 && a.rows.count <= 65535 && (a.rows.count * across >= full / 2 || a.rows.each <= 2 * span_unit<T>())) {
     a.span = a.rows.each > 0 ? a.rows.each : 1;
     a.spans = a.rows.count;
     return;
@@ -1313,8 +1325,9 @@ template <typename T> static void cut(Args<T>& a, int64_t across, int64_t full) 
   int64_t spans = full / across;
   if (spans < 1) spans = 1;
   if (spans > 65535) spans = 65535;
-  int64_t span = ceil_div(ceil_div(a.rows.tokens, spans), SPAN) * SPAN;
-  if (span < 2 * SPAN) span = 2 * SPAN;
+  constexpr int unit = span_unit<T>();
+  int64_t span = ceil_div(ceil_div(a.rows.tokens, spans), unit) * unit;
+  if (span < 2 * unit) span = 2 * unit;
   a.span = span;
   a.spans = (int)ceil_div(a.rows.tokens, span);
   if (a.spans < 1) a.spans = 1;
