@@ -168,6 +168,9 @@ inline void launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t s
 inline bool dtype_ok(prad_dtype dt) { return dt == PRAD_F32 || dt == PRAD_F64; }
 inline size_t dtype_size(prad_dtype dt) { return dt == PRAD_F64 ? 8 : 4; }
 
+// whether all pointers are multiples of a value's size (null is)
+template <typename... P> inline bool natural(prad_dtype dt, P... p) { return ((... | (uintptr_t)p) & (dtype_size(dt) - 1)) == 0; }
+
 // grows ctx->ws to at least `bytes` (256-byte aligned) ; previous contents are lost
 prad_status ensure_workspace(prad_ctx* ctx, size_t bytes);
 // grows the pinned host scratch

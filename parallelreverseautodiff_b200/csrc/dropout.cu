@@ -129,6 +129,7 @@ extern "C" prad_status prad_dropout(prad_ctx* ctx, prad_dtype dt, const void* x,
   PRAD_REQUIRE(n >= 0, PRAD_ERR_SHAPE, "prad_dropout: negative size");
   PRAD_REQUIRE(p >= 0.0 && p <= 1.0, PRAD_ERR_INVALID, "prad_dropout: p must be in [0, 1], got %g", p);
   PRAD_REQUIRE(n == 0 || (x && y), PRAD_ERR_INVALID, "prad_dropout: null pointer");
+  PRAD_REQUIRE(natural(dt, x, residual, y) && ((uintptr_t)step & 7) == 0, PRAD_ERR_INVALID, "prad_dropout: unaligned pointer");
   PRAD_CHECK_CTX(ctx);
   if (n == 0) return PRAD_OK;
   // the nearest whole number of words; p so close to 1 that none is left keeps nothing, as p == 1 does

@@ -6,6 +6,10 @@
 // the registers of a few lanes, one pass over the memory each way.  Several positions: a cluster of CTAs takes a sample (or some of
 // its groups), each CTA a block of its positions; they sum, exchange the sums through each other's shared memory and read their
 // blocks again, now out of the L2.  Too few samples for that, or groups wider than a CTA: sums and results in launches of their own.
+// Floats, forward and backward: 16384 rows of 2048 in groups of 128, 52 and 70 us (5.2 and 5.8 TB/s); 64 samples of 3136 positions and
+// 96 channels in groups of 12 with swish, 39 and 70 us (3.9 and 3.3 TB/s: the clusters of the whole input run at once, so that
+// backward its second reading misses the L2; clusters of 16, or blocks of half the channels, took 14 and 17 us longer).
+//
 // Means and variances are summed around a pivot out of the data (the average of the group's first values), so that a mean far
 // from zero takes nothing from the variance; sums go from float to double every few values.
 #include <cooperative_groups.h>
@@ -853,6 +857,7 @@ extern "C" prad_status prad_group_norm_forward(prad_ctx* ctx, prad_dtype dt, con
   if (st) return st;
   PRAD_REQUIRE(eps >= 0.0, PRAD_ERR_INVALID, "prad_group_norm_forward: eps must not be negative");
   PRAD_REQUIRE(samples == 0 || positions == 0 || (x && y && mean && rstd), PRAD_ERR_INVALID, "prad_group_norm_forward: null pointer");
+  PRAD_REQUIRE(natural(dt, x, gamma, beta, y, mean, rstd), PRAD_ERR_INVALID, "prad_group_norm_forward: unaligned pointer");
   PRAD_CHECK_CTX(ctx);
   if (samples == 0 || positions == 0) return PRAD_OK;
   return dt == PRAD_F32 ? forward_t<float>(ctx, x, gamma, beta, y, mean, rstd, samples, positions, channels, groups, eps, swish)
@@ -866,6 +871,8 @@ extern "C" prad_status prad_group_norm_backward(prad_ctx* ctx, prad_dtype dt, co
   if (st) return st;
   PRAD_REQUIRE(samples == 0 || positions == 0 || (x && mean && rstd && dy && dx), PRAD_ERR_INVALID,
                "prad_group_norm_backward: null pointer");
+  PRAD_REQUIRE(natural(dt, x, gamma, beta, mean, rstd, dy, dx, dgamma, dbeta), PRAD_ERR_INVALID,
+               "prad_group_norm_backward: unaligned pointer");
   PRAD_CHECK_CTX(ctx);
   if (samples == 0 || positions == 0) {      // nothing was normalised: the parameters' gradients are zero
     if (dgamma) PRAD_CUDA(cudaMemsetAsync(dgamma, 0, channels * dtype_size(dt), ctx->stream));

@@ -6,14 +6,22 @@
 //   dA_n = sum_t g_n dt a_n h_n(t - 1),  dB_n = sum over the group's channels of g_n dt u,  dC_n likewise of v h_n,
 //   dD = sum v u,  dz = dy r swish'(z),  ddelta = ddt sigmoid(delta + delta_bias),  dh0 = a_n g_n of the first token.
 //
-// L lanes share a channel, S states each; a CTA takes THREADS / L channels of one group over a span of the tokens, TT of them at a
+// L lanes share a channel, S states each; a CTA takes THREADS / L channels of one group over a span of the tokens, a tile of TT at a
 // time in shared memory.  What bounds it is arithmetic, not memory: N exponentials and 4 N multiply-adds for 16 bytes of a float.
 //
 // The token axis of all sequences is one recurrence in which the state is replaced where a sequence begins.  When the sequences
 // alone give too few CTAs, it is cut into spans of equal length: one pass finds what each span makes of a zero state (and of any
 // other: exp(A sum dt) times it, as decays multiply), a second strings the spans together, and the main pass starts each span from
-// the state it has.  The backward pass runs the same way from the last span up, on checkpoints of the state every TT tokens that
+// the state it has.  The backward pass runs the same way from the last span up, on checkpoints of the state every POINT tokens that
 // the forward pass leaves.
+//
+// 16384 tokens of 1024 float channels with 16 states: edges 97 us, main pass 132 us (a prompt; the exponentials alone would take 60 us
+// each time, the memory 42 us); backward edges 80 us, main pass 522 us.  In both main passes about half of the cycles of the special
+// function unit, of the multiply-add pipe and of the issue slots are used, at the same time: chains of dependent instructions on the
+// eight (backward) and sixteen warps that registers and shared memory leave to an SM are what is left.  Tried and taken back: more
+// CTAs with fewer registers each (spills; 162 us for 155 forward), one channel a thread backward (604 us for 575 then), half of a
+// tile's states at a time so that three CTAs fit an SM backward (661 us for 530), and exponentials by polynomials, which take more issue
+// slots than they free.
 #include "common.cuh"
 #include "packed_sequences.cuh"
 
@@ -593,7 +601,7 @@ forward_kernel(const Args<T> a) {
 // Strings the spans together: edge[p] becomes the state that span p begins with.  FORWARD: edge[p + 1] holds what span p ends in
 // from zero; otherwise edge[p] holds what span p hands up from zero, and becomes what it is handed from below.
 // A span takes what it is given, x, to own + through x.  A CTA has JOINED neighbouring states and 32 spans at a time, a warp each
-// state: the lanes' maps are composed in five steps (one thread for all spans of a state took 12 us for 18 spans of 16384 states).
+// state: the lanes' maps are composed in five steps (18 spans of 8040 double states: 4 us; one thread for all spans of a state, 28 us).
 constexpr int JOINED = 8;
 template <typename T, bool FORWARD>
 __global__ void __launch_bounds__(32 * JOINED)
@@ -1425,6 +1433,7 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   PRAD_LAUNCHED(ctx);
   if (a.blocks > 1 && a.rows.tokens) {
     const int64_t n = a.rows.tokens * a.groups * 2 * a.state;
+    PRAD_REQUIRE(ceil_div(n, 256) <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many rows of B and C");
     launch_chained(row_totals_kernel<T>, (unsigned)ceil_div(n, 256), 256, 0, ctx->stream, a);
     PRAD_LAUNCHED(ctx);
   }
@@ -1454,7 +1463,7 @@ template <typename T> static prad_status pick(prad_ctx* ctx, Args<T> a, Pass pas
   }
 }
 
-static prad_status check(const char* who, prad_dtype dt, const prad_scan_t* s) {
+static prad_status check_shape(const char* who, prad_dtype dt, const prad_scan_t* s) {
   PRAD_REQUIRE(dtype_ok(dt), PRAD_ERR_INVALID, "%s: unknown dtype %d", who, (int)dt);
   PRAD_REQUIRE(s, PRAD_ERR_INVALID, "%s: null scan", who);
   PRAD_REQUIRE(s->tokens >= 0 && s->sequences >= 0 && s->dim > 0 && s->state > 0 && s->groups > 0, PRAD_ERR_SHAPE, "%s: bad shape", who);
@@ -1462,11 +1471,17 @@ static prad_status check(const char* who, prad_dtype dt, const prad_scan_t* s) {
   PRAD_REQUIRE(s->state <= MAX_STATE, PRAD_ERR_UNSUPPORTED, "%s: at most %d states, got %d", who, MAX_STATE, s->state);
   PRAD_REQUIRE(s->tokens <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens", who);
   PRAD_REQUIRE(s->dim <= 1 << 20, PRAD_ERR_UNSUPPORTED, "%s: more than 2^20 channels", who);
+  return PRAD_OK;
+}
+static prad_status check(const char* who, prad_dtype dt, const prad_scan_t* s) {
+  prad_status st = check_shape(who, dt, s);
+  if (st) return st;
   const int64_t rows = (int64_t)s->groups * s->state;
   PRAD_REQUIRE((!s->ld_u || s->ld_u >= s->dim) && (!s->ld_delta || s->ld_delta >= s->dim) && (!s->ld_z || s->ld_z >= s->dim) &&
                    (!s->ld_B || s->ld_B >= rows) && (!s->ld_C || s->ld_C >= rows),
                PRAD_ERR_SHAPE, "%s: a pitch below the row", who);
   PRAD_REQUIRE(s->tokens == 0 || (s->u && s->delta && s->A && s->B && s->C), PRAD_ERR_INVALID, "%s: null pointer", who);
+  PRAD_REQUIRE(natural(dt, s->u, s->delta, s->z, s->A, s->B, s->C, s->D, s->delta_bias, s->h0), PRAD_ERR_INVALID, "%s: unaligned pointer", who);
   return PRAD_OK;
 }
 static prad_status check_sequences(const char* who, const prad_scan_t* s) {
@@ -1517,7 +1532,7 @@ static prad_status backward_t(prad_ctx* ctx, const prad_scan_t* scan, const void
 }
 
 extern "C" prad_status prad_selective_scan_saved_bytes(prad_dtype dt, const prad_scan_t* scan, size_t* out_bytes) {
-  prad_status st = ssm::check("prad_selective_scan_saved_bytes", dt, scan);
+  prad_status st = ssm::check_shape("prad_selective_scan_saved_bytes", dt, scan);
   if (st) return st;
   PRAD_REQUIRE(out_bytes, PRAD_ERR_INVALID, "prad_selective_scan_saved_bytes: null output");
   *out_bytes = (size_t)ceil_div(scan->tokens, ssm::POINT) * scan->dim * scan->state * dtype_size(dt);
@@ -1534,6 +1549,7 @@ extern "C" prad_status prad_selective_scan_forward(prad_ctx* ctx, prad_dtype dt,
   PRAD_REQUIRE(scan->tokens == 0 || y, PRAD_ERR_INVALID, "%s: null pointer", who);
   PRAD_REQUIRE(scan->tokens == 0 || (y != scan->u && y != scan->delta && y != scan->z), PRAD_ERR_INVALID, "%s: y may not be an input", who);
   PRAD_REQUIRE(!h_last || h_last != scan->h0, PRAD_ERR_INVALID, "%s: h_last may not be h0", who);
+  PRAD_REQUIRE(natural(dt, y, h_last, saved), PRAD_ERR_INVALID, "%s: unaligned pointer", who);
   PRAD_CHECK_CTX(ctx);
   if (scan->tokens == 0) {       // every final state is the initial one
     const size_t bytes = (size_t)scan->sequences * scan->dim * scan->state * dtype_size(dt);
@@ -1559,6 +1575,8 @@ extern "C" prad_status prad_selective_scan_backward(prad_ctx* ctx, prad_dtype dt
   PRAD_REQUIRE(!g->dh0 || scan->h0, PRAD_ERR_INVALID, "%s: dh0 without an h0", who);
   PRAD_REQUIRE(scan->tokens == 0 || (saved && dy && g->du && g->ddelta && g->dB && g->dC && (!scan->z || g->dz)), PRAD_ERR_INVALID,
                "%s: null pointer", who);
+  PRAD_REQUIRE(natural(dt, saved, dy, g->du, g->ddelta, g->dz, g->dA, g->dB, g->dC, g->dD, g->ddelta_bias, g->dh0), PRAD_ERR_INVALID,
+               "%s: unaligned pointer", who);
   PRAD_CHECK_CTX(ctx);
   if (scan->tokens == 0) {
     const size_t s = dtype_size(dt), states = (size_t)scan->dim * scan->state;
@@ -1578,6 +1596,7 @@ extern "C" prad_status prad_selective_scan_step(prad_ctx* ctx, prad_dtype dt, co
   PRAD_REQUIRE(!ld_y || ld_y >= scan->dim, PRAD_ERR_SHAPE, "%s: a pitch below dim", who);
   PRAD_REQUIRE(!scan->offsets && scan->sequences == scan->tokens, PRAD_ERR_SHAPE, "%s: one token for each sequence", who);
   PRAD_REQUIRE(scan->tokens == 0 || (scan->h0 && h_out && y), PRAD_ERR_INVALID, "%s: null pointer", who);
+  PRAD_REQUIRE(natural(dt, y, h_out), PRAD_ERR_INVALID, "%s: unaligned pointer", who);
   PRAD_CHECK_CTX(ctx);
   if (scan->tokens == 0) return PRAD_OK;
   return dt == PRAD_F32 ? forward_t<float>(ctx, scan, y, ld_y, h_out, nullptr, ssm::Pass::Step)

@@ -43,6 +43,24 @@ def _divided(n: int, by: int, what: str, parts: str) -> int:
     return n // by
 
 
+def _expect(who: str, dtype, *sized) -> None:
+    """(name, matrix or None, shape) each: a matrix of another type, or with another number of values than the shape, is refused before
+    a kernel could reach past it."""
+    for name, m, shape in sized:
+        if m is None or (m.shape == shape and m.dtype is dtype):
+            continue
+        if m.dtype != dtype:
+            raise _lib.PradError(_lib.ERR_INVALID, f"{who}: {name} is {m.dtype}, not {dtype}")
+        n = 1
+        for d in shape:
+            n *= d
+        if m.size != n:
+            raise _lib.PradError(_lib.ERR_SHAPE, f"{who}: {name} has {m.size} values, not {n}")
+
+
+_I32, _U64 = np.dtype(np.int32), np.dtype(np.uint64)
+
+
 class DeviceMatrix:
     """A dense row-major device buffer: Matrix (2-D) or DeepMatrix (3-D, depth first)."""
 
@@ -51,7 +69,7 @@ class DeviceMatrix:
     def __init__(self, engine: "Engine", ptr: int, shape: Sequence[int], dtype, owned=True):
         self.engine = engine
         self.ptr = ptr
-        self.shape = tuple(map(int, shape))
+        self.shape = tuple(shape) if isinstance(shape, tuple) else tuple(map(int, shape))
         self.dtype = dtype if isinstance(dtype, np.dtype) else np.dtype(dtype)
         self._owned = owned
 
@@ -862,6 +880,8 @@ class Engine:
         """x / (1 - p) where the generator keeps it, else 0, plus the residual; on dy with the same seed and offset it is the
         Backward (prad_dropout)."""
         out = out or self.empty(x.shape, x.dtype)
+        _expect("dropout", x.dtype, ("residual", residual, x.shape), ("out", out, x.shape))
+        _expect("dropout", _U64, ("step", step, (1,)))
         check(self.lib.prad_dropout(self.ctx, dtype_code(x.dtype), x.ptr, self._p(residual), out.ptr, x.size, p, seed, offset,
                                     self._p(step)))
         return out
@@ -872,6 +892,9 @@ class Engine:
         samples = _divided(rows, positions, "rows", "positions")
         y, mean, rstd = out or (self.empty(x.shape, x.dtype), self.empty((samples, groups), x.dtype),
                                 self.empty((samples, groups), x.dtype))
+        stats, each = (samples, groups), (channels,)
+        _expect("group_norm_forward", x.dtype, ("gamma", gamma, each), ("beta", beta, each), ("y", y, x.shape), ("mean", mean, stats),
+                ("rstd", rstd, stats))
         check(self.lib.prad_group_norm_forward(self.ctx, dtype_code(x.dtype), x.ptr, self._p(gamma), self._p(beta), y.ptr, mean.ptr,
                                                rstd.ptr, samples, positions, channels, groups, eps, int(swish)))
         return y, mean, rstd
@@ -881,6 +904,9 @@ class Engine:
         rows, channels = x.size // x.shape[-1], x.shape[-1]
         samples = _divided(rows, positions, "rows", "positions")
         dx, dgamma, dbeta = out or (self.empty(x.shape, x.dtype), self.empty((channels,), x.dtype), self.empty((channels,), x.dtype))
+        stats, each = (samples, groups), (channels,)
+        _expect("group_norm_backward", x.dtype, ("gamma", gamma, each), ("beta", beta, each), ("mean", mean, stats), ("rstd", rstd, stats),
+                ("dy", dy, x.shape), ("dx", dx, x.shape), ("dgamma", dgamma, each), ("dbeta", dbeta, each))
         check(self.lib.prad_group_norm_backward(self.ctx, dtype_code(x.dtype), x.ptr, self._p(gamma), self._p(beta), mean.ptr, rstd.ptr,
                                                 dy.ptr, dx.ptr, self._p(dgamma), self._p(dbeta), samples, positions, channels, groups,
                                                 int(swish)))
@@ -894,6 +920,10 @@ class Engine:
         out = out or self.empty((tokens, dim), x.dtype)
         if state_out is True:
             state_out = self.empty((sequences, (width - 1) * dim), x.dtype)
+        states = (sequences, (width - 1) * dim)
+        _expect("causal_conv_forward", x.dtype, ("w", w, (dim, width)), ("bias", bias, (dim,)), ("state", state, states),
+                ("state_out", state_out, states), ("out", None if ld_y else out, x.shape))
+        _expect("causal_conv_forward", _I32, ("offsets", offsets, (sequences + 1,)))
         check(self.lib.prad_causal_conv_forward(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), self._p(state),
                                                 self._p(offsets), out.ptr, ld_y, self._p(state_out), sequences, tokens, dim, width,
                                                 int(swish)))
@@ -905,6 +935,11 @@ class Engine:
         (tokens, dim), width = x.shape, w.shape[1]
         if out is None:
             out = {k: self.empty(m.shape, x.dtype) for k, m in (("x", x), ("w", w), ("bias", bias), ("state", state)) if m is not None}
+        states, each = (sequences, (width - 1) * dim), (dim,)
+        _expect("causal_conv_backward", x.dtype, ("w", w, (dim, width)), ("bias", bias, each), ("state", state, states), ("dy", dy, x.shape),
+                ("dx", out["x"], x.shape), ("dw", out.get("w"), (dim, width)), ("dbias", out.get("bias"), each),
+                ("dstate", out.get("state"), states))
+        _expect("causal_conv_backward", _I32, ("offsets", offsets, (sequences + 1,)))
         check(self.lib.prad_causal_conv_backward(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), self._p(state),
                                                  self._p(offsets), dy.ptr, ld_dy, out["x"].ptr, ld_dx, self._p(out.get("w")),
                                                  self._p(out.get("bias")), self._p(out.get("state")), sequences, tokens, dim, width,
@@ -915,6 +950,9 @@ class Engine:
         """One new row of each sequence; the state is replaced, or goes to `state_out`.  Returns y."""
         (batch, dim), width = x.shape, w.shape[1]
         out = out or self.empty((batch, dim), x.dtype)
+        states = (batch, (width - 1) * dim)
+        _expect("causal_conv_step", x.dtype, ("w", w, (dim, width)), ("bias", bias, (dim,)), ("state", state if width > 1 else None, states),
+                ("state_out", state_out if width > 1 else None, states), ("out", None if ld_y else out, x.shape))
         check(self.lib.prad_causal_conv_step(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), state.ptr, out.ptr, ld_y,
                                              state.ptr if state_out is None else state_out.ptr, batch, dim, width, int(swish)))
         return out
@@ -922,11 +960,22 @@ class Engine:
     @staticmethod
     def _scan(u, delta, A, B, C_, D, z, delta_bias, h0, offsets, sequences, groups, delta_softplus, pitches):
         dim, state = A.shape
+        T = u.shape[0]
+        tokens, rows, each = (T, dim), (T, groups * state), (dim,)
+        _expect("selective_scan", u.dtype, ("u", u, tokens), ("delta", delta, tokens), ("A", A, A.shape), ("B", B, rows), ("C", C_, rows),
+                ("D", D, each), ("z", z, tokens), ("delta_bias", delta_bias, each), ("h", h0, (sequences, dim * state)))
+        _expect("selective_scan", _I32, ("offsets", offsets, (sequences + 1,)))
         s = _lib.Scan(u.shape[0], sequences, dim, state, groups, int(delta_softplus), *[None if m is None else m.ptr for m in (
             offsets, u, delta, z, A, B, C_, D, delta_bias, h0)])
         for k, ld in (pitches or {}).items():
             setattr(s, "ld_" + k, ld)
         return s
+
+    def selective_scan_saved(self, tokens, dim, state, dtype) -> int:
+        """How many values `save` of selective_scan_forward needs."""
+        s, n, dtype = _lib.Scan(tokens, 1, dim, state, 1), C.c_size_t(), np.dtype(dtype)
+        check(self.lib.prad_selective_scan_saved_bytes(dtype_code(dtype), C.byref(s), C.byref(n)))
+        return max(1, n.value // dtype.itemsize)
 
     def selective_scan_forward(self, u, delta, A, B, C, D=None, z=None, delta_bias=None, h0=None, offsets=None, sequences=1, groups=1,
                                delta_softplus=True, out=None, h_last=None, save=False, pitches=None, ld_y=0):
@@ -938,11 +987,15 @@ class Engine:
         out = out or self.empty(u.shape, u.dtype)
         if h_last is True:
             h_last = self.empty((sequences, s.dim * s.state), u.dtype)
-        if save is True:
-            n = _size_t()
+        n = _size_t()
+        if save:
             check(self.lib.prad_selective_scan_saved_bytes(dt, ref, _byref(n)))
-            save = self.empty((max(1, n.value // u.dtype.itemsize),), u.dtype)
+            if save is True:
+                save = self.empty((max(1, n.value // u.dtype.itemsize),), u.dtype)
+            elif save.nbytes < n.value:
+                raise _lib.PradError(_lib.ERR_SHAPE, f"selective_scan_forward: save has {save.nbytes} bytes, not {n.value}")
         save = save or None
+        _expect("selective_scan_forward", u.dtype, ("h_last", h_last, (sequences, s.dim * s.state)), ("out", None if ld_y else out, u.shape))
         check(self.lib.prad_selective_scan_forward(self.ctx, dt, ref, out.ptr, ld_y, self._p(h_last), self._p(save)))
         return out, h_last, save
 
@@ -953,6 +1006,10 @@ class Engine:
         if out is None:
             out = {k: self.empty(m.shape, u.dtype) for k, m in (("u", u), ("delta", delta), ("z", z), ("A", A), ("B", B), ("C", C),
                                                                 ("D", D), ("delta_bias", delta_bias), ("h0", h0)) if m is not None}
+        for k, m in (("u", u), ("delta", delta), ("z", z), ("A", A), ("B", B), ("C", C), ("D", D), ("delta_bias", delta_bias), ("h0", h0)):
+            if m is not None:
+                _expect("selective_scan_backward", u.dtype, ("gradient of " + k, out.get(k), m.shape))
+        _expect("selective_scan_backward", u.dtype, ("dy", dy, u.shape))
         g = _lib.ScanGradients(*[self._p(out.get(k)) for k in ("u", "delta", "z", "A", "B", "C", "D", "delta_bias", "h0")])
         for k, ld in (gradient_pitches or {}).items():
             setattr(g, "ld_d" + k, ld)
@@ -964,6 +1021,7 @@ class Engine:
         """One new token for each sequence; the states `h` are replaced, or go to `h_out`.  Returns y."""
         s = self._scan(u, delta, A, B, C, D, z, delta_bias, h, None, u.shape[0], groups, delta_softplus, pitches)
         out = out or self.empty(u.shape, u.dtype)
+        _expect("selective_scan_step", u.dtype, ("h_out", h_out, h.shape), ("out", None if ld_y else out, u.shape))
         check(self.lib.prad_selective_scan_step(self.ctx, dtype_code(u.dtype), _byref(s), out.ptr, ld_y, (h_out or h).ptr))
         return out
 

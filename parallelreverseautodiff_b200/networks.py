@@ -989,19 +989,19 @@ class StateSpaceBlock:
     def forward(self, x: E.DeviceMatrix, offsets=None, sequences=1, states=None, states_out=None, training=True, step=None):
         """x [tokens x dim].  `states`: in front of the sequences (new_states or an earlier states_out), `states_out`: to take those
         behind them; `step`: a device counter that draws another dropout mask at each value (Engine.dropout_step)."""
-        e, p, B_, T = self.eng, self.p, self._buf, x.shape[0]
+        e, p, d, B_, T = self.eng, self.p, self.inner, self._buf, x.shape[0]
         self.x, self.rows, self.step_counter, self.training = x, dict(offsets=offsets, sequences=sequences), step, training
         before = states or {"conv": None, "h": None}
         after = states_out or {"conv": None, "h": None}
         self.before = before
         conv = lambda u, out: e.causal_conv_forward(u, p["Wc"], p["bc"], before["conv"], **self.rows, out=out,  # noqa: E731
-                                                    state_out=after["conv"], ld_x=2 * self.inner)[0]
+                                                    state_out=after["conv"], ld_x=2 * d)[0]
         self.uz, self.c, self.dbc, self.delta = self._mix(x, T, conv)
         parts, pitches = self._parts(self.uz, self.dbc)
-        saved = B_("saved", (max(1, (T + 15) // 16 * self.inner * self.state),)) if training else False
+        saved = B_("saved", (e.selective_scan_saved(T, d, self.state, self.dtype),)) if training else False
         self.y, _, self.saved = e.selective_scan_forward(
             self.c, self.delta, p["A"], parts["B"], parts["C"], p["D"], parts["z"], p["bdt"], before["h"], groups=self.groups, **self.rows,
-            out=B_("y", (T, self.inner)), h_last=after["h"], save=saved, pitches=pitches)
+            out=B_("y", (T, d)), h_last=after["h"], save=saved, pitches=pitches)
         self.out = self._project(x, self.y, T, training, step)
         return self.out
 

@@ -373,6 +373,75 @@ def test_dropout_keeps_the_share_it_says(engine):
     assert abs(((y != 0) & (z != 0)).mean() - 0.49) < 6 * np.sqrt(0.25 / n)
 
 
+def test_matrices_that_do_not_fit_are_refused(engine):
+    e, f = engine, np.float32
+    m = lambda *s: e.zeros(s, f)  # noqa: E731
+    u, A, B = m(6, 8), m(8, 4), m(6, 4)
+    off, last = e.sequence_offsets([6]), m(1, 32)
+    good = dict(u=u, delta=u, A=A, B=B, C=B)
+    for bad in (dict(delta=m(5, 8)), dict(B=m(6, 3)), dict(C=m(6, 5)), dict(D=m(7)), dict(z=m(6, 7)), dict(delta_bias=m(9)), dict(h0=m(1, 31)),
+                dict(offsets=off, sequences=2), dict(out=m(6, 7)), dict(h_last=m(2, 32)), dict(save=m(31))):
+        with pytest.raises(_lib.PradError) as err:
+            e.selective_scan_forward(**{**good, **bad})
+        assert err.value.status == _lib.ERR_SHAPE, bad
+    _, _, saved = e.selective_scan_forward(**good, save=True)
+    for bad in (dict(dy=m(6, 7)), dict(out=dict(u=u, delta=u, A=m(8, 3), B=B, C=B)), dict(out=dict(u=m(5, 8), delta=u, A=A, B=B, C=B))):
+        with pytest.raises(_lib.PradError):
+            e.selective_scan_backward(**{**good, "saved": saved, "dy": u, **bad})
+    for call in (lambda: e.selective_scan_step(u, u, A, B, B, m(5, 32)), lambda: e.causal_conv_forward(u, m(7, 4)),
+                 lambda: e.causal_conv_forward(u, m(8, 4), state=m(2, 24)), lambda: e.causal_conv_backward(u, m(8, 4), m(6, 9)),
+                 lambda: e.causal_conv_step(u, m(8, 4), m(6, 16)), lambda: e.group_norm_forward(u, 2, gamma=m(7)),
+                 lambda: e.group_norm_forward(u, 2, positions=4), lambda: e.group_norm_backward(u, m(6, 2), m(5, 2), u, 2),
+                 lambda: e.dropout(u, 0.1, 1, residual=m(6, 7))):
+        with pytest.raises(_lib.PradError) as err:
+            call()
+        assert err.value.status == _lib.ERR_SHAPE
+    other = e.zeros((6, 8), np.float64)
+    for call in (lambda: e.dropout(u, 0.1, 1, step=u), lambda: e.dropout(u, 0.1, 1, residual=other),
+                 lambda: e.selective_scan_forward(**{**good, "delta": other}), lambda: e.selective_scan_forward(**good, offsets=m(2)),
+                 lambda: e.causal_conv_forward(u, e.zeros((8, 4), np.float64)), lambda: e.group_norm_forward(u, 2, out=(other, m(6, 2), m(6, 2)))):
+        with pytest.raises(_lib.PradError) as err:
+            call()
+        assert err.value.status == _lib.ERR_INVALID
+    with pytest.raises(ValueError):
+        e.sequence_offsets([3, -1])
+    assert last.numpy().shape == (1, 32)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+def test_matrices_at_odd_addresses(engine, dtype):
+    """One value behind an allocation's start nothing can be read sixteen bytes at a time: the same values as at its start."""
+    e, f, r = engine, F[dtype], np.random.default_rng(13)
+
+    owners = []                          # (a view does not keep its matrix)
+
+    def shifted(a):
+        owners.append(e.upload(np.concatenate([[0], a.reshape(-1)]).astype(f)))
+        return owners[-1].view(a.shape, 1)
+
+    T, d, n = 75, 36, 8
+    x = scan_case(r, f, T, d, n, 1, 2)
+    dy, off = r.standard_normal((T, d)).astype(f), e.sequence_offsets([40, 35])
+    w = r.standard_normal((d, 4)).astype(f)
+    gamma = r.standard_normal(d).astype(f)
+    limit = 400 * 75 * STEP[dtype]       # the same sums in another order: as in the module's bound with T = 75
+
+    def run(up):
+        dev = {k: up(v) for k, v in x.items()}
+        y, last, saved = e.selective_scan_forward(**dev, offsets=off, sequences=2, h_last=True, save=True)
+        g = e.selective_scan_backward(**dev, offsets=off, sequences=2, saved=saved, dy=up(dy))
+        c, _ = e.causal_conv_forward(dev["u"], up(w), offsets=off, sequences=2)
+        gc = e.causal_conv_backward(dev["u"], up(w), up(dy), offsets=off, sequences=2)
+        out = [y, last, *(g[k] for k in sorted(g)), c, gc["x"], gc["w"]]
+        for positions in (1, 25):
+            v, mean, rstd = e.group_norm_forward(dev["u"], 3, up(gamma), positions=positions, swish=True)
+            out += [v, mean, rstd, *e.group_norm_backward(dev["u"], mean, rstd, up(dy), 3, up(gamma), positions=positions, swish=True)]
+        return [m.numpy().astype(np.float64) for m in out]
+
+    for got, want in zip(run(shifted), run(e.upload)):
+        near(got, want, limit * (1 + np.abs(want).max()), f"odd addresses {dtype}")
+
+
 def test_empty_calls(engine):
     e, f = engine, np.float32
     x = e.empty((0, 8), f)

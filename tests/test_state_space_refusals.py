@@ -61,6 +61,8 @@ def test_scan_refuses_more():
          _lib.ERR_INVALID, "null pointer"),
         ("prad_selective_scan_backward", (0, ref, Q, Q, 0, C.byref(_lib.ScanGradients(Q, Q, Q, Q, Q, Q, None, None, Q))),
          _lib.ERR_INVALID, "dh0 without an h0"),
+        ("prad_selective_scan_forward", (0, C.byref(_scan(delta=(1 << 20) + 2)), Q, 0, None, None), _lib.ERR_INVALID, "unaligned pointer"),
+        ("prad_selective_scan_forward", (1, ref, C.c_void_p((1 << 21) + 4), 0, None, None), _lib.ERR_INVALID, "unaligned pointer"),
         ("prad_selective_scan_step", (0, ref, Q, 0, Q), _lib.ERR_SHAPE, "one token for each sequence"),
         ("prad_selective_scan_step", (0, C.byref(_scan(sequences=12)), Q, 0, Q), _lib.ERR_INVALID, "null pointer"),
         # a call that is right otherwise: there is no context
@@ -73,6 +75,8 @@ def test_scan_refuses_more():
     n = C.c_size_t()
     assert _status("prad_selective_scan_saved_bytes", 0, ref, C.byref(n))[0] == 0 and n.value >= 8 * 4 * 4
     assert _status("prad_selective_scan_saved_bytes", 0, ref, None)[0] == _lib.ERR_INVALID
+    assert _status("prad_selective_scan_saved_bytes", 0, C.byref(_lib.Scan(12, 3, 8, 4, 2)), C.byref(n))[0] == 0
+    assert _status("prad_selective_scan_saved_bytes", 0, C.byref(_lib.Scan(12, 3, 8, 4, 3)), C.byref(n))[0] == _lib.ERR_SHAPE
 
 
 def test_conv_refuses():
@@ -86,6 +90,7 @@ def test_conv_refuses():
         (dict(tokens=7), _lib.ERR_SHAPE, "do not divide"), (dict(ld_x=4), _lib.ERR_SHAPE, "pitch"),
         (dict(w=None), _lib.ERR_INVALID, "null pointer"), (dict(y=P), _lib.ERR_INVALID, "y may not be x"),
         (dict(state=P, state_out=P), _lib.ERR_INVALID, "state_out may not be the state"),
+        (dict(bias=C.c_void_p((1 << 20) + 1)), _lib.ERR_INVALID, "unaligned pointer"),
         (dict(), _lib.ERR_NOT_INITIALIZED, "prad_init"),
     ]:
         got, message = call(**over)
