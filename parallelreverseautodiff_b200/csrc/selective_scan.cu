@@ -789,6 +789,7 @@ template <typename T, int L, int S> struct Backward {
     T red[WARPS][FT][2 * N];
     alignas(16) T v[TT][CH], u[TT][CH], slope[TT][CH], w[OWN ? 1 : TT][CH];      // slope: d dt / d delta, w: dz / r
     alignas(16) T r[TT][CH + (OWN ? 4 : 8)];
+    int begins[TT];                                                   // the sequence that begins at a token
   };
 };
 __device__ __forceinline__ void read_step(const float* m, Two<float>& dt, Two<float>& x) {
@@ -946,7 +947,11 @@ backward_kernel(const Args<T> a) {
       // the tokens that begin sequences
       uint32_t starts = 0;
       while (start >= tile0 + from) {
-        if (start < tile0 + to) starts |= 1u << (int)(start - tile0);
+        if (start < tile0 + to) {
+          const uint32_t bit = 1u << (int)(start - tile0);
+          if (threadIdx.x == 0 && !(starts & bit)) m.begins[start - tile0] = s;      // (those before it there have no token)
+          starts |= bit;
+        }
         if (s == 0) {
           start = -1;
           break;
@@ -957,7 +962,7 @@ backward_kernel(const Args<T> a) {
       __syncthreads();
       const T(*rows_B)[N] = m.B[buf];
       const T(*rows_C)[N] = m.C[buf];
-      const auto initial = [&](int t) { return a.h0 ? a.h0 + a.rows.at(tile0 + t) * states : nullptr; };
+      const auto initial = [&](int t) { return a.h0 ? a.h0 + m.begins[t] * states : nullptr; };
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += 4) {
         T part[CC][4];
@@ -1096,7 +1101,7 @@ backward_kernel(const Args<T> a) {
               for (int k = 0; k < CC; ++k) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) two[k][j] = j / 2 == i ? sums[k][j % 2] : two[k][j];
-                if (begins && a.dh0) store(a.dh0 + a.rows.at(tile0 + t0 + i) * states, k, e[k]);
+                if (begins && a.dh0) store(a.dh0 + m.begins[t0 + i] * states, k, e[k]);
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
                   if (begins) e[k][j] = {(T)0, (T)0};

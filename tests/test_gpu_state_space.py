@@ -87,6 +87,24 @@ def test_scan_of_packed_sequences(engine, dtype, lengths, d, n, q):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f64"])
+def test_many_sequences_of_a_token_or_two(engine, dtype):
+    lengths = [1] * 40 + [0] * 3 + [2] * 30 + [0, 3, 0, 0, 1]
+    check_scan(engine, dtype, lengths, 70, 16)
+    check_scan(engine, dtype, [1] * 90, 24, 5, 3, packed=False)
+    e, f, r = engine, F[dtype], np.random.default_rng(1)
+    T, S, d = sum(lengths), len(lengths), 20
+    x = {k: r.standard_normal(s).astype(f) for k, s in (("x", (T, d)), ("w", (d, 4)), ("bias", (d,)), ("state", (S, 3 * d)))}
+    dy = r.standard_normal((T, d)).astype(f)
+    want, size = (R.conv(**x, lengths=lengths, dy=dy, magnitude=m) for m in (False, True))
+    of = dict({k: e.upload(v) for k, v in x.items()}, offsets=e.sequence_offsets(lengths), sequences=S)
+    y, last = e.causal_conv_forward(**of, state_out=True)
+    near(y.numpy(), want["y"], 16 * STEP[dtype] * size["y"], f"conv y {dtype}")
+    assert np.array_equal(last.numpy(), want["last"].astype(f))
+    for k, m in e.causal_conv_backward(**of, dy=e.upload(dy)).items():
+        near(m.numpy(), want[k], (16 + (T if k in ("w", "bias") else 0)) * STEP[dtype] * size[k], f"conv d{k} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
 @pytest.mark.parametrize("n", [1, 2, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 128])
 @pytest.mark.parametrize("d,q", [(1, 1), (66, 2)])
 def test_scan_of_every_number_of_states(engine, dtype, n, d, q):
