@@ -16,12 +16,11 @@
 // the forward pass leaves.
 //
 // 16384 tokens of 1024 float channels with 16 states: edges 97 us, main pass 132 us (a prompt; the exponentials alone would take 60 us
-// each time, the memory 42 us); backward edges 80 us, main pass 522 us.  In both main passes about half of the cycles of the special
+// each time, the memory 42 us); backward edges 80 us, main pass 431 us.  In both main passes about half of the cycles of the special
 // function unit, of the multiply-add pipe and of the issue slots are used, at the same time: chains of dependent instructions on the
-// eight (backward) and sixteen warps that registers and shared memory leave to an SM are what is left.  Tried and taken back: more
-// CTAs with fewer registers each (spills; 162 us for 155 forward), one channel a thread backward (604 us for 575 then), half of a
-// tile's states at a time so that three CTAs fit an SM backward (661 us for 530), and exponentials by polynomials, which take more issue
-// slots than they free.
+// twelve (backward) and sixteen warps that registers leave to an SM are what is left.  Tried and taken back: more CTAs with fewer
+// registers each (spills; 162 us for 155 forward), one channel a thread backward (604 us for 575 then), and exponentials by polynomials,
+// which take more issue slots than they free.
 #include "common.cuh"
 #include "packed_sequences.cuh"
 
@@ -40,7 +39,9 @@ constexpr int THREADS = 128;
 template <typename T, int L> constexpr int tile() { return sizeof(T) == 8 || L == 2 ? 16 : 32; }
 // spans are multiples of this many tokens, and two of them at least
 template <typename T> constexpr int span_unit() { return sizeof(T) == 8 ? 16 : 32; }
-constexpr int POINT = 16;        // tokens per checkpoint, and TT of the main backward pass
+// Tokens per checkpoint, and TT of the main backward pass: with 8 shared memory leaves room for three CTAs (16384 tokens of 1024 floats
+// with 16 states: 470 us when this was chosen; with 16, half of the checkpoints and two CTAs, 518).
+constexpr int POINT = 8;
 constexpr int MAX_STATE = 128;
 
 template <typename T> struct Args {
@@ -328,9 +329,10 @@ template <typename T, int CH, int TT> struct Cells {
   __device__ __forceinline__ int64_t first(int64_t ld, int64_t tile0) const { return (tile0 + row) * ld + col; }
   // rows [from, to) of the tile; what lies outside, and channels that do not exist, as zero
   __device__ __forceinline__ void load(const T* at, int64_t ld, int from, int to, T (&v)[E][V]) const {
-    if (wide && to - from == TT && ROWS <= TT) {
+    if (wide && to - from == TT) {
 #pragma unroll
       for (int e = 0; e < E; ++e, at += ROWS * ld) {
+        if (!in(e)) break;
         const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(at);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[e][j] = w.v[j];
@@ -345,9 +347,10 @@ template <typename T, int CH, int TT> struct Cells {
     }
   }
   __device__ __forceinline__ void store(T* at, int64_t ld, int from, int to, const T (&v)[E][V]) const {
-    if (wide && to - from == TT && ROWS <= TT) {
+    if (wide && to - from == TT) {
 #pragma unroll
       for (int e = 0; e < E; ++e, at += ROWS * ld) {
+        if (!in(e)) break;
         Pack<T, V> w;
 #pragma unroll
         for (int j = 0; j < V; ++j) w.v[j] = v[e][j];
@@ -786,7 +789,7 @@ template <typename T, int L, int S> struct Backward {
     Pack<T, S> h[CC][TT + 1][THREADS];                                // the state in front of each token, and behind the last
     alignas(16) T B[2][TT][N], C[2][TT][N];
     Step step[TT][CH];
-    T red[WARPS][FT][2 * N];
+    alignas(16) T red[WARPS][FT][2 * N];
     alignas(16) T v[TT][CH], u[TT][CH], slope[TT][CH], w[OWN ? 1 : TT][CH];      // slope: d dt / d delta, w: dz / r
     alignas(16) T r[TT][CH + (OWN ? 4 : 8)];
     int begins[TT];                                                   // the sequence that begins at a token
@@ -803,7 +806,7 @@ __device__ __forceinline__ void read_step(const double* m, Two<double>& dt, Two<
 }
 
 template <typename T, int L, int S>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 2)
 backward_kernel(const Args<T> a) {
   chain_begin();
   using K = Backward<T, L, S>;
@@ -824,7 +827,7 @@ backward_kernel(const Args<T> a) {
   const int64_t begin = span.begin, finish = span.finish;
   const auto load = [&](const T* from, int k, Two<T>(&h)[P]) {       // null: zero
     const int ch = ch0 + k * HALF;
-    T w[S];      // (value by value: with the checkpoints read 16 bytes at a time the kernel took 590 us for 540)
+    T w[S];
 #pragma unroll
     for (int j = 0; j < S; ++j) w[j] = from && ch < channels && n0 + j < a.state ? from[(int64_t)(c0 + ch) * a.state + n0 + j] : (T)0;
 #pragma unroll
@@ -872,6 +875,8 @@ backward_kernel(const Args<T> a) {
     T* to_z = a.z ? a.dz + c0 + mine.first(a.ld_dz, top) : nullptr;
     Rows<T, N, TT> B_rows(a.B, a.ld_B, q * a.state, a.state, a.wide_B, top);
     Rows<T, N, TT> C_rows(a.C, a.ld_C, q * a.state, a.state, a.wide_C, top);
+    const T* point = a.saved + top / TT * states + (int64_t)(c0 + ch0) * a.state + n0;      // the checkpoint of the tile to fetch
+    const bool even = a.state % S == 0;         // then a thread has S states or none
     const auto fetch = [&](int64_t tile0) {      // of the tiles in turn, from the last one
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
       mine.load(pu, a.ld_u, from, to, u);
@@ -889,7 +894,20 @@ backward_kernel(const Args<T> a) {
       B_rows.at -= TT * a.ld_B;
       C_rows.at -= TT * a.ld_C;
 #pragma unroll
-      for (int k = 0; k < CC; ++k) load(from == 0 ? a.saved + tile0 / TT * states : nullptr, k, next[k]);
+      for (int k = 0; k < CC; ++k) {
+        if (even && from == 0) {      // (value by value: reads of 16 bytes took 590 us for 540, as their zeros wait for what they load into)
+          const bool on = ch0 + k * HALF < channels && n0 < a.state;
+          const T* at = point + k * HALF * a.state;
+          T w[S];
+#pragma unroll
+          for (int j = 0; j < S; ++j) w[j] = on ? at[j] : (T)0;
+#pragma unroll
+          for (int j = 0; j < P; ++j) next[k][j] = {w[2 * j], w[2 * j + 1]};
+        } else {
+          load(from == 0 ? a.saved + tile0 / TT * states : nullptr, k, next[k]);
+        }
+      }
+      point -= states;
     };
     int s = a.rows.at(finish - 1);              // the sequence of the last token of the tile, and its first token
     int64_t start = a.rows.start(s);
@@ -1127,25 +1145,44 @@ backward_kernel(const Args<T> a) {
         }
         __syncthreads();
         // the warps' sums, in the order of the warps
-        constexpr int ACROSS = 2 * N < THREADS ? 2 * N : THREADS;
-        for (int n = threadIdx.x % ACROSS; n < 2 * N; n += ACROSS) {
-          const int state = n < N ? n : n - N;
-          if (state >= a.state) continue;
-          T* to0 = n < N ? a.dB + q * a.state + state : a.dC + q * a.state + state;
-          int64_t ld = n < N ? a.ld_dB : a.ld_dC;
-          if (a.blocks > 1) {
-            to0 = a.part_BC + ((int64_t)(blockIdx.x % a.blocks) * a.rows.tokens * a.groups + q) * 2 * a.state + (n < N ? 0 : a.state) + state;
-            ld = (int64_t)a.groups * 2 * a.state;
-          }
-          to0 += (tile0 + f) * ld;
-#pragma unroll
-          for (int t = threadIdx.x / ACROSS; t < FT; t += THREADS / ACROSS)
+        constexpr int WIDE = 16 / sizeof(T), FOURS = 2 * N / WIDE;
+        if (a.blocks > 1 && a.state == N) {     // whole rows of the partial sums, 16 bytes at a time
+          T* to0 = a.part_BC + ((blockIdx.x % a.blocks * a.rows.tokens + tile0 + f) * a.groups + q) * 2 * N;
+          for (int i = threadIdx.x; i < FT * FOURS; i += THREADS) {
+            const int t = i / FOURS, n = i % FOURS * WIDE;
             if (f + t >= from && f + t < to) {
-              T sum = 0;
+              T sum[WIDE], next_sum[WIDE];
+              pick(&m.red[0][t][n], sum);
 #pragma unroll
-              for (int w = 0; w < K::WARPS; ++w) sum += m.red[w][t][n];
-              to0[t * ld] = sum;
+              for (int w = 1; w < K::WARPS; ++w) {
+                pick(&m.red[w][t][n], next_sum);
+#pragma unroll
+                for (int j = 0; j < WIDE; ++j) sum[j] += next_sum[j];
+              }
+              put(to0 + (int64_t)t * a.groups * 2 * N + n, sum);
             }
+          }
+        } else {
+          constexpr int ACROSS = 2 * N < THREADS ? 2 * N : THREADS;
+          for (int n = threadIdx.x % ACROSS; n < 2 * N; n += ACROSS) {
+            const int state = n < N ? n : n - N;
+            if (state >= a.state) continue;
+            T* to0 = n < N ? a.dB + q * a.state + state : a.dC + q * a.state + state;
+            int64_t ld = n < N ? a.ld_dB : a.ld_dC;
+            if (a.blocks > 1) {
+              to0 = a.part_BC + ((int64_t)(blockIdx.x % a.blocks) * a.rows.tokens * a.groups + q) * 2 * a.state + (n < N ? 0 : a.state) + state;
+              ld = (int64_t)a.groups * 2 * a.state;
+            }
+            to0 += (tile0 + f) * ld;
+#pragma unroll
+            for (int t = threadIdx.x / ACROSS; t < FT; t += THREADS / ACROSS)
+              if (f + t >= from && f + t < to) {
+                T sum = 0;
+#pragma unroll
+                for (int w = 0; w < K::WARPS; ++w) sum += m.red[w][t][n];
+                to0[t * ld] = sum;
+              }
+          }
         }
         if (f > 0) __syncthreads();
       }
