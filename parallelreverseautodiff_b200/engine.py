@@ -967,9 +967,15 @@ class Engine:
         _expect("selective_scan", _I32, ("offsets", offsets, (sequences + 1,)))
         s = _lib.Scan(u.shape[0], sequences, dim, state, groups, int(delta_softplus), *[None if m is None else m.ptr for m in (
             offsets, u, delta, z, A, B, C_, D, delta_bias, h0)])
-        for k, ld in (pitches or {}).items():
-            setattr(s, "ld_" + k, ld)
+        Engine._set_pitches(s, "ld_", pitches)
         return s
+
+    @staticmethod
+    def _set_pitches(struct, prefix, pitches):
+        for k, ld in (pitches or {}).items():
+            if k not in ("u", "delta", "z", "B", "C"):
+                raise _lib.PradError(_lib.ERR_INVALID, f"selective_scan: {k} has no pitch")
+            setattr(struct, prefix + k, ld)
 
     def selective_scan_saved(self, tokens, dim, state, dtype) -> int:
         """How many values `save` of selective_scan_forward needs."""
@@ -1010,9 +1016,11 @@ class Engine:
             if m is not None:
                 _expect("selective_scan_backward", u.dtype, ("gradient of " + k, out.get(k), m.shape))
         _expect("selective_scan_backward", u.dtype, ("dy", dy, u.shape))
+        n = self.selective_scan_saved(u.shape[0], s.dim, s.state, u.dtype) * u.dtype.itemsize
+        if saved is not None and saved.nbytes < n:
+            raise _lib.PradError(_lib.ERR_SHAPE, f"selective_scan_backward: saved has {saved.nbytes} bytes, not {n}")
         g = _lib.ScanGradients(*[self._p(out.get(k)) for k in ("u", "delta", "z", "A", "B", "C", "D", "delta_bias", "h0")])
-        for k, ld in (gradient_pitches or {}).items():
-            setattr(g, "ld_d" + k, ld)
+        self._set_pitches(g, "ld_d", gradient_pitches)
         check(self.lib.prad_selective_scan_backward(self.ctx, dtype_code(u.dtype), _byref(s), self._p(saved), dy.ptr, ld_dy, _byref(g)))
         return out
 

@@ -426,6 +426,26 @@ def test_matrices_that_do_not_fit_are_refused(engine):
     assert last.numpy().shape == (1, 32)
 
 
+def test_what_was_not_saved_and_pitches_of_nothing_are_refused(engine):
+    e = engine
+    m = lambda *s: e.zeros(s, np.float32)  # noqa: E731
+    u, A, B = m(20, 8), m(8, 4), m(20, 4)
+    scan = dict(u=u, delta=u, A=A, B=B, C=B)
+    _, _, saved = e.selective_scan_forward(**scan, save=True)
+    assert saved.size == e.selective_scan_saved(20, 8, 4, np.float32)
+    with pytest.raises(_lib.PradError) as err:          # what a shorter batch saved
+        e.selective_scan_backward(**scan, saved=e.empty((saved.size - 1,), np.float32), dy=u)
+    assert err.value.status == _lib.ERR_SHAPE
+    with pytest.raises(_lib.PradError) as err:          # a forward that kept nothing
+        e.selective_scan_backward(**scan, saved=None, dy=u)
+    assert err.value.status == _lib.ERR_INVALID
+    for call in (lambda: e.selective_scan_forward(**scan, pitches={"y": 8}), lambda: e.selective_scan_step(u, u, A, B, B, m(20, 32), pitches={"Z": 8}),
+                 lambda: e.selective_scan_backward(**scan, saved=saved, dy=u, gradient_pitches={"dz": 8})):
+        with pytest.raises(_lib.PradError) as err:
+            call()
+        assert err.value.status == _lib.ERR_INVALID
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f64"])
 def test_matrices_at_odd_addresses(engine, dtype):
     """One value behind an allocation's start nothing can be read sixteen bytes at a time: the same values as at its start."""
