@@ -59,9 +59,9 @@ template <typename T, bool VECTOR> __device__ __forceinline__ void store4(T* p, 
 }
 
 // A thread takes U blocks of four words, THREADS apart.  Bound by memory, and by how the CTAs come and what they compute beside it:
-// 65536 x 4096 floats with a residual take 592 us with as many CTAs as the device holds and a loop over the blocks, 463 us (7.0 TB/s of the three matrices) with a CTA
-// for every U * THREADS blocks, which the device starts one by one as others end; whole blocks take a path without tests, as the
-// generator's integers leave little room under the power limit.
+// 65536 x 4096 floats with a residual take 592 us with as many CTAs as the device holds and a loop over the blocks, 463 us (7.0 TB/s
+// of the three matrices) with a CTA for every U * THREADS blocks, which the device starts one by one as others end; whole blocks take
+// a path without tests, as the generator's integers leave little room under the power limit.
 constexpr int U = 4;
 template <typename T, bool RESIDUAL>
 __device__ __forceinline__ Four<T> drop(const Four<T>& in, const Four<T>& residual, int64_t block, uint64_t keep, T scale, uint64_t seed,
@@ -82,25 +82,23 @@ dropout_kernel(const T* x, const T* residual, T* y, int64_t n, uint64_t keep, T 
                const uint64_t* step) {
   chain_begin();
   if (step) offset += *step;
-  const int64_t blocks = (n + 3) / 4, stride = (int64_t)gridDim.x * THREADS * U;
-  for (int64_t b0 = (int64_t)blockIdx.x * THREADS * U + threadIdx.x; b0 < blocks; b0 += stride) {
-    if (VECTOR && (b0 + (U - 1) * THREADS + 1) * 4 <= n) {
-      Four<T> in[U], out[U];
+  const int64_t blocks = (n + 3) / 4, b0 = (int64_t)blockIdx.x * THREADS * U + threadIdx.x;
+  if (VECTOR && (b0 + (U - 1) * THREADS + 1) * 4 <= n) {
+    Four<T> in[U], out[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        in[i] = load4<T, true>(x + (b0 + i * THREADS) * 4, 4);
-        if (RESIDUAL) out[i] = load4<T, true>(residual + (b0 + i * THREADS) * 4, 4);
-      }
+    for (int i = 0; i < U; ++i) {
+      in[i] = load4<T, true>(x + (b0 + i * THREADS) * 4, 4);
+      if (RESIDUAL) out[i] = load4<T, true>(residual + (b0 + i * THREADS) * 4, 4);
+    }
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        store4<T, true>(y + (b0 + i * THREADS) * 4, drop<T, RESIDUAL>(in[i], out[i], b0 + i * THREADS, keep, scale, seed, offset), 4);
-    } else {
-      for (int64_t b = b0; b < blocks && b < b0 + U * THREADS; b += THREADS) {
-        const int left = n - b * 4 < 4 ? (int)(n - b * 4) : 4;
-        Four<T> in = load4<T, VECTOR>(x + b * 4, left), out;
-        if (RESIDUAL) out = load4<T, VECTOR>(residual + b * 4, left);
-        store4<T, VECTOR>(y + b * 4, drop<T, RESIDUAL>(in, out, b, keep, scale, seed, offset), left);
-      }
+    for (int i = 0; i < U; ++i)
+      store4<T, true>(y + (b0 + i * THREADS) * 4, drop<T, RESIDUAL>(in[i], out[i], b0 + i * THREADS, keep, scale, seed, offset), 4);
+  } else {
+    for (int64_t b = b0; b < blocks && b < b0 + U * THREADS; b += THREADS) {
+      const int left = n - b * 4 < 4 ? (int)(n - b * 4) : 4;
+      Four<T> in = load4<T, VECTOR>(x + b * 4, left), out;
+      if (RESIDUAL) out = load4<T, VECTOR>(residual + b * 4, left);
+      store4<T, VECTOR>(y + b * 4, drop<T, RESIDUAL>(in, out, b, keep, scale, seed, offset), left);
     }
   }
 }
@@ -109,8 +107,7 @@ template <typename T>
 static prad_status run(prad_ctx* ctx, const void* x, const void* residual, void* y, int64_t n, uint64_t keep, double scale,
                        uint64_t seed, uint64_t offset, const uint64_t* step) {
   const bool vector = (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) & 15) == 0;
-  const int64_t need = ceil_div((n + 3) / 4, THREADS * U);
-  const unsigned grid = (unsigned)(need < 0x7fffffff ? need : 0x7fffffff);
+  const unsigned grid = (unsigned)ceil_div((n + 3) / 4, THREADS * U);
   auto kernel = vector ? (residual ? dropout_kernel<T, true, true> : dropout_kernel<T, true, false>)
                        : (residual ? dropout_kernel<T, false, true> : dropout_kernel<T, false, false>);
   launch_chained(kernel, grid, THREADS, 0, ctx->stream, (const T*)x, (const T*)residual, (T*)y, n, keep, (T)scale, seed, offset, step);
@@ -128,6 +125,7 @@ extern "C" prad_status prad_dropout(prad_ctx* ctx, prad_dtype dt, const void* x,
   PRAD_REQUIRE(dtype_ok(dt), PRAD_ERR_INVALID, "prad_dropout: unknown dtype %d", (int)dt);
   PRAD_REQUIRE(n >= 0, PRAD_ERR_SHAPE, "prad_dropout: negative size");
   PRAD_REQUIRE(p >= 0.0 && p <= 1.0, PRAD_ERR_INVALID, "prad_dropout: p must be in [0, 1], got %g", p);
+  PRAD_REQUIRE(n <= (int64_t)0x7fffffff * 4 * drop::THREADS * drop::U, PRAD_ERR_UNSUPPORTED, "prad_dropout: too many values");
   PRAD_REQUIRE(n == 0 || (x && y), PRAD_ERR_INVALID, "prad_dropout: null pointer");
   PRAD_REQUIRE(natural(dt, x, residual, y) && ((uintptr_t)step & 7) == 0, PRAD_ERR_INVALID, "prad_dropout: unaligned pointer");
   PRAD_CHECK_CTX(ctx);

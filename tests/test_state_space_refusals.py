@@ -126,6 +126,11 @@ def test_norm_and_dropout_refuse():
         assert got == status and text in message, (over, message)
 
 
+def test_dropout_refuses_more_than_a_launch_holds():
+    got, message = _status("prad_dropout", None, 0, P, None, Q, 1 << 62, 0.5, 1, 2, None)
+    assert got == _lib.ERR_UNSUPPORTED and "too many" in message, message
+
+
 def test_the_structs_are_the_headers():
     assert C.sizeof(_lib.Scan) == 8 + 24 + 10 * 8 + 5 * 8 and _lib.Scan.offsets.offset == 32
     assert C.sizeof(_lib.ScanGradients) == 14 * 8
