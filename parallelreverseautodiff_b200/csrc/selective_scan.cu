@@ -780,18 +780,20 @@ template <int L, int S, typename T> __device__ __forceinline__ void channel_sums
 template <typename T, int L, int S> struct Backward {
   static constexpr int CC = sizeof(T) == 8 && L < 32 ? 1 : 2, HALF = THREADS / L, CH = CC * HALF, TT = POINT, N = L * S, P = S / 2;
   static constexpr int WARPS = THREADS / 32;
-  // In double what a thread keeps for itself stays in registers, and fewer tokens are gathered at a time: two CTAs fit an SM.
-  static constexpr bool OWN = sizeof(T) == 8;
+  // In double the decays are kept for the way back beside the states: an exponential takes as long there as all else of a token's
+  // state, and shared memory has room for them, as registers leave two CTAs to an SM either way.
+  static constexpr bool KEEP = sizeof(T) == 8;
   // tokens whose dB and dC are gathered at a time
-  static constexpr int MOST = OWN ? 4 : 8, FT = 8 * 16 / N < 2 ? 2 : 8 * 16 / N < MOST ? 8 * 16 / N : MOST;
+  static constexpr int FT = 8 * 16 / N < 2 ? 2 : 8 * 16 / N < 8 ? 8 * 16 / N : 8;
   struct alignas(16) Step { T dt, gB, x, gA; };                       // in float first {dt, dt, x, x}
   struct Shared {
     Pack<T, S> h[CC][TT + 1][THREADS];                                // the state in front of each token, and behind the last
+    Pack<T, S> a[KEEP ? CC : 1][KEEP ? TT : 1][KEEP ? THREADS : 1];   // the decays, where they are kept
     alignas(16) T B[2][TT][N], C[2][TT][N];
     Step step[TT][CH];
     alignas(16) T red[WARPS][FT][2 * N];
-    alignas(16) T v[TT][CH], u[TT][CH], slope[TT][CH], w[OWN ? 1 : TT][CH];      // slope: d dt / d delta, w: dz / r
-    alignas(16) T r[TT][CH + (OWN ? 4 : 8)];
+    alignas(16) T v[TT][CH], u[TT][CH], slope[TT][CH], w[TT][CH];      // slope: d dt / d delta, w: dz / r
+    alignas(16) T r[TT][CH + 32 / sizeof(T)];
     int begins[TT];                                                   // the sequence that begins at a token
   };
 };
@@ -916,7 +918,6 @@ backward_kernel(const Args<T> a) {
     for (int64_t tile0 = top; tile0 >= bottom; tile0 -= TT) {
       const int buf = (int)(tile0 / TT & 1);
       const int from = begin > tile0 ? (int)(begin - tile0) : 0, to = finish < tile0 + TT ? (int)(finish - tile0) : TT;
-      T own_w[E][V];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int r = mine.row + i * ROWS;
@@ -943,11 +944,8 @@ backward_kernel(const Args<T> a) {
           put(&m.v[r][mine.col], v);
           put(&m.u[r][mine.col], u[i]);
           put(&m.slope[r][mine.col], slope);
-          if constexpr (!K::OWN) put(&m.w[r][mine.col], w);
+          put(&m.w[r][mine.col], w);
         }
-        if constexpr (K::OWN)
-#pragma unroll
-          for (int j = 0; j < V; ++j) own_w[i][j] = w[j];
       }
       Two<T> h[CC][P];
 #pragma unroll
@@ -992,14 +990,17 @@ backward_kernel(const Args<T> a) {
           for (int k = 0; k < CC; ++k) {
             Two<T> dt, x, r;
             read_step(&m.step[t][at0[k]].dt, dt, x);
-            Pack<T, S> now;
+            Pack<T, S> now, decays;
 #pragma unroll
             for (int j = 0; j < P; ++j) {
-              h[k][j] = fma(decay(mul(dt, A[k][j])), h[k][j], mul(x, B[j]));
+              const Two<T> d = decay(mul(dt, A[k][j]));
+              if constexpr (K::KEEP) d.get(decays.v[2 * j], decays.v[2 * j + 1]);
+              h[k][j] = fma(d, h[k][j], mul(x, B[j]));
               h[k][j].get(now.v[2 * j], now.v[2 * j + 1]);
               r = j ? fma(C[j], h[k][j], r) : mul(C[j], h[k][j]);
             }
             m.h[k][t + 1][threadIdx.x] = now;
+            if constexpr (K::KEEP) m.a[k][t][threadIdx.x] = decays;
             sums[k] = total(r);
           }
         };
@@ -1055,10 +1056,13 @@ backward_kernel(const Args<T> a) {
               read_step(&m.step[t][at0[k]].dt, dt, x);
               const T v1 = m.v[t][ch0 + k * HALF];
               const Two<T> v = {v1, v1};
+              Two<T> decays[P];
+              if constexpr (K::KEEP) read(m.a[k][t][threadIdx.x].v, decays);
 #pragma unroll
               for (int j = 0; j < P; ++j) {
                 const Two<T> g = fma(C[j], v, e[k][j]);
-                e[k][j] = mul(decay(mul(dt, A[k][j])), g);
+                if constexpr (K::KEEP) e[k][j] = mul(decays[j], g);
+                else e[k][j] = mul(decay(mul(dt, A[k][j])), g);
                 const Two<T> w = mul(e[k][j], before[k][j]);
                 gB = j ? fma(g, B[j], gB) : mul(g, B[j]);
                 gA = j ? fma(w, A[k][j], gA) : mul(w, A[k][j]);
@@ -1200,12 +1204,7 @@ backward_kernel(const Args<T> a) {
         pick(&m.u[r][mine.col], ut);
         pick(&m.v[r][mine.col], v);
         pick(&m.slope[r][mine.col], slope);
-        if constexpr (!K::OWN) {
-          pick(&m.w[r][mine.col], w);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) w[j] = own_w[i][j];
-        }
+        pick(&m.w[r][mine.col], w);
         pick(&m.r[r][mine.col], rt);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
