@@ -1250,12 +1250,8 @@ backward_kernel(const Args<T> a) {
   }
 }
 
-// sums of the spans, in double: dA, then dD and dbias
-template <typename T>
-__global__ void __launch_bounds__(THREADS)
-span_totals_kernel(const Args<T> a) {
-  chain_begin();
-  int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+// Value i of dA, then of dD and of dbias: the sum of the spans, in double.
+template <typename T> __device__ __forceinline__ void span_total(const Args<T>& a, int64_t i) {
   const int64_t states = (int64_t)a.dim * a.state;
   const T* from = a.part_A;
   T* to = a.dA;
@@ -1275,22 +1271,35 @@ span_totals_kernel(const Args<T> a) {
   for (int p = 0; p < a.spans; ++p) sum += (double)from[p * each + i];
   to[i] = (T)sum;
 }
-
-// dB and dC: sums of the CTAs of a group
-template <typename T>
-__global__ void __launch_bounds__(256)
-row_totals_kernel(const Args<T> a) {
-  chain_begin();
+// Pack i of V values of dB and dC: the sum of the CTAs of a group.
+template <typename T, int V> __device__ __forceinline__ void row_total(const Args<T>& a, int64_t i) {
   const int64_t lo = a.rows.begin(), hi = a.rows.finish(), each = (int64_t)a.groups * 2 * a.state;
-  const int64_t i = lo * each + (int64_t)blockIdx.x * 256 + threadIdx.x;
+  i = lo * each + i * V;
   if (i >= hi * each) return;
   const int64_t row = i / each, stride = a.rows.tokens * each;
-  const int q = (int)(i % each / (2 * a.state)), n = (int)(i % (2 * a.state));
-  T sum = 0;
+  const int at = (int)(i % each), q = at / (2 * a.state), n = at % (2 * a.state);
+  T sum[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum[j] = 0;
 #pragma unroll 8
-  for (int b = 0; b < a.blocks; ++b) sum += a.part_BC[b * stride + i];
-  if (n < a.state) a.dB[row * a.ld_dB + q * a.state + n] = sum;
-  else a.dC[row * a.ld_dC + q * a.state + n - a.state] = sum;
+  for (int b = 0; b < a.blocks; ++b) {
+    const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(a.part_BC + b * stride + i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] += w.v[j];
+  }
+  T* to = n < a.state ? a.dB + row * a.ld_dB + q * a.state + n : a.dC + row * a.ld_dC + q * a.state + n - a.state;
+#pragma unroll
+  for (int j = 0; j < V; ++j) to[j] = sum[j];
+}
+// the CTAs below `span_blocks` take the spans' sums, the others the rows', 16 bytes at a time where states come in such packs
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+totals_kernel(const Args<T> a, int span_blocks) {
+  chain_begin();
+  constexpr int V = 16 / sizeof(T);
+  if ((int)blockIdx.x < span_blocks) span_total(a, (int64_t)blockIdx.x * THREADS + threadIdx.x);
+  else if (a.state % V == 0) row_total<T, V>(a, (int64_t)(blockIdx.x - span_blocks) * THREADS + threadIdx.x);
+  else row_total<T, 1>(a, (int64_t)(blockIdx.x - span_blocks) * THREADS + threadIdx.x);
 }
 
 // ---------------------------------------------------------------- one token
@@ -1459,6 +1468,11 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
+  // of the last launch: the spans' sums, and the rows of dB and dC in packs
+  constexpr int V = 16 / (int)sizeof(T);
+  const int64_t span_blocks = ceil_div(states + 2 * (int64_t)a.dim, THREADS);
+  const int64_t packs = a.blocks > 1 ? a.rows.tokens * a.groups * 2 * a.state / (a.state % V ? 1 : V) : 0;
+  PRAD_REQUIRE(span_blocks + ceil_div(packs, THREADS) <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many rows of B and C");
   if (a.dh0) PRAD_CUDA(cudaMemsetAsync(a.dh0, 0, (size_t)a.rows.count * states * sizeof(T), ctx->stream));
   if (joined(a)) {
     Args<T> b = a;
@@ -1470,14 +1484,8 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   }
   launch_chained(backward_kernel<T, L, S>, dim3(x, (unsigned)a.spans), THREADS, sizeof(Shared), ctx->stream, a);
   PRAD_LAUNCHED(ctx);
-  launch_chained(span_totals_kernel<T>, (unsigned)ceil_div(states + 2 * (int64_t)a.dim, THREADS), THREADS, 0, ctx->stream, a);
+  launch_chained(totals_kernel<T>, (unsigned)(span_blocks + ceil_div(packs, THREADS)), THREADS, 0, ctx->stream, a, (int)span_blocks);
   PRAD_LAUNCHED(ctx);
-  if (a.blocks > 1 && a.rows.tokens) {
-    const int64_t n = a.rows.tokens * a.groups * 2 * a.state;
-    PRAD_REQUIRE(ceil_div(n, 256) <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many rows of B and C");
-    launch_chained(row_totals_kernel<T>, (unsigned)ceil_div(n, 256), 256, 0, ctx->stream, a);
-    PRAD_LAUNCHED(ctx);
-  }
   return PRAD_OK;
 }
 template <typename T> static prad_status pick(prad_ctx* ctx, Args<T> a, Pass pass) {
