@@ -8,7 +8,8 @@
 // blocks again, now out of the L2.  Too few samples for that, or groups wider than a CTA: sums and results in launches of their own.
 // Floats, forward and backward: 16384 rows of 2048 in groups of 128, 52 and 70 us (5.2 and 5.8 TB/s); 64 samples of 3136 positions and
 // 96 channels in groups of 12 with swish, 39 and 70 us (3.9 and 3.3 TB/s: the clusters of the whole input run at once, so that
-// backward its second reading misses the L2; clusters of 16, or blocks of half the channels, took 14 and 17 us longer).
+// backward its second reading misses the L2; clusters of 16, or blocks of half the channels, took 14 and 17 us longer, and blocks that
+// stay in shared memory, so that fewer of them run at a time, 54 and 113 us).
 //
 // Means and variances are summed around a pivot out of the data (the average of the group's first values), so that a mean far
 // from zero takes nothing from the variance; sums go from float to double every few values.
@@ -264,6 +265,13 @@ template <typename T> struct Place {
   }
 };
 
+// The second reading of a block goes from its end to its start, as what was read last is what the caches still have (64 images of 3136
+// positions and 96 channels, forward and backward: 117.5 us, 119.3 from start to end): N rows of a thread at a time, from these on.
+template <int N, typename T> __device__ __forceinline__ int64_t last_rows(const Place<T>& w) {
+  const int64_t mine = w.p1 - w.p0 - w.ty - 1;       // (negative: none)
+  return mine < 0 ? w.p0 - 1 : w.p0 + w.ty + mine / ((int64_t)N * w.rows) * N * w.rows;
+}
+
 // the average of four values of a group
 template <typename T> __device__ __forceinline__ double pivot(const Args<T>& a, int64_t s, int g) {
   const T* x = a.x + s * a.positions * a.channels + (int64_t)g * a.per;
@@ -382,7 +390,7 @@ __device__ __forceinline__ void apply(const Args<T>& a, const Place<T>& w, const
     const Pack<T, V> gammas = parameters<T, V>(a, a.gamma, c, (T)1), betas = parameters<T, V>(a, a.beta, c, (T)0);
     const T(&gamma)[V] = gammas.v;
     const T(&beta)[V] = betas.v;
-    for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)4 * w.rows) {
+    for (int64_t p = last_rows<4>(w); p >= w.p0; p -= (int64_t)4 * w.rows) {
       Pack<T, V> v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -564,7 +572,7 @@ __device__ __forceinline__ void input_gradients(const Args<T>& a, const Place<T>
     const Pack<T, V> gammas = parameters<T, V>(a, a.gamma, c, (T)1), betas = parameters<T, V>(a, a.beta, c, (T)0);
     const T(&gamma)[V] = gammas.v;
     const T(&beta)[V] = betas.v;
-    for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)2 * w.rows) {
+    for (int64_t p = last_rows<2>(w); p >= w.p0; p -= (int64_t)2 * w.rows) {
       Pack<T, V> x[2], d[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r)

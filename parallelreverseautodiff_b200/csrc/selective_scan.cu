@@ -15,12 +15,13 @@
 // the state it has.  The backward pass runs the same way from the last span up, on checkpoints of the state every POINT tokens that
 // the forward pass leaves.
 //
-// 16384 tokens of 1024 float channels with 16 states: edges 97 us, main pass 132 us (a prompt; the exponentials alone would take 60 us
-// each time, the memory 42 us); backward edges 80 us, main pass 431 us.  In both main passes about half of the cycles of the special
-// function unit, of the multiply-add pipe and of the issue slots are used, at the same time: chains of dependent instructions on the
-// twelve (backward) and sixteen warps that registers leave to an SM are what is left.  Tried and taken back: more CTAs with fewer
-// registers each (spills; 162 us for 155 forward), one channel a thread backward (604 us for 575 then), and exponentials by polynomials,
-// which take more issue slots than they free.
+// 16384 tokens of 1024 float channels with 16 states: edges 93 us, main pass 132 us (a prompt; the exponentials alone would take 60 us
+// each time, the memory 42 us); backward edges 78 us, main pass 431 to 446 us on two devices.  The edges' passes use the special
+// function unit at 70 %.  In both main passes no unit is used much above half of its cycles, and several are at the same time: chains
+// of dependent instructions on the twelve (backward) and sixteen warps that registers leave to an SM are what is left.  Tried and taken
+// back: more CTAs with fewer registers each (spills; 162 us for 155 forward), one channel a thread backward (614 us for 446, four CTAs
+// an SM), and exponentials by polynomials (every fourth pair in the edges' passes: 95 us for 93, backward 83 for 78), which take more
+// issue slots than they free.
 #include "common.cuh"
 #include "packed_sequences.cuh"
 
