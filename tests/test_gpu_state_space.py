@@ -133,6 +133,28 @@ def test_scan_without_some_inputs(engine, dtype, absent, softplus):
     check_scan(engine, dtype, [40, 3, 20], 34, 10, 2, softplus=softplus, **{absent: False})
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+@pytest.mark.parametrize("lengths,d,n", [([40, 0, 3], 5, 3), ([700], 33, 16), ([1500, 900], 9, 70)])
+def test_steps_of_no_time_leave_the_states_as_they_are(engine, dtype, lengths, d, n):
+    """A decay over no time is 1 exactly, however many tokens it is repeated for, and both ways."""
+    e, f, T, S = engine, F[dtype], sum(lengths), len(lengths)
+    x = scan_case(np.random.default_rng(T), f, T, d, n, 1, S, z=False, D=False, bias=False)
+    x["delta"][:] = 0
+    x["C"][:] = 0
+    dev = {k: e.upload(v) for k, v in x.items()}
+    of = dict(dev, sequences=S, offsets=e.sequence_offsets(lengths), delta_softplus=False)
+    _, last, saved = e.selective_scan_forward(**of, h_last=True, save=True)
+    assert np.array_equal(last.numpy(), x["h0"])
+    # only the last tokens ask for a state: its gradient reaches the first one unchanged
+    ends = np.cumsum(lengths) - 1
+    x["C"][ends] = 1
+    dy = np.zeros((T, d), f)
+    dy[ends] = 0.375
+    grads = e.selective_scan_backward(**dict(of, C=e.upload(x["C"])), saved=saved, dy=e.upload(dy))
+    want = np.repeat([0.375 if m else 0.0 for m in lengths], d * n).reshape(S, d * n)
+    assert np.array_equal(grads["h0"].numpy(), want.astype(f))
+
+
 def test_scan_gradients_against_differences(engine):
     """The double kernels against central differences of their own forward, along one random direction in all inputs at once.
     With h = 1e-5 the third derivatives leave about h^2 = 1e-10 of the functional's scale, rounding 1e-16 / h = 1e-11 of it."""
