@@ -121,6 +121,13 @@ def test_scan_in_spans(engine, dtype, lengths):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f64"])
+@pytest.mark.parametrize("n", [8, 16, 32, 64, 128])
+def test_scan_of_many_channels_in_spans(engine, dtype, n):
+    """Sums of dB and dC over several CTAs' channels, tile by tile, where the states fill the lanes."""
+    check_scan(engine, dtype, [3, 700, 45, 0, 301], 150, n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
 @pytest.mark.parametrize("lengths,d", [([50] * 3, 33), ([1] * 9, 64), ([7] * 40, 5), ([100] * 30, 700)])
 def test_scan_of_equal_sequences(engine, dtype, lengths, d):
     check_scan(engine, dtype, lengths, d, 6, packed=False)
