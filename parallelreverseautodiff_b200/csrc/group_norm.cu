@@ -54,23 +54,38 @@ __device__ __forceinline__ double inverse_root(double x) { return 1.0 / sqrt(x);
 // ---------------------------------------------------------------- one position per sample
 // LW lanes share the values of a (sample, group), E packs of V values each; a lane keeps its channels for all its samples, so the
 // sums for dgamma and dbeta stay in registers as well.  Slot k of the grid takes group k mod groups: neighbouring slots read
-// neighbouring memory.
+// neighbouring memory; its samples are `step` apart.
 template <int LW, typename A> __device__ __forceinline__ A lanes_sum(A v) {
 #pragma unroll
   for (int o = LW / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
+// the first sample of a slot, and its group
+struct Slot {
+  int64_t row;
+  int group;
+  __device__ __forceinline__ Slot(int64_t slot, int groups) {
+    if (slot >> 32 == 0) {         // (a division of 64 bits takes as long as a row's arithmetic)
+      const uint32_t q = (uint32_t)slot / (uint32_t)groups;
+      row = q;
+      group = (int)((uint32_t)slot - q * (uint32_t)groups);
+    } else {
+      row = slot / groups;
+      group = (int)(slot - row * groups);
+    }
+  }
+};
+
 // samples of a slot in the forward pass, whose values are on their way at the same time
 template <int E> constexpr int rows_at_once() { return E == 1 ? 4 : E == 2 ? 2 : 1; }
 template <typename T, int V, int LW, int E>
 __global__ void __launch_bounds__(THREADS)
-rows_forward_kernel(const Args<T> a, int64_t slots) {
+rows_forward_kernel(const Args<T> a, int64_t step) {
   chain_begin();
   constexpr int R = rows_at_once<E>();
-  const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
-  const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
-  const int64_t step = slots / a.groups;
+  const Slot slot(((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW, a.groups);
+  const int l = threadIdx.x % LW, g = slot.group;
   int c[E];
   bool on[E];
   Pack<T, V> gamma[E], beta[E];
@@ -84,7 +99,7 @@ rows_forward_kernel(const Args<T> a, int64_t slots) {
     }
   }
   // all lanes of a warp take part in its sums: those beyond the last sample with nothing to add
-  const int64_t first = slot < slots ? slot / a.groups : a.samples;
+  const int64_t first = slot.row < step ? slot.row : a.samples;
   const T inv = (T)1 / (T)a.per, eps = (T)a.eps;
   Pack<T, V> x[R][E];
 #pragma unroll
@@ -136,11 +151,10 @@ rows_forward_kernel(const Args<T> a, int64_t slots) {
 // partial[row block][2][channels]: this slot's sums of dv xhat and of dv
 template <typename T, int V, int LW, int E>
 __global__ void __launch_bounds__(THREADS)
-rows_backward_kernel(const Args<T> a, int64_t slots, T* __restrict__ partial) {
+rows_backward_kernel(const Args<T> a, int64_t step, T* __restrict__ partial) {
   chain_begin();
-  const int64_t slot = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW;
-  const int l = threadIdx.x % LW, g = (int)(slot % a.groups);
-  const int64_t step = slots / a.groups;
+  const Slot slot(((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW, a.groups);
+  const int l = threadIdx.x % LW, g = slot.group;
   int c[E];
   bool on[E];
   Pack<T, V> gamma[E], beta[E], dg[E], db[E];
@@ -156,7 +170,7 @@ rows_backward_kernel(const Args<T> a, int64_t slots, T* __restrict__ partial) {
       dg[e].v[j] = db[e].v[j] = 0;
     }
   }
-  const int64_t first = slot < slots ? slot / a.groups : a.samples;
+  const int64_t first = slot.row < step ? slot.row : a.samples;
   const int64_t rounds = (a.samples + step - 1) / step;
   const T inv = (T)1 / (T)a.per;
   for (int64_t k = 0; k < rounds; ++k) {
@@ -200,13 +214,13 @@ rows_backward_kernel(const Args<T> a, int64_t slots, T* __restrict__ partial) {
         *reinterpret_cast<Pack<T, V>*>(a.dx + at + c[e]) = d[e];
       }
   }
-  if (slot < slots)
+  if (slot.row < step)
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (on[e])
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          T* to = partial + (slot / a.groups * 2) * a.channels + g * a.per + c[e] + j;
+          T* to = partial + (slot.row * 2) * a.channels + g * a.per + c[e] + j;
           to[0] = dg[e].v[j];
           to[a.channels] = db[e].v[j];
         }
@@ -682,13 +696,13 @@ template <typename T, int V, int LW, int E> static prad_status rows(prad_ctx* ct
   const int64_t grid = ceil_div(slots * LW, THREADS);
   PRAD_REQUIRE(grid <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "group norm: too many groups");
   if (!backward) {
-    launch_chained(rows_forward_kernel<T, V, LW, E>, (unsigned)grid, THREADS, 0, ctx->stream, a, slots);
+    launch_chained(rows_forward_kernel<T, V, LW, E>, (unsigned)grid, THREADS, 0, ctx->stream, a, per_group);
     PRAD_LAUNCHED(ctx);
     return PRAD_OK;
   }
   prad_status st = ensure_workspace(ctx, (size_t)per_group * 2 * a.channels * sizeof(T));
   if (st) return st;
-  launch_chained(rows_backward_kernel<T, V, LW, E>, (unsigned)grid, THREADS, 0, ctx->stream, a, slots, (T*)ctx->ws);
+  launch_chained(rows_backward_kernel<T, V, LW, E>, (unsigned)grid, THREADS, 0, ctx->stream, a, per_group, (T*)ctx->ws);
   PRAD_LAUNCHED(ctx);
   if (a.dgamma || a.dbeta) {
     launch_chained(column_totals_kernel<T, T>, dim3((unsigned)ceil_div(a.channels, 32), 2), TOTALS, 0, ctx->stream, (const T*)ctx->ws, per_group,
