@@ -6,7 +6,7 @@
 // the registers of a few lanes, one pass over the memory each way.  Several positions: a cluster of CTAs takes a sample (or some of
 // its groups), each CTA a block of its positions; they sum, exchange the sums through each other's shared memory and read their
 // blocks again, now out of the L2.  Too few samples for that, or groups wider than a CTA: sums and results in launches of their own.
-// Floats, forward and backward: 16384 rows of 2048 in groups of 128, 52 and 70 us (5.2 and 5.8 TB/s); 64 samples of 3136 positions and
+// Floats, forward and backward: 16384 rows of 2048 in groups of 128, 49 and 66 us (5.5 and 6.1 TB/s); 64 samples of 3136 positions and
 // 96 channels in groups of 12 with swish, 39 and 70 us (3.9 and 3.3 TB/s: the clusters of the whole input run at once, so that
 // backward its second reading misses the L2; clusters of 16, or blocks of half the channels, took 14 and 17 us longer, and blocks that
 // stay in shared memory, so that fewer of them run at a time, 54 and 113 us).
@@ -150,7 +150,7 @@ rows_forward_kernel(const Args<T> a, int64_t step) {
 
 // partial[row block][2][channels]: this slot's sums of dv xhat and of dv
 template <typename T, int V, int LW, int E>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 && E == 1 ? 4 : 0)
 rows_backward_kernel(const Args<T> a, int64_t step, T* __restrict__ partial) {
   chain_begin();
   const Slot slot(((int64_t)blockIdx.x * THREADS + threadIdx.x) / LW, a.groups);
@@ -173,18 +173,42 @@ rows_backward_kernel(const Args<T> a, int64_t step, T* __restrict__ partial) {
   const int64_t first = slot.row < step ? slot.row : a.samples;
   const int64_t rounds = (a.samples + step - 1) / step;
   const T inv = (T)1 / (T)a.per;
+  // One pack of floats a lane: the next sample's is on its way while this one's sums go round (16384 rows of 2048 in groups of 128,
+  // forward and backward: 122 us, 126 without, and 131 if its registers take a CTA of an SM's four); more have no registers for it.
+  constexpr bool AHEAD = sizeof(T) == 4 && E == 1;
+  Pack<T, V> next_x, next_d;
+  T next_mean = 0, next_rstd = 0;
+  const auto fetch = [&](int64_t s) {
+    if (s >= a.samples) return;
+    const int64_t at = s * a.channels + (int64_t)g * a.per;
+    next_mean = a.mean[s * a.groups + g];
+    next_rstd = a.rstd[s * a.groups + g];
+    if (on[0]) {
+      next_x = load<T, V>(a.x + at + c[0]);
+      next_d = load<T, V>(a.dy + at + c[0]);
+    }
+  };
+  if constexpr (AHEAD) fetch(first);
   for (int64_t k = 0; k < rounds; ++k) {
     const int64_t s = first + k * step;
     const bool live = s < a.samples;
     const int64_t at = s * a.channels + (int64_t)g * a.per;
-    const T mean = live ? a.mean[s * a.groups + g] : (T)0, rstd = live ? a.rstd[s * a.groups + g] : (T)0;
+    T mean, rstd;
     Pack<T, V> x[E], d[E];
     T s1 = 0, s2 = 0;
+    if constexpr (AHEAD) {
+      mean = next_mean, rstd = next_rstd;
+      x[0] = next_x, d[0] = next_d;
+      fetch(s + step);
+    } else {
+      mean = live ? a.mean[s * a.groups + g] : (T)0;
+      rstd = live ? a.rstd[s * a.groups + g] : (T)0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (live && on[e]) {
-        x[e] = load<T, V>(a.x + at + c[e]);
-        d[e] = load<T, V>(a.dy + at + c[e]);
+      for (int e = 0; e < E; ++e) {
+        if (live && on[e]) {
+          x[e] = load<T, V>(a.x + at + c[e]);
+          d[e] = load<T, V>(a.dy + at + c[e]);
+        }
       }
     }
 #pragma unroll
