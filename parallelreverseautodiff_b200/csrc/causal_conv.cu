@@ -418,11 +418,12 @@ enum class Pass { Forward, Backward, Step };
 
 template <typename T, int V, int W, bool BACKWARD> static prad_status launch(prad_ctx* ctx, Args<T> a, Pass pass) {
   const unsigned across = (unsigned)ceil_div(a.dim, LANES * V);
-  if (!BACKWARD && pass == Pass::Step) {
-    launch_chained(step_kernel<T, V, W>, dim3((unsigned)ceil_div(a.rows.tokens, WARPS), across), THREADS, 0, ctx->stream, a, a.rows.tokens);
-    PRAD_LAUNCHED(ctx);
-    return PRAD_OK;
-  }
+  if constexpr (!BACKWARD)
+    if (pass == Pass::Step) {
+      launch_chained(step_kernel<T, V, W>, dim3((unsigned)ceil_div(a.rows.tokens, WARPS), across), THREADS, 0, ctx->stream, a, a.rows.tokens);
+      PRAD_LAUNCHED(ctx);
+      return PRAD_OK;
+    }
   // Runs of 32 tokens, of 64 backward (16384 tokens of 2048 floats: forward 45 us, 51 with 64; backward 93 us, 85 with 64), or shorter
   // ones where those give less than two CTAs an SM (2047 tokens of 333 doubles, backward: 26 us with runs of 32, 13 with runs of 8).
   a.run = BACKWARD ? 64 : 32;

@@ -1466,8 +1466,10 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
       if (b.z) b.z += r0 * a.ld_z;
       b.h0 += r0 * states, b.h_last += r0 * states;
       const dim3 grid((unsigned)across, (unsigned)ceil_div(b.rows.tokens, R));
-      if (R == 1) launch_chained(step_kernel<T, L, S, 1>, grid, THREADS, 0, ctx->stream, b);
-      else launch_chained(step_kernel<T, L, S, 4>, grid, THREADS, 0, ctx->stream, b);
+      void (*kernel)(const Args<T>) = step_kernel<T, L, S, 1>;
+      if constexpr (sizeof(T) == 4)
+        if (R == 4) kernel = step_kernel<T, L, S, 4>;
+      launch_chained(kernel, grid, THREADS, 0, ctx->stream, b);
       PRAD_LAUNCHED(ctx);
     }
     return PRAD_OK;
