@@ -968,9 +968,9 @@ class StateSpaceBlock:
                  "B": dbc.view((T, n), self.rank), "C": dbc.view((T, n), self.rank + n)}
         return parts, {"z": 2 * d, "B": self.columns, "C": self.columns}
 
-    def _mix(self, x, T, convolve):
-        """x -> uz, c, dbc, delta; `convolve` is the convolution of a prompt or of single tokens."""
-        e, p, d, B_ = self.eng, self.p, self.inner, self._buf
+    def _mix(self, x, T, convolve, B_):
+        """x -> uz, c, dbc, delta; `convolve` is the convolution of a prompt or of single tokens, `B_` gives the buffers."""
+        e, p, d = self.eng, self.p, self.inner
         uz, dbc, delta = B_("uz", (T, 2 * d)), B_("dbc", (T, self.columns)), B_("delta", (T, d))
         e.matmul_forward(x, p["Win"], Y=uz)
         c = convolve(uz.view((T, d)), B_("c", (T, d)))
@@ -978,13 +978,13 @@ class StateSpaceBlock:
         e.gemm(dbc, p["Wdt"], delta, M=T, N=d, K=self.rank, lda=self.columns)
         return uz, c, dbc, delta
 
-    def _project(self, x, y, T, drop, step):
-        """y -> x + dropout(groupnorm(y) Wout)."""
-        e, p, d, B_ = self.eng, self.p, self.inner, self._buf
-        self.norm = e.group_norm_forward(y, self.norm_groups, p["gamma"], p["beta"], out=(B_("v", (T, d)), B_("mean", (T, self.norm_groups)),
-                                                                                       B_("rstd", (T, self.norm_groups))))
-        proj = e.matmul_forward(self.norm[0], p["Wout"], Y=B_("proj", (T, self.dim)))
-        return e.dropout(proj, self.p_drop if drop else 0.0, self.seed, 0, residual=x, step=step, out=B_("out", (T, self.dim)))
+    def _project(self, x, y, T, drop, step, B_):
+        """y -> v, mean, rstd = groupnorm(y) and x + dropout(v Wout)."""
+        e, p, d = self.eng, self.p, self.inner
+        norm = e.group_norm_forward(y, self.norm_groups, p["gamma"], p["beta"], out=(B_("v", (T, d)), B_("mean", (T, self.norm_groups)),
+                                                                                  B_("rstd", (T, self.norm_groups))))
+        proj = e.matmul_forward(norm[0], p["Wout"], Y=B_("proj", (T, self.dim)))
+        return norm, e.dropout(proj, self.p_drop if drop else 0.0, self.seed, 0, residual=x, step=step, out=B_("out", (T, self.dim)))
 
     def forward(self, x: E.DeviceMatrix, offsets=None, sequences=1, states=None, states_out=None, training=True, step=None):
         """x [tokens x dim].  `states`: in front of the sequences (new_states or an earlier states_out), `states_out`: to take those
@@ -996,17 +996,17 @@ class StateSpaceBlock:
         self.before = before
         conv = lambda u, out: e.causal_conv_forward(u, p["Wc"], p["bc"], before["conv"], **self.rows, out=out,  # noqa: E731
                                                     state_out=after["conv"], ld_x=2 * d)[0]
-        self.uz, self.c, self.dbc, self.delta = self._mix(x, T, conv)
+        self.uz, self.c, self.dbc, self.delta = self._mix(x, T, conv, B_)
         parts, pitches = self._parts(self.uz, self.dbc)
         saved = B_("saved", (e.selective_scan_saved(T, d, self.state, self.dtype),)) if training else False
         self.y, _, self.saved = e.selective_scan_forward(
             self.c, self.delta, p["A"], parts["B"], parts["C"], p["D"], parts["z"], p["bdt"], before["h"], groups=self.groups, **self.rows,
             out=B_("y", (T, d)), h_last=after["h"], save=saved, pitches=pitches)
-        self.out = self._project(x, self.y, T, training, step)
+        self.norm, self.out = self._project(x, self.y, T, training, step, B_)
         return self.out
 
     def backward(self, d_out: E.DeviceMatrix):
-        """Gradients of the parameters into `g` (and of the states into d_states, where there were any); returns d_x."""
+        """Gradients of the last forward's parameters into `g` (and of the states into d_states, where there were any); returns d_x."""
         e, p, g, d, T, B_ = self.eng, self.p, self.g, self.inner, d_out.shape[0], self._buf
         parts, pitches = self._parts(self.uz, self.dbc)
         d_proj = e.dropout(d_out, self.p_drop if self.training else 0.0, self.seed, 0, step=self.step_counter, out=B_("d_proj", (T, self.dim)))
@@ -1039,11 +1039,12 @@ class StateSpaceBlock:
         return d_x
 
     def step(self, x: E.DeviceMatrix, states):
-        """One new token [sequences x dim] for each sequence; `states` are replaced."""
+        """One new token [sequences x dim] for each sequence; `states` are replaced.  What a forward keeps for its backward stays."""
         e, p, T = self.eng, self.p, x.shape[0]
+        B_ = lambda name, shape: self._buf("step " + name, shape)  # noqa: E731
         conv = lambda u, out: e.causal_conv_step(u, p["Wc"], states["conv"], p["bc"], out=out, ld_x=2 * self.inner)  # noqa: E731
-        uz, c, dbc, delta = self._mix(x, T, conv)
+        uz, c, dbc, delta = self._mix(x, T, conv, B_)
         parts, pitches = self._parts(uz, dbc)
         y = e.selective_scan_step(c, delta, p["A"], parts["B"], parts["C"], states["h"], p["D"], parts["z"], p["bdt"], groups=self.groups,
-                                  out=self._buf("y", (T, self.inner)), pitches=pitches)
-        return self._project(x, y, T, False, None)
+                                  out=B_("y", (T, self.inner)), pitches=pitches)
+        return self._project(x, y, T, False, None, B_)[1]
