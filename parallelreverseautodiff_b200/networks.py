@@ -28,6 +28,7 @@ from typing import Callable, List, Optional, Sequence
 
 import numpy as np
 
+from . import _lib
 from . import engine as E
 
 
@@ -951,7 +952,7 @@ class StateSpaceBlock:
         self.p = {"Win": z(dim, 2 * d), "Wc": z(d, width), "bc": z(d), "Wx": z(d, self.columns), "Wdt": z(self.rank, d), "bdt": z(d),
                   "A": z(d, n), "D": z(d), "gamma": z(d), "beta": z(d), "Wout": z(d, dim)}
         self.g = {k: z(*v.shape) for k, v in self.p.items()}
-        self._cache = {}
+        self._cache, self.saved = {}, None
 
     _buf = SwinBlock._buf
     set_parameters = SwinBlock.set_parameters
@@ -990,7 +991,9 @@ class StateSpaceBlock:
         """x [tokens x dim].  `states`: in front of the sequences (new_states or an earlier states_out), `states_out`: to take those
         behind them; `step`: a device counter that draws another dropout mask at each value (Engine.dropout_step)."""
         e, p, d, B_, T = self.eng, self.p, self.inner, self._buf, x.shape[0]
-        self.x, self.rows, self.step_counter, self.training = x, dict(offsets=offsets, sequences=sequences), step, training
+        E._expect("StateSpaceBlock.forward", self.dtype, ("x", x, (T, self.dim)))
+        self.saved = None                 # (nothing to go back from until this forward is complete)
+        self.x, self.rows, self.step_counter = x, dict(offsets=offsets, sequences=sequences), step
         before = states or {"conv": None, "h": None}
         after = states_out or {"conv": None, "h": None}
         self.before = before
@@ -999,17 +1002,23 @@ class StateSpaceBlock:
         self.uz, self.c, self.dbc, self.delta = self._mix(x, T, conv, B_)
         parts, pitches = self._parts(self.uz, self.dbc)
         saved = B_("saved", (e.selective_scan_saved(T, d, self.state, self.dtype),)) if training else False
-        self.y, _, self.saved = e.selective_scan_forward(
+        self.y, _, saved = e.selective_scan_forward(
             self.c, self.delta, p["A"], parts["B"], parts["C"], p["D"], parts["z"], p["bdt"], before["h"], groups=self.groups, **self.rows,
             out=B_("y", (T, d)), h_last=after["h"], save=saved, pitches=pitches)
         self.norm, self.out = self._project(x, self.y, T, training, step, B_)
+        self.saved = saved
         return self.out
 
     def backward(self, d_out: E.DeviceMatrix):
         """Gradients of the last forward's parameters into `g` (and of the states into d_states, where there were any); returns d_x."""
+        if self.saved is None:
+            raise _lib.PradError(_lib.ERR_INVALID, "StateSpaceBlock.backward: no training forward to go back from")
+        if d_out.shape != self.x.shape or d_out.dtype != self.dtype:
+            raise _lib.PradError(_lib.ERR_SHAPE, f"StateSpaceBlock.backward: d_out is {d_out.shape} of {d_out.dtype}, "
+                                                 f"the forward's x {self.x.shape} of {self.dtype}")
         e, p, g, d, T, B_ = self.eng, self.p, self.g, self.inner, d_out.shape[0], self._buf
         parts, pitches = self._parts(self.uz, self.dbc)
-        d_proj = e.dropout(d_out, self.p_drop if self.training else 0.0, self.seed, 0, step=self.step_counter, out=B_("d_proj", (T, self.dim)))
+        d_proj = e.dropout(d_out, self.p_drop, self.seed, 0, step=self.step_counter, out=B_("d_proj", (T, self.dim)))
         v, mean, rstd = self.norm
         d_v, _ = e.matmul_backward(v, p["Wout"], d_proj, dA=B_("d_v", (T, d)), dB=g["Wout"])
         d_y, _, _ = e.group_norm_backward(self.y, mean, rstd, d_v, self.norm_groups, p["gamma"], p["beta"],
@@ -1041,6 +1050,7 @@ class StateSpaceBlock:
     def step(self, x: E.DeviceMatrix, states):
         """One new token [sequences x dim] for each sequence; `states` are replaced.  What a forward keeps for its backward stays."""
         e, p, T = self.eng, self.p, x.shape[0]
+        E._expect("StateSpaceBlock.step", self.dtype, ("x", x, (T, self.dim)))
         B_ = lambda name, shape: self._buf("step " + name, shape)  # noqa: E731
         conv = lambda u, out: e.causal_conv_step(u, p["Wc"], states["conv"], p["bc"], out=out, ld_x=2 * self.inner)  # noqa: E731
         uz, c, dbc, delta = self._mix(x, T, conv, B_)

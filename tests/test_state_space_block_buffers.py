@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from parallelreverseautodiff_b200 import _lib
 from parallelreverseautodiff_b200.networks import StateSpaceBlock
 from recording_library import recording_engine
 
@@ -25,3 +26,34 @@ def test_single_tokens_use_buffers_of_their_own(sequences, width):
     assert not kept & (e.lib.touched() - parameters) and b.norm is norm
     b.backward(e.empty((9, 8), F))
     assert {b.uz.ptr, b.c.ptr, b.dbc.ptr, b.delta.ptr, b.y.ptr, b.saved.ptr, *(m.ptr for m in norm)} <= e.lib.touched() & kept
+
+
+def test_a_backward_that_no_forward_fits_is_refused_before_its_first_launch():
+    e, b, _ = _block()
+    x, d_out = e.empty((9, 8), F), e.empty((9, 8), F)
+    e.lib.taken()
+
+    def refused(call, status):
+        with pytest.raises(_lib.PradError) as err:
+            call()
+        assert err.value.status == status and not e.lib.taken()
+
+    refused(lambda: b.backward(d_out), _lib.ERR_INVALID)
+    for bad, status in ((e.empty((9, 7), F), _lib.ERR_SHAPE), (e.empty((9, 8), np.float64), _lib.ERR_INVALID)):
+        refused(lambda: b.forward(bad), status)
+        refused(lambda: b.step(bad, {}), status)
+    b.forward(x, sequences=3)
+    e.lib.taken()
+    for bad in ((10, 8), (8, 8), (8, 9)):
+        refused(lambda: b.backward(e.empty(bad, F)), _lib.ERR_SHAPE)
+    refused(lambda: b.backward(e.empty((9, 8), np.float64)), _lib.ERR_SHAPE)
+    b.backward(d_out)
+    # an answer that keeps nothing, and a forward that was refused half way
+    b.forward(x, sequences=3, training=False)
+    e.lib.taken()
+    refused(lambda: b.backward(d_out), _lib.ERR_INVALID)
+    b.forward(x, sequences=3)
+    with pytest.raises(_lib.PradError):
+        b.forward(x, sequences=3, states={"conv": None, "h": e.empty((2, 48), F)})
+    e.lib.taken()
+    refused(lambda: b.backward(d_out), _lib.ERR_INVALID)
