@@ -249,7 +249,8 @@ class Engine:
     def record(self, fn) -> "Sequence":
         """Runs `fn()` with the context recording (prad_capture_begin/end): its launches are not
         executed but kept as a sequence that `Sequence.launch()` replays in one submission.  Run
-        `fn()` once unrecorded first so that library scratch has its final size."""
+        `fn()` once unrecorded first so that library scratch has its final size.  The sequence keeps
+        what `fn` allocates and what it passes to `hold`; all else that it works on is the caller's to keep."""
         check(self.lib.prad_capture_begin(self.ctx))
         self._record_keep = keep = []
         self._deferred_free, self._deferred_packed = [], []
@@ -287,9 +288,13 @@ class Engine:
             n *= int(s)
         p = C.c_void_p()
         check(self.lib.prad_alloc(self.ctx, n * dtype.itemsize, C.byref(p)))
-        m = DeviceMatrix(self, p.value, shape, dtype)
+        return self.hold(DeviceMatrix(self, p.value, shape, dtype))     # (born inside a recording: lives as long as the sequence)
+
+    def hold(self, m):
+        """`m`, which lives as long as the sequence that is being recorded, if one is: for a buffer from before the recording
+        that its owner may replace behind it."""
         keep = getattr(self, "_record_keep", None)
-        if keep is not None:       # a buffer born inside a recording lives as long as the sequence
+        if keep is not None:
             keep.append(m)
         return m
 

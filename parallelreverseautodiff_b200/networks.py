@@ -743,12 +743,13 @@ class SwinBlock:
         self._cache = {}
 
     def _buf(self, name, shape):
-        """Device buffer reused across calls (no allocation in the steady state)."""
+        """Device buffer reused across calls (no allocation in the steady state).  A call of another shape replaces it: a recorded
+        sequence keeps the one that it was recorded with."""
         b = self._cache.get(name)
         if b is None or b.shape != tuple(shape):
             b = self.eng.empty(shape, self.dtype)
             self._cache[name] = b
-        return b
+        return self.eng.hold(b)
 
     def set_parameters(self, params):
         for k, v in params.items():
@@ -813,7 +814,7 @@ class SwinBlock:
         if p is None or (p.rows, p.cols) != (rows, cols):
             p = self.eng.packed(rows, cols, forms, 128, 128)
             self._cache["packed " + name] = p
-        return p
+        return self.eng.hold(p)
 
     def _weight(self, name, forward: bool):
         """This call's packed weight: by columns it multiplies activations, by rows it multiplies gradients."""
@@ -1017,6 +1018,7 @@ class StateSpaceBlock:
             raise _lib.PradError(_lib.ERR_SHAPE, f"StateSpaceBlock.backward: d_out is {d_out.shape} of {d_out.dtype}, "
                                                  f"the forward's x {self.x.shape} of {self.dtype}")
         e, p, g, d, T, B_ = self.eng, self.p, self.g, self.inner, d_out.shape[0], self._buf
+        e.hold((self.x, self.uz, self.c, self.dbc, self.delta, self.saved, self.y, self.norm, self.before, self.rows, self.step_counter))
         parts, pitches = self._parts(self.uz, self.dbc)
         d_proj = e.dropout(d_out, self.p_drop, self.seed, 0, step=self.step_counter, out=B_("d_proj", (T, self.dim)))
         v, mean, rstd = self.norm

@@ -22,3 +22,31 @@ def test_single_tokens_between_forward_and_backward(engine, sequences):
         got.append({"x": b.backward(d_out).numpy(), **{k: v.numpy() for k, v in b.g.items()}})
     for k in got[0]:
         assert np.array_equal(got[0][k], got[1][k]), k
+
+
+def test_a_recorded_step_after_calls_of_other_sizes(engine):
+    """Replayed behind them, with new allocations where the block's old buffers would be, it gives what it gave before them."""
+    e, f, r = engine, np.float32, np.random.default_rng(6)
+    b, _ = _block(e, f, r)
+    x, d_out = (e.upload(r.standard_normal((9, b.dim)).astype(f)) for _ in range(2))
+
+    def train():
+        b.forward(x, sequences=3)
+        b.backward(d_out)
+
+    train()
+    sequence = e.record(train)
+    out, d_x = b.out, b.d_x
+    sequence.launch()
+    want = [m.numpy() for m in (out, d_x, *b.g.values())]
+    for n in (6, 12):
+        more = e.upload(r.standard_normal((n, b.dim)).astype(f))
+        b.forward(more, sequences=1)
+        b.step(more, b.new_states(n))
+        b.backward(more)
+    others = [e.upload(np.full(s, 7, f)) for s in ((9, b.inner), (9, 2 * b.inner), (9, b.dim), (9, b.columns), (9, b.norm_groups)) for _ in range(4)]
+    sequence.launch()
+    for m, w in zip((out, d_x, *b.g.values()), want):
+        assert np.array_equal(m.numpy(), w)
+    assert all((m.numpy() == 7).all() for m in others)
+    sequence.close()

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from parallelreverseautodiff_b200 import _lib
-from parallelreverseautodiff_b200.networks import StateSpaceBlock
+from parallelreverseautodiff_b200.networks import StateSpaceBlock, SwinBlock
 from recording_library import recording_engine
 
 F = np.dtype(np.float32)
@@ -57,3 +57,46 @@ def test_a_backward_that_no_forward_fits_is_refused_before_its_first_launch():
         b.forward(x, sequences=3, states={"conv": None, "h": e.empty((2, 48), F)})
     e.lib.taken()
     refused(lambda: b.backward(d_out), _lib.ERR_INVALID)
+
+
+@pytest.mark.parametrize("recorded", ["step", "backward"])
+def test_a_recorded_step_keeps_its_buffers(recorded):
+    """Calls of other sizes behind a recording: what it was recorded with stays allocated until the sequence is closed."""
+    e, b, parameters = _block()
+    x, d_out, states = e.empty((9, 8), F), e.empty((9, 8), F), b.new_states(3)
+
+    def train():
+        b.forward(x, sequences=3, states=states)
+        b.backward(d_out)
+
+    train()
+    e.lib.taken()
+    sequence = e.record(train if recorded == "step" else lambda: b.backward(d_out))
+    used = e.lib.touched()
+    assert len(used - parameters) > 15
+    for n in (12, 5):
+        b.forward(e.empty((n, 8), F), sequences=1)
+        b.step(e.empty((n, 8), F), b.new_states(n))
+        b.backward(e.empty((n, 8), F))
+    assert used <= set(e.lib.live)
+    sequence.close()
+    assert not used <= set(e.lib.live)
+
+
+def test_a_recorded_attention_block_keeps_its_buffers():
+    e = recording_engine()
+    b = SwinBlock(e, F, 32, 2, 4)
+    x, d_out = e.empty((8, 32), F), e.empty((8, 32), F)
+
+    def train():
+        b.forward(x)
+        b.backward(d_out)
+
+    train()
+    e.lib.taken()
+    sequence = e.record(train)
+    used = e.lib.touched()
+    b.forward(e.empty((12, 32), F))
+    b.backward(e.empty((12, 32), F))
+    assert used <= set(e.lib.live)
+    sequence.close()
