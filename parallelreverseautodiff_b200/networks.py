@@ -970,6 +970,13 @@ class StateSpaceBlock:
                  "B": dbc.view((T, n), self.rank), "C": dbc.view((T, n), self.rank + n)}
         return parts, {"z": 2 * d, "B": self.columns, "C": self.columns}
 
+    def _clear(self, *buffers):
+        """The scan and the convolution leave rows of no sequence as they were, and products over all rows read them: zero, not what
+        an earlier batch had there.  Only the device knows whether there are any."""
+        if self.rows["offsets"] is not None:
+            for m in buffers:
+                self.eng.zero_(m)
+
     def _mix(self, x, T, convolve, B_):
         """x -> uz, c, dbc, delta; `convolve` is the convolution of a prompt or of single tokens, `B_` gives the buffers."""
         e, p, d = self.eng, self.p, self.inner
@@ -989,8 +996,10 @@ class StateSpaceBlock:
         return norm, e.dropout(proj, self.p_drop if drop else 0.0, self.seed, 0, residual=x, step=step, out=B_("out", (T, self.dim)))
 
     def forward(self, x: E.DeviceMatrix, offsets=None, sequences=1, states=None, states_out=None, training=True, step=None):
-        """x [tokens x dim].  `states`: in front of the sequences (new_states or an earlier states_out), `states_out`: to take those
-        behind them; `step`: a device counter that draws another dropout mask at each value (Engine.dropout_step)."""
+        """x [tokens x dim].  Rows that `offsets` gives to no sequence (padding) pass through the layer as tokens whose y is zero, so with
+        a d_out of zero there they add nothing to a gradient; x and d_out have to be finite in them.  `states`: in front of the
+        sequences (new_states or an earlier states_out), `states_out`: to take those behind them; `step`: a device counter that
+        draws another dropout mask at each value (Engine.dropout_step)."""
         e, p, d, B_, T = self.eng, self.p, self.inner, self._buf, x.shape[0]
         E._expect("StateSpaceBlock.forward", self.dtype, ("x", x, (T, self.dim)))
         self.saved = None                 # (nothing to go back from until this forward is complete)
@@ -998,6 +1007,7 @@ class StateSpaceBlock:
         before = states or {"conv": None, "h": None}
         after = states_out or {"conv": None, "h": None}
         self.before = before
+        self._clear(B_("c", (T, d)), B_("y", (T, d)))
         conv = lambda u, out: e.causal_conv_forward(u, p["Wc"], p["bc"], before["conv"], **self.rows, out=out,  # noqa: E731
                                                     state_out=after["conv"], ld_x=2 * d)[0]
         self.uz, self.c, self.dbc, self.delta = self._mix(x, T, conv, B_)
@@ -1028,6 +1038,7 @@ class StateSpaceBlock:
         d_uz, d_dbc = B_("d_uz", (T, 2 * d)), B_("d_dbc", (T, self.columns))
         d_parts, _ = self._parts(d_uz, d_dbc)
         d_c, d_delta = B_("d_c", (T, d)), B_("d_delta", (T, d))
+        self._clear(d_uz, d_dbc, d_delta)
         out = {"u": d_c, "delta": d_delta, "z": d_parts["z"], "A": g["A"], "B": d_parts["B"], "C": d_parts["C"], "D": g["D"],
                "delta_bias": g["bdt"]}
         self.d_states = {}

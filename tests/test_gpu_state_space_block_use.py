@@ -50,3 +50,33 @@ def test_a_recorded_step_after_calls_of_other_sizes(engine):
         assert np.array_equal(m.numpy(), w)
     assert all((m.numpy() == 7).all() for m in others)
     sequence.close()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_padded_batches(engine, dtype):
+    """Rows in front of the first sequence and behind the last: out and every gradient are those of the batch without them, whatever a
+    batch before it left in the buffers.  The sums are the same, over some zeros more and in other tiles: a result is a sum of fewer
+    than 100 products that have passed at most 60 roundings each, and the results here are sums of values of about their size."""
+    e, r = engine, np.random.default_rng(15)
+    b, p = _block(e, dtype, r)
+    lengths, front, back = [12, 0, 7], 3, 5
+    T = sum(lengths)
+    rows = T + front + back
+    full, padded = (e._upload_raw(np.array(m, np.int32)) for m in ([0, 9, 9, rows], np.cumsum([front] + lengths)))
+    x, d_out = r.standard_normal((rows, b.dim)).astype(dtype), r.standard_normal((rows, b.dim)).astype(dtype)
+    d_out[:front] = d_out[front + T:] = 0
+    up = lambda a: e.upload(np.ascontiguousarray(a))  # noqa: E731
+
+    def run(x, d_out, offsets):
+        out = b.forward(up(x), offsets, 3)
+        return {"out": out.numpy(), "x": b.backward(up(d_out)).numpy(), **{k: v.numpy() for k, v in b.g.items()}}
+
+    inside = slice(front, front + T)
+    want = run(x[inside], d_out[inside], e.sequence_offsets(lengths))
+    run(x * 3, d_out + 1, full)          # every row of every buffer holds something
+    for _ in range(2):
+        got = run(x, d_out, padded)
+        assert (got["x"][:front] == 0).all() and (got["x"][front + T:] == 0).all()
+        got["out"], got["x"] = got["out"][inside], got["x"][inside]
+        for k in want:
+            assert np.abs(got[k] - want[k]).max() <= 6000 * np.finfo(dtype).eps / 2 * (1 + np.abs(want[k]).max()), k
