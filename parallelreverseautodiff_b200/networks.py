@@ -988,12 +988,12 @@ class StateSpaceBlock:
         return uz, c, dbc, delta
 
     def _project(self, x, y, T, drop, step, B_):
-        """y -> v, mean, rstd = groupnorm(y) and x + dropout(v Wout)."""
+        """y -> v, mean, rstd = groupnorm(y), and x + dropout(v Wout) in a matrix of its own."""
         e, p, d = self.eng, self.p, self.inner
         norm = e.group_norm_forward(y, self.norm_groups, p["gamma"], p["beta"], out=(B_("v", (T, d)), B_("mean", (T, self.norm_groups)),
                                                                                   B_("rstd", (T, self.norm_groups))))
         proj = e.matmul_forward(norm[0], p["Wout"], Y=B_("proj", (T, self.dim)))
-        return norm, e.dropout(proj, self.p_drop if drop else 0.0, self.seed, 0, residual=x, step=step, out=B_("out", (T, self.dim)))
+        return norm, e.dropout(proj, self.p_drop if drop else 0.0, self.seed, 0, residual=x, step=step)
 
     def forward(self, x: E.DeviceMatrix, offsets=None, sequences=1, states=None, states_out=None, training=True, step=None):
         """x [tokens x dim].  Rows that `offsets` gives to no sequence (padding) pass through the layer as tokens whose y is zero, so with
@@ -1021,7 +1021,8 @@ class StateSpaceBlock:
         return self.out
 
     def backward(self, d_out: E.DeviceMatrix):
-        """Gradients of the last forward's parameters into `g` (and of the states into d_states, where there were any); returns d_x."""
+        """Gradients of the last forward's parameters into `g` (and of the states into d_states, where there were any); returns d_x,
+        which like d_states is the block's and holds until the next backward."""
         if self.saved is None:
             raise _lib.PradError(_lib.ERR_INVALID, "StateSpaceBlock.backward: no training forward to go back from")
         if d_out.shape != self.x.shape or d_out.dtype != self.dtype:

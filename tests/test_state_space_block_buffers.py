@@ -100,3 +100,11 @@ def test_a_recorded_attention_block_keeps_its_buffers():
     b.backward(e.empty((12, 32), F))
     assert used <= set(e.lib.live)
     sequence.close()
+
+
+def test_results_are_the_callers_to_keep():
+    """Several prompts and tokens in a row: none of the outputs is written again."""
+    e, b, _ = _block()
+    x, states = e.empty((9, 8), F), b.new_states(9)
+    results = [*(b.forward(x, sequences=3, training=t) for t in (True, False)), *(b.step(x, states) for _ in range(3))]
+    assert len({m.ptr for m in results}) == 5
