@@ -69,7 +69,7 @@ class DeviceMatrix:
     def __init__(self, engine: "Engine", ptr: int, shape: Sequence[int], dtype, owned=True):
         self.engine = engine
         self.ptr = ptr
-        self.shape = tuple(shape) if isinstance(shape, tuple) else tuple(map(int, shape))
+        self.shape = tuple(map(int, shape))      # (numpy's integers would overflow in `size`)
         self.dtype = dtype if isinstance(dtype, np.dtype) else np.dtype(dtype)
         self._owned = owned
 
