@@ -58,20 +58,30 @@ def _expect(who: str, dtype, *sized) -> None:
             raise _lib.PradError(_lib.ERR_SHAPE, f"{who}: {name} has {m.size} values, not {n}")
 
 
+def _expect_room(who: str, *pitched) -> None:
+    """(name, matrix or None, shape, pitch or 0) each: rows that a pitch puts beyond the end of the matrix' allocation, where that is
+    known (it is not for memory of others), are refused."""
+    for name, m, (rows, cols), ld in pitched:
+        if m is not None and ld and rows and m._room is not None and (rows - 1) * ld + cols > m._room:
+            raise _lib.PradError(_lib.ERR_SHAPE, f"{who}: {rows} rows of {cols} values with a pitch of {ld} do not fit {name}, "
+                                                 f"which has {m._room} values from its first on")
+
+
 _I32, _U64 = np.dtype(np.int32), np.dtype(np.uint64)
 
 
 class DeviceMatrix:
     """A dense row-major device buffer: Matrix (2-D) or DeepMatrix (3-D, depth first)."""
 
-    __slots__ = ("engine", "ptr", "shape", "dtype", "_owned")
+    __slots__ = ("engine", "ptr", "shape", "dtype", "_owned", "_room")
 
-    def __init__(self, engine: "Engine", ptr: int, shape: Sequence[int], dtype, owned=True):
+    def __init__(self, engine: "Engine", ptr: int, shape: Sequence[int], dtype, owned=True, room: Optional[int] = None):
         self.engine = engine
         self.ptr = ptr
         self.shape = tuple(map(int, shape))      # (numpy's integers would overflow in `size`)
         self.dtype = dtype if isinstance(dtype, np.dtype) else np.dtype(dtype)
         self._owned = owned
+        self._room = room          # values from the first one to the end of the allocation, where that is known
 
     @property
     def size(self) -> int:
@@ -101,8 +111,8 @@ class DeviceMatrix:
 
     def view(self, shape: Sequence[int], offset_elems: int = 0) -> "DeviceMatrix":
         """A non-owning alias of (part of) this buffer with another shape."""
-        return DeviceMatrix(self.engine, self.ptr + offset_elems * self.dtype.itemsize, shape,
-                            self.dtype, owned=False)
+        return DeviceMatrix(self.engine, self.ptr + offset_elems * self.dtype.itemsize, shape, self.dtype, owned=False,
+                            room=None if self._room is None else self._room - offset_elems)
 
     def slice(self, d: int) -> "DeviceMatrix":
         """Slice d of a DeepMatrix as a Matrix (alias)."""
@@ -288,7 +298,7 @@ class Engine:
             n *= int(s)
         p = C.c_void_p()
         check(self.lib.prad_alloc(self.ctx, n * dtype.itemsize, C.byref(p)))
-        return self.hold(DeviceMatrix(self, p.value, shape, dtype))     # (born inside a recording: lives as long as the sequence)
+        return self.hold(DeviceMatrix(self, p.value, shape, dtype, room=n))     # (born inside a recording: lives as long as the sequence)
 
     def hold(self, m):
         """`m`, which lives as long as the sequence that is being recorded, if one is: for a buffer from before the recording
@@ -866,7 +876,7 @@ class Engine:
         """Device copy of an array of any type: row numbers and counters, which are no matrices of the library."""
         p = C.c_void_p()
         check(self.lib.prad_alloc(self.ctx, a.nbytes, C.byref(p)))
-        m = DeviceMatrix(self, p.value, a.shape, a.dtype)
+        m = DeviceMatrix(self, p.value, a.shape, a.dtype, room=a.size)
         check(self.lib.prad_upload(self.ctx, m.ptr, a.ctypes.data, a.nbytes))
         return m
 
@@ -927,8 +937,10 @@ class Engine:
             state_out = self.empty((sequences, (width - 1) * dim), x.dtype)
         states = (sequences, (width - 1) * dim)
         _expect("causal_conv_forward", x.dtype, ("w", w, (dim, width)), ("bias", bias, (dim,)), ("state", state, states),
-                ("state_out", state_out, states), ("out", None if ld_y else out, x.shape))
+                ("state_out", state_out, states), ("out", out, out.shape if ld_y else x.shape))
         _expect("causal_conv_forward", _I32, ("offsets", offsets, (sequences + 1,)))
+        if ld_x or ld_y:
+            _expect_room("causal_conv_forward", ("x", x, x.shape, ld_x), ("out", out, x.shape, ld_y))
         check(self.lib.prad_causal_conv_forward(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), self._p(state),
                                                 self._p(offsets), out.ptr, ld_y, self._p(state_out), sequences, tokens, dim, width,
                                                 int(swish)))
@@ -945,6 +957,8 @@ class Engine:
                 ("dx", out["x"], x.shape), ("dw", out.get("w"), (dim, width)), ("dbias", out.get("bias"), each),
                 ("dstate", out.get("state"), states))
         _expect("causal_conv_backward", _I32, ("offsets", offsets, (sequences + 1,)))
+        if ld_x or ld_dy or ld_dx:
+            _expect_room("causal_conv_backward", ("x", x, x.shape, ld_x), ("dy", dy, x.shape, ld_dy), ("dx", out["x"], x.shape, ld_dx))
         check(self.lib.prad_causal_conv_backward(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), self._p(state),
                                                  self._p(offsets), dy.ptr, ld_dy, out["x"].ptr, ld_dx, self._p(out.get("w")),
                                                  self._p(out.get("bias")), self._p(out.get("state")), sequences, tokens, dim, width,
@@ -957,7 +971,9 @@ class Engine:
         out = out or self.empty((batch, dim), x.dtype)
         states = (batch, (width - 1) * dim)
         _expect("causal_conv_step", x.dtype, ("w", w, (dim, width)), ("bias", bias, (dim,)), ("state", state if width > 1 else None, states),
-                ("state_out", state_out if width > 1 else None, states), ("out", None if ld_y else out, x.shape))
+                ("state_out", state_out if width > 1 else None, states), ("out", out, out.shape if ld_y else x.shape))
+        if ld_x or ld_y:
+            _expect_room("causal_conv_step", ("x", x, x.shape, ld_x), ("out", out, x.shape, ld_y))
         check(self.lib.prad_causal_conv_step(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), state.ptr, out.ptr, ld_y,
                                              state.ptr if state_out is None else state_out.ptr, batch, dim, width, int(swish)))
         return out
@@ -972,15 +988,17 @@ class Engine:
         _expect("selective_scan", _I32, ("offsets", offsets, (sequences + 1,)))
         s = _lib.Scan(u.shape[0], sequences, dim, state, groups, int(delta_softplus), *[None if m is None else m.ptr for m in (
             offsets, u, delta, z, A, B, C_, D, delta_bias, h0)])
-        Engine._set_pitches(s, "ld_", pitches)
+        if pitches:
+            Engine._set_pitches(s, "ld_", pitches, dict(u=u, delta=delta, z=z, B=B, C=C_), tokens, rows)
         return s
 
     @staticmethod
-    def _set_pitches(struct, prefix, pitches):
-        for k, ld in (pitches or {}).items():
+    def _set_pitches(struct, prefix, pitches, matrices, tokens, rows):
+        for k, ld in pitches.items():
             if k not in ("u", "delta", "z", "B", "C"):
                 raise _lib.PradError(_lib.ERR_INVALID, f"selective_scan: {k} has no pitch")
             setattr(struct, prefix + k, ld)
+            _expect_room("selective_scan", (prefix[3:] + k, matrices.get(k), rows if k in ("B", "C") else tokens, ld))
 
     def selective_scan_saved(self, tokens, dim, state, dtype) -> int:
         """How many values `save` of selective_scan_forward needs."""
@@ -1006,7 +1024,10 @@ class Engine:
             elif save.nbytes < n.value:
                 raise _lib.PradError(_lib.ERR_SHAPE, f"selective_scan_forward: save has {save.nbytes} bytes, not {n.value}")
         save = save or None
-        _expect("selective_scan_forward", u.dtype, ("h_last", h_last, (sequences, s.dim * s.state)), ("out", None if ld_y else out, u.shape))
+        _expect("selective_scan_forward", u.dtype, ("h_last", h_last, (sequences, s.dim * s.state)),
+                ("out", out, out.shape if ld_y else u.shape))
+        if ld_y:
+            _expect_room("selective_scan_forward", ("out", out, u.shape, ld_y))
         check(self.lib.prad_selective_scan_forward(self.ctx, dt, ref, out.ptr, ld_y, self._p(h_last), self._p(save)))
         return out, h_last, save
 
@@ -1025,7 +1046,10 @@ class Engine:
         if saved is not None and saved.nbytes < n:
             raise _lib.PradError(_lib.ERR_SHAPE, f"selective_scan_backward: saved has {saved.nbytes} bytes, not {n}")
         g = _lib.ScanGradients(*[self._p(out.get(k)) for k in ("u", "delta", "z", "A", "B", "C", "D", "delta_bias", "h0")])
-        self._set_pitches(g, "ld_d", gradient_pitches)
+        if gradient_pitches:
+            self._set_pitches(g, "ld_d", gradient_pitches, out, u.shape, B.shape)
+        if ld_dy:
+            _expect_room("selective_scan_backward", ("dy", dy, u.shape, ld_dy))
         check(self.lib.prad_selective_scan_backward(self.ctx, dtype_code(u.dtype), _byref(s), self._p(saved), dy.ptr, ld_dy, _byref(g)))
         return out
 
@@ -1034,7 +1058,9 @@ class Engine:
         """One new token for each sequence; the states `h` are replaced, or go to `h_out`.  Returns y."""
         s = self._scan(u, delta, A, B, C, D, z, delta_bias, h, None, u.shape[0], groups, delta_softplus, pitches)
         out = out or self.empty(u.shape, u.dtype)
-        _expect("selective_scan_step", u.dtype, ("h_out", h_out, h.shape), ("out", None if ld_y else out, u.shape))
+        _expect("selective_scan_step", u.dtype, ("h_out", h_out, h.shape), ("out", out, out.shape if ld_y else u.shape))
+        if ld_y:
+            _expect_room("selective_scan_step", ("out", out, u.shape, ld_y))
         check(self.lib.prad_selective_scan_step(self.ctx, dtype_code(u.dtype), _byref(s), out.ptr, ld_y, (h_out or h).ptr))
         return out
 
