@@ -966,7 +966,7 @@ class Engine:
         return out
 
     def causal_conv_step(self, x, w, state, bias=None, swish=True, out=None, state_out=None, ld_x=0, ld_y=0):
-        """One new row of each sequence; the state is replaced, or goes to `state_out`.  Returns y."""
+        """One new row of each sequence; the state (None where width 1 has none) is replaced, or goes to `state_out`.  Returns y."""
         (batch, dim), width = x.shape, w.shape[1]
         out = out or self.empty((batch, dim), x.dtype)
         states = (batch, (width - 1) * dim)
@@ -974,8 +974,8 @@ class Engine:
                 ("state_out", state_out if width > 1 else None, states), ("out", out, out.shape if ld_y else x.shape))
         if ld_x or ld_y:
             _expect_room("causal_conv_step", ("x", x, x.shape, ld_x), ("out", out, x.shape, ld_y))
-        check(self.lib.prad_causal_conv_step(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), state.ptr, out.ptr, ld_y,
-                                             state.ptr if state_out is None else state_out.ptr, batch, dim, width, int(swish)))
+        check(self.lib.prad_causal_conv_step(self.ctx, dtype_code(x.dtype), x.ptr, ld_x, w.ptr, self._p(bias), self._p(state), out.ptr,
+                                             ld_y, self._p(state if state_out is None else state_out), batch, dim, width, int(swish)))
         return out
 
     @staticmethod

@@ -87,3 +87,10 @@ def test_inputs_with_a_pitch_have_room():
         _refused(e, call, _lib.ERR_SHAPE)
     nothing = m(0, D)
     e.causal_conv_forward(nothing, w, sequences=0, ld_x=2 * D, ld_y=2 * D)
+
+
+def test_a_single_token_of_width_one_needs_no_state():
+    e = recording_engine()
+    x, w = e.empty((T, D), F), e.empty((D, 1), F)
+    y = e.causal_conv_step(x, w, None)
+    assert e.lib.taken()[-1] == ("prad_causal_conv_step", (1, E.F32, x.ptr, 0, w.ptr, None, None, y.ptr, 0, None, T, D, 1, 1))

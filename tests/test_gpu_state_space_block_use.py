@@ -80,3 +80,10 @@ def test_padded_batches(engine, dtype):
         got["out"], got["x"] = got["out"][inside], got["x"][inside]
         for k in want:
             assert np.abs(got[k] - want[k]).max() <= 6000 * np.finfo(dtype).eps / 2 * (1 + np.abs(want[k]).max()), k
+
+
+def test_a_single_token_of_width_one(engine):
+    e, r = engine, np.random.default_rng(2)
+    x, w = r.standard_normal((5, 12)), r.standard_normal((12, 1))
+    y = e.causal_conv_step(e.upload(x), e.upload(w), None, swish=False).numpy()
+    assert np.array_equal(y, x * w[:, 0])
