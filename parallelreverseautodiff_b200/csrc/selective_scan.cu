@@ -1400,25 +1400,29 @@ template <auto Kernel> static int64_t resident(prad_ctx* ctx, int smem) {
 
 // How the token axis is cut: by sequences where they are of equal length and fill at least half of the device (the edges' pass is
 // about half of the work again), else into spans of whole tiles, as many as the device holds at a time: one CTA more takes as long
-// as twice as many.
+// as twice as many.  Each span costs a CTA's beginning and end and leaves sums of its own, dim x state values, which is more than
+// short sequences bring: where there are many of those, a span has as many as give every place of the device two CTAs (backward,
+// 1024 floats with 16 states: 16384 sequences of one token 772 us, 791 with one CTA a place, 813 with eight and 6190 with a span
+// each; 1024 of 16 tokens 471, 472, 492 and 596 us).
 template <typename T> static void cut(Args<T>& a, int64_t across, int64_t full) {
-  if (!a.rows.offsets && a.rows.count > 0 && a.rows.count <= 65535 && (a.rows.count * across >= full / 2 || a.rows.each <= 2 * span_unit<T>())) {
-    a.span = a.rows.each > 0 ? a.rows.each : 1;
-    a.spans = a.rows.count;
+  constexpr int unit = span_unit<T>();
+  const int64_t count = a.rows.count, each = a.rows.each;
+  const auto at_most = [&](int64_t spans) { return spans < 1 ? 1 : spans > 65535 ? 65535 : spans; };
+  const bool brief = each <= 2 * unit;
+  if (!a.rows.offsets && each > 0 && (brief || (count <= 65535 && count * across >= full / 2))) {
+    const int64_t together = brief && count * across > 8 * full ? ceil_div(count, at_most(2 * full / across)) : 1;
+    a.span = together * each;
+    a.spans = (int)ceil_div(count, together);
     return;
   }
-  int64_t spans = full / across;
-  if (spans < 1) spans = 1;
-  if (spans > 65535) spans = 65535;
-  constexpr int unit = span_unit<T>();
-  int64_t span = ceil_div(ceil_div(a.rows.tokens, spans), unit) * unit;
+  int64_t span = ceil_div(ceil_div(a.rows.tokens, at_most(full / across)), unit) * unit;
   if (span < 2 * unit) span = 2 * unit;
   a.span = span;
   a.spans = (int)ceil_div(a.rows.tokens, span);
   if (a.spans < 1) a.spans = 1;
 }
 // whether a span may begin inside a sequence
-template <typename T> static bool joined(const Args<T>& a) { return a.spans > 1 && (a.rows.offsets || a.span != a.rows.each); }
+template <typename T> static bool joined(const Args<T>& a) { return a.spans > 1 && (a.rows.offsets || a.span % a.rows.each != 0); }
 
 template <typename T> struct Carve {
   char* at;
