@@ -51,6 +51,7 @@ template <typename T> struct Args {
   int spans, dim, state, groups, per, blocks;   // per: channels of a group, in `blocks` CTAs
   int softplus;
   int wide, wide_B, wide_C, wide_h;     // the token matrices, B, C and the matrices of states: 16 bytes at a time
+  int block0;                   // backward: the first of a group's CTAs in this launch
   int64_t ld_u, ld_delta, ld_z, ld_B, ld_C, ld_y, ld_dy, ld_du, ld_ddelta, ld_dz, ld_dB, ld_dC;
   const T *u, *delta, *z, *A, *B, *C, *D, *bias, *h0, *dy;
   T *y, *h_last, *saved;
@@ -843,7 +844,7 @@ backward_kernel(const Args<T> a) {
   extern __shared__ __align__(16) unsigned char raw[];
   typename K::Shared& m = *reinterpret_cast<typename K::Shared*>(raw);
   // channels of the CTA: CH of a group; of a thread: ch[0], ch[0] + HALF
-  const int q = blockIdx.x / a.blocks, chan0 = blockIdx.x % a.blocks * CH, c0 = q * a.per + chan0;
+  const int q = blockIdx.x / a.blocks, chan0 = (a.block0 + (int)(blockIdx.x % a.blocks)) * CH, c0 = q * a.per + chan0;
   const int channels = a.per - chan0 < CH ? a.per - chan0 : CH;
   const int wl = threadIdx.x & 31, warp = threadIdx.x >> 5, lane = Lanes<L>::state(wl), n0 = lane * S;
   const int ch0 = warp * (32 / L) + Lanes<L>::channel(wl);
@@ -1177,7 +1178,7 @@ backward_kernel(const Args<T> a) {
         __syncthreads();
         // the warps' sums, in the order of the warps
         constexpr int WIDE = 16 / sizeof(T), FOURS = 2 * N / WIDE;
-        if (a.blocks > 1 && a.state == N) {     // whole rows of the partial sums, 16 bytes at a time
+        if (a.part_BC && a.state == N) {     // whole rows of the partial sums, 16 bytes at a time
           T* to0 = a.part_BC + ((blockIdx.x % a.blocks * a.rows.tokens + tile0 + f) * a.groups + q) * 2 * N;
           for (int i = threadIdx.x; i < FT * FOURS; i += THREADS) {
             const int t = i / FOURS, n = i % FOURS * WIDE;
@@ -1200,7 +1201,7 @@ backward_kernel(const Args<T> a) {
             if (state >= a.state) continue;
             T* to0 = n < N ? a.dB + q * a.state + state : a.dC + q * a.state + state;
             int64_t ld = n < N ? a.ld_dB : a.ld_dC;
-            if (a.blocks > 1) {
+            if (a.part_BC) {
               to0 = a.part_BC + ((int64_t)(blockIdx.x % a.blocks) * a.rows.tokens * a.groups + q) * 2 * a.state + (n < N ? 0 : a.state) + state;
               ld = (int64_t)a.groups * 2 * a.state;
             }
@@ -1298,7 +1299,7 @@ template <typename T> __device__ __forceinline__ void span_total(const Args<T>& 
   for (int p = 0; p < a.spans; ++p) sum += (double)from[p * each + i];
   to[i] = (T)sum;
 }
-// Pack i of V values of dB and dC: the sum of the CTAs of a group.
+// Pack i of V values of dB and dC: the sum of the CTAs of a group, added to that of the launches before this one.
 template <typename T, int V> __device__ __forceinline__ void row_total(const Args<T>& a, int64_t i) {
   const int64_t lo = a.rows.begin(), hi = a.rows.finish(), each = (int64_t)a.groups * 2 * a.state;
   i = lo * each + i * V;
@@ -1316,7 +1317,7 @@ template <typename T, int V> __device__ __forceinline__ void row_total(const Arg
   }
   T* to = n < a.state ? a.dB + row * a.ld_dB + q * a.state + n : a.dC + row * a.ld_dC + q * a.state + n - a.state;
 #pragma unroll
-  for (int j = 0; j < V; ++j) to[j] = sum[j];
+  for (int j = 0; j < V; ++j) to[j] = a.block0 ? to[j] + sum[j] : sum[j];
 }
 // the CTAs below `span_blocks` take the spans' sums, the others the rows', 16 bytes at a time where states come in such packs
 template <typename T>
@@ -1433,7 +1434,8 @@ template <typename T> struct Carve {
     return p;
   }
 };
-template <typename T> static size_t carve(Args<T>& a, bool backward, void* ws) {
+// `rows`: CTAs whose sums of dB and dC there is room for
+template <typename T> static size_t carve(Args<T>& a, bool backward, int rows, void* ws) {
   Carve<T> c{(char*)ws};
   const int64_t states = (int64_t)a.dim * a.state;
   if (joined(a)) {
@@ -1445,11 +1447,12 @@ template <typename T> static size_t carve(Args<T>& a, bool backward, void* ws) {
     a.part_A = c.template take<T>(a.spans * states);
     a.part_D = c.template take<T>((int64_t)a.spans * a.dim);
     a.part_bias = c.template take<T>((int64_t)a.spans * a.dim);
-    if (a.blocks > 1) a.part_BC = c.template take<T>((int64_t)a.blocks * a.rows.tokens * a.groups * 2 * a.state);
+    if (rows) a.part_BC = c.template take<T>((int64_t)rows * a.rows.tokens * a.groups * 2 * a.state);
   }
   return c.used;
 }
 
+constexpr int64_t ROWS_ROOM = 256 << 20;
 // FL lanes of FS states a channel in the forward passes, L of S backward and for single tokens
 template <typename T, int L, int S, int FL, int FS> static prad_status launch(prad_ctx* ctx, Args<T> a, Pass pass) {
   using Main = Backward<T, L, S>;
@@ -1457,6 +1460,17 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   // the edges' pass has THREADS / L channels a CTA, the main backward pass CC times as many
   const int edge_blocks = (int)ceil_div(a.per, THREADS / L);
   a.blocks = backward ? (int)ceil_div(a.per, Main::CH) : pass == Pass::Forward ? (int)ceil_div(a.per, THREADS / FL) : edge_blocks;
+  // Backward each of a group's CTAs leaves sums of dB and dC over its channels, Main::CH, for the last launch to add up: 2 state / CH
+  // token matrices in all, half a one with 16 float states and 32 with 128, where CH is 8.  Beyond 256 MB and beyond one token matrix
+  // the group's CTAs come in several launches, whose sums go to the same place, on spans that fill the device again (16384 tokens with
+  // 128 states: 2048 floats 15.5 ms with 0.4 GB of scratch, 16.6 ms with 5.4 GB in one launch; 1024 doubles 27.8 and 26.5 ms).
+  const int all_blocks = a.blocks;
+  if (backward) {
+    const int64_t each = a.rows.tokens * a.groups * 2 * a.state * (int64_t)sizeof(T), matrix = a.rows.tokens * a.dim * (int64_t)sizeof(T);
+    const int64_t most = (matrix > ROWS_ROOM ? matrix : ROWS_ROOM) / each;
+    if (most < a.blocks) a.blocks = (int)ceil_div(a.blocks, ceil_div(a.blocks, most < 1 ? 1 : most));
+  }
+  const int rows = backward && all_blocks > 1 ? a.blocks : 0;
   const int64_t across = (int64_t)a.groups * a.blocks;
   PRAD_REQUIRE(across <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many channels");
   if (pass == Pass::Step) {
@@ -1485,9 +1499,9 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   if (!st) st = backward ? allow_smem<backward_edges_kernel<T, L, S>>(ctx, edge_bytes) : allow_smem<forward_kernel<T, FL, FS, true>>(ctx, bytes);
   if (st) return st;
   cut(a, across, backward ? resident<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : resident<forward_kernel<T, FL, FS, false>>(ctx, bytes));
-  st = ensure_workspace(ctx, carve(a, backward, nullptr));
+  st = ensure_workspace(ctx, carve(a, backward, rows, nullptr));
   if (st) return st;
-  carve(a, backward, ctx->ws);
+  carve(a, backward, rows, ctx->ws);
   const int64_t states = (int64_t)a.dim * a.state;
   const unsigned x = (unsigned)across;
   if (!backward) {
@@ -1504,7 +1518,7 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   // of the last launch: the spans' sums, and the rows of dB and dC in packs
   constexpr int V = 16 / (int)sizeof(T);
   const int64_t span_blocks = ceil_div(states + 2 * (int64_t)a.dim, THREADS);
-  const int64_t packs = a.blocks > 1 ? a.rows.tokens * a.groups * 2 * a.state / (a.state % V ? 1 : V) : 0;
+  const int64_t packs = rows ? a.rows.tokens * a.groups * 2 * a.state / (a.state % V ? 1 : V) : 0;
   PRAD_REQUIRE(span_blocks + ceil_div(packs, THREADS) <= 0x7fffffff, PRAD_ERR_UNSUPPORTED, "selective scan: too many rows of B and C");
   if (a.dh0) PRAD_CUDA(cudaMemsetAsync(a.dh0, 0, (size_t)a.rows.count * states * sizeof(T), ctx->stream));
   if (joined(a)) {
@@ -1515,10 +1529,14 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
     launch_chained(join_kernel<T, false>, (unsigned)ceil_div(states, JOINED), 32 * JOINED, 0, ctx->stream, a);
     PRAD_LAUNCHED(ctx);
   }
-  launch_chained(backward_kernel<T, L, S>, dim3(x, (unsigned)a.spans), THREADS, sizeof(Shared), ctx->stream, a);
-  PRAD_LAUNCHED(ctx);
-  launch_chained(totals_kernel<T>, (unsigned)(span_blocks + ceil_div(packs, THREADS)), THREADS, 0, ctx->stream, a, (int)span_blocks);
-  PRAD_LAUNCHED(ctx);
+  for (const int most = a.blocks; a.block0 < all_blocks; a.block0 += most) {
+    if (a.blocks > all_blocks - a.block0) a.blocks = all_blocks - a.block0;
+    const int64_t sums = a.block0 + a.blocks == all_blocks ? span_blocks : 0;
+    launch_chained(backward_kernel<T, L, S>, dim3((unsigned)(a.groups * a.blocks), (unsigned)a.spans), THREADS, sizeof(Shared), ctx->stream, a);
+    PRAD_LAUNCHED(ctx);
+    launch_chained(totals_kernel<T>, (unsigned)(sums + ceil_div(packs, THREADS)), THREADS, 0, ctx->stream, a, (int)sums);
+    PRAD_LAUNCHED(ctx);
+  }
   return PRAD_OK;
 }
 template <typename T> static prad_status pick(prad_ctx* ctx, Args<T> a, Pass pass) {
