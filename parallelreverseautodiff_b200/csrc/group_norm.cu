@@ -11,8 +11,10 @@
 // backward its second reading misses the L2; clusters of 16, or blocks of half the channels, took 14 and 17 us longer, and blocks that
 // stay in shared memory, so that fewer of them run at a time, 54 and 113 us).
 //
-// Means and variances are summed around a pivot out of the data (the average of the group's first values), so that a mean far
-// from zero takes nothing from the variance; sums go from float to double every few values.
+// Over several positions a thread sums the deviations of a few values at a time from one of them, the median of three, and joins them
+// with the others in double, around a pivot out of the data: neither a mean far from zero nor single values far from the others take
+// anything from the variance. The backward sums go from float to double every few values too; with one position per sample the variance is
+// of deviations from the mean that is already there.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -310,16 +312,18 @@ template <int N, typename T> __device__ __forceinline__ int64_t last_rows(const 
   return mine < 0 ? w.p0 - 1 : w.p0 + w.ty + mine / ((int64_t)N * w.rows) * N * w.rows;
 }
 
-// the average of four values of a group
+// the average of the middle two of four values of a group: what the joined sums are relative to
 template <typename T> __device__ __forceinline__ double pivot(const Args<T>& a, int64_t s, int g) {
   const T* x = a.x + s * a.positions * a.channels + (int64_t)g * a.per;
-  double sum = 0.0;
+  double v[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) sum += (double)x[(a.positions - 1) * k / 3 * a.channels + (a.per - 1) * k / 3];
-  return (double)(T)(sum * 0.25);
+  for (int k = 0; k < 4; ++k) v[k] = (double)x[(a.positions - 1) * k / 3 * a.channels + (a.per - 1) * k / 3];
+  const double lower = fmax(fmin(v[0], v[1]), fmin(v[2], v[3])), upper = fmin(fmax(v[0], v[1]), fmax(v[2], v[3]));
+  return (double)(T)(0.5 * lower + 0.5 * upper);
 }
 
-constexpr int RUN = 8;     // positions that are summed in T before they go into a double
+template <typename T> __device__ __forceinline__ T median(T a, T b, T c) { return max(min(a, b), min(max(a, b), c)); }
+constexpr int RUN = 8;     // positions whose deviations are summed in T before they go into a double
 
 // sums of x - pivot and of its square over the CTA's block, for each of its groups, to `out(group, s1, s2)`
 template <typename T, int V> struct SumsShared {
@@ -333,28 +337,32 @@ __device__ __forceinline__ void block_sums(const Args<T>& a, const Place<T>& w, 
   double s1 = 0.0, s2 = 0.0;
   if (w.ty < w.rows)
     for (int q = w.tx; q < w.packs; q += THREADS) {
-      const T k = m.piv[q * V / a.per];
+      const double k = (double)m.piv[q * V / a.per];
       const T* x = a.x + (w.s * a.positions) * a.channels + w.c0 + (int64_t)q * V;
       for (int64_t p = w.p0 + w.ty; p < w.p1; p += (int64_t)RUN * w.rows) {
-        T r1 = 0, r2 = 0;
         Pack<T, V> v[RUN];
+        int rows = 0;
 #pragma unroll
         for (int i = 0; i < RUN; ++i) {
-          const int64_t at = p + (int64_t)i * w.rows;
+          const bool live = i == 0 || p + (int64_t)i * w.rows < w.p1;
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[i].v[j] = k;
-          if (at < w.p1) v[i] = load<T, V>(x + at * a.channels);
+          for (int j = 0; j < V; ++j) v[i].v[j] = 0;
+          if (live) v[i] = load<T, V>(x + (p + (int64_t)i * w.rows) * a.channels);
+          rows += live;
         }
+        const T at = median(v[0].v[0], rows > 1 ? v[1].v[V / 2] : v[0].v[0], rows > 2 ? v[2].v[V - 1] : v[0].v[V - 1]);
+        T r1 = 0, r2 = 0;
 #pragma unroll
         for (int i = 0; i < RUN; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const T d = v[i].v[j] - k;
+            const T d = i < rows ? v[i].v[j] - at : (T)0;
             r1 += d;
             r2 += d * d;
           }
-        s1 += (double)r1;
-        s2 += (double)r2;
+        const double e = (double)at - k, all = (double)(rows * V) * e, rest = (double)r1;
+        s1 += all + rest;
+        s2 += (double)r2 + e * (all + 2.0 * rest);
       }
     }
   m.part[threadIdx.x][0] = s1;
