@@ -45,3 +45,17 @@ def test_single_values_far_from_all_others(engine, dtype, samples, positions, ch
     near(m.numpy(), mean, of_mean, f"far value, mean {dtype}")
     limit = 68 * step * np.abs(want) + (of_mean * rstd)[:, None, :, None] * (1 + 68 * step)
     near(y.numpy().reshape(x.shape), want, limit, f"far value, y {dtype}")
+
+
+def test_sums_over_many_samples(engine):
+    """One value per group, so many groups that each has one place on the device: 5000 equal gradients, whose sum in one float would be
+    off by more than 1000 half steps. At most 512 are added up before they go into a double: 512 half steps, and one of the result."""
+    e, f, samples, channels = engine, np.float32, 5000, 80000
+    if e.device_info()["free_bytes"] < 8 << 30:
+        pytest.skip("needs 5 GB of device memory")
+    c = f(1.518797)
+    assert abs(float(np.cumsum(np.full(samples, c, f), dtype=f)[-1]) / (samples * float(c)) - 1) > 1000 * 2.0 ** -24
+    zero, dy = e.zeros((samples, channels), f), e.upload(np.full((samples, channels), c, f))
+    _, _, dbeta = e.group_norm_backward(zero, zero, zero, dy, channels, out=(dy, e.empty((channels,), f), e.empty((channels,), f)))
+    want = np.full(channels, samples * float(c))
+    near(dbeta.numpy(), want, 513 * 2.0 ** -24 * want, "sums over many samples")
