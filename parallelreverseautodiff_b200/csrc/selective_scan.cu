@@ -70,9 +70,13 @@ template <typename T> struct Args {
 constexpr float LIFT = 2.2351741790771484e-8f;
 __device__ __forceinline__ float decay(float dt, float rate) { return seq::exp2_approx(fmaf(dt, rate, LIFT)); }
 __device__ __forceinline__ double decay(double dt, double rate) { return exp(dt * rate); }
-template <typename T> __device__ __forceinline__ T rate(T a);
-template <> __device__ __forceinline__ float rate(float a) { return a * 1.4426950408889634f; }
-template <> __device__ __forceinline__ double rate(double a) { return a; }
+// A' no lower than the type's lowest value: a state of A = -inf, which forgets everything, keeps its value over rows without a token,
+// where dt is zero, and takes no NaN into the gradient of dt.
+__device__ __forceinline__ float rate(float a) {
+  a *= 1.4426950408889634f;
+  return a < -3.402823466e38f ? -3.402823466e38f : a;        // (a NaN stays)
+}
+__device__ __forceinline__ double rate(double a) { return a < -1.7976931348623157e308 ? -1.7976931348623157e308 : a; }
 template <typename T> __device__ __forceinline__ T per_rate();         // A per A'
 template <> __device__ __forceinline__ float per_rate<float>() { return 0.6931471805599453f; }
 template <> __device__ __forceinline__ double per_rate<double>() { return 1.0; }
@@ -756,7 +760,9 @@ backward_edges_kernel(const Args<T> a) {
       landed<1>();
       __syncthreads();
       const T(*rows)[N] = m.C[tile0 / TT & 1];
-#pragma unroll 4
+      // (16384 tokens of 1024 channels with 16 states, backward: doubles 2338 us one by one and 2519 four by four, floats 560 and 542)
+      constexpr int AT_ONCE = sizeof(T) == 8 ? 1 : 4;
+#pragma unroll AT_ONCE
       for (int t = TT - 1; t >= 0; --t) {
         Two<T> dt, v2, C[P];
         read(&m.step[t][at], dt, v2);
