@@ -15,6 +15,8 @@
 namespace prad {
 namespace conv {
 
+using seq::load;
+using seq::Pack;
 using seq::Sequences;
 using seq::swish;
 using seq::swish_slope;
@@ -32,8 +34,6 @@ template <typename T> struct Args {
   unsigned blocks;               // CTAs along the tokens; those behind them see to the states
 };
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
-template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
 
 // A thread's ring of rows: rows go in by asynchronous copies, one group of copies a row, and come out in their order.
 template <typename T, int V> struct Ring {

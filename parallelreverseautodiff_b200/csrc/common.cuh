@@ -217,6 +217,20 @@ template <auto Kernel> inline prad_status allow_smem(prad_ctx* ctx, int bytes) {
   return PRAD_OK;
 }
 
+// CTAs of a kernel that the device holds at a time
+template <auto Kernel> inline int64_t resident(prad_ctx* ctx, int threads, int smem) {
+  static std::atomic<int> each{0};           // per SM: the same for every device this library is built for
+  int n = each.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, smem) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = 1;
+    }
+    each.store(n, std::memory_order_relaxed);
+  }
+  return (int64_t)n * ctx->sm_count;
+}
+
 // ---- internal entry points shared between translation units -------------------------------
 struct GemmEpilogue {
   // C = alpha*acc + beta*C ; then  + bias[n] ; store Z_out ; then act / act' multiply

@@ -3,6 +3,7 @@
 // numbers: as easy as 1, 2, 3", 2011) with the counter (i / 4, offset) and the key seed is below (1 - p) 2^32, and is 0 otherwise,
 // whatever x_i is.  The words depend neither on the launch nor on alignment.
 #include "common.cuh"
+#include "packed_sequences.cuh"
 
 namespace prad {
 namespace drop {
@@ -25,7 +26,7 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint64_
   return make_uint4(x0, x1, x2, x3);
 }
 
-template <typename T> struct alignas(16) Vec { T v[16 / sizeof(T)]; };
+template <typename T> using Vec = seq::Pack<T, 16 / sizeof(T)>;
 template <typename T> struct Four { T v[4]; };
 template <typename T, bool VECTOR> __device__ __forceinline__ Four<T> load4(const T* p, int left) {
   Four<T> f;

@@ -23,6 +23,8 @@
 namespace prad {
 namespace gn {
 
+using seq::load;
+using seq::Pack;
 using seq::swish;
 using seq::swish_slope;
 
@@ -37,9 +39,6 @@ template <typename T> struct Args {
   int act, wide;                 // wide: gamma and beta can be read as many values at a time as x
 };
 
-__host__ __device__ inline int64_t ceil_rounds(int64_t n, int64_t by) { return (n + by - 1) / by; }
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
-template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
 
 // V values of gamma or beta from channel c on; `none` without any
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> parameters(const Args<T>& a, const T* p, int c, T none) {
@@ -705,25 +704,11 @@ cluster_backward_kernel(const Args<T> a, const Parts k, double* __restrict__ sum
 constexpr int SUMMED = 512;
 template <typename T, int V> constexpr int most_in_registers() { return 32 * 8 * V; }
 
-// CTAs of a kernel that an SM holds (the same for every device this library is built for)
-template <auto Kernel> static int resident() {
-  static std::atomic<int> each{0};
-  int n = each.load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, THREADS, 0) != cudaSuccess || n < 1) {
-      (void)cudaGetLastError();
-      n = 1;
-    }
-    each.store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 template <typename T, int V, int LW, int E> static prad_status rows(prad_ctx* ctx, const Args<T>& a, bool backward) {
   // Forward a slot for every R samples of a group.  Backward as many slots as the device holds, or a multiple: each leaves sums of its own.
   int64_t per_group = ceil_div(a.samples, rows_at_once<E>());
   if (backward) {
-    const int64_t fill = (int64_t)ctx->sm_count * resident<rows_backward_kernel<T, V, LW, E>>() * THREADS / LW;
+    const int64_t fill = resident<rows_backward_kernel<T, V, LW, E>>(ctx, THREADS, 0) * THREADS / LW;
     per_group = fill / a.groups;
     if (per_group < 1) per_group = 1;
     if (sizeof(T) == 4) per_group *= ceil_div(a.samples, per_group * SUMMED);

@@ -1,5 +1,5 @@
-// What the kernels over packed sequences share: which rows of the token matrix belong to which sequence, and the scalar
-// functions of the layers they run in.
+// What the kernels of state space layers share: which rows of the token matrix belong to which sequence, packs of values, and the
+// scalar functions of the layers they run in.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -33,6 +33,10 @@ struct Sequences {
     return lo;
   }
 };
+
+// V values side by side, read and written at a time
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
 
 // 1 / (1 + 2^(-x log2 e)): two steps of the special function unit, each within 2 units of the last place
 __device__ __forceinline__ float reciprocal(float x) {

@@ -28,6 +28,7 @@
 namespace prad {
 namespace ssm {
 
+using seq::Pack;
 using seq::Sequences;
 using seq::swish;
 using seq::swish_slope;
@@ -178,8 +179,6 @@ __device__ __forceinline__ void read(const StepD* m, Two<double>& dt, Two<double
   dt = {q.x, q.x};
   x = {q.y, q.y};
 }
-
-template <typename T, int S> struct alignas(sizeof(T) * S) Pack { T v[S]; };
 
 // How a warp's lanes share channels and states: a lane's number among the L of its channel is made of the lane's bits 1, 4, 3, 2, 0 (as
 // many as L needs), its channel's number of the others.  A 128-bit read of shared memory takes two cycles if its address does not
@@ -1391,20 +1390,6 @@ step_kernel(const Args<T> a) {
 // ---------------------------------------------------------------- launches
 enum class Pass { Forward, Backward, Step };
 
-// CTAs of a kernel that the device holds at a time
-template <auto Kernel> static int64_t resident(prad_ctx* ctx, int smem) {
-  static std::atomic<int> each{0};           // per SM: the same for every device this library is built for
-  int n = each.load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, THREADS, smem) != cudaSuccess || n < 1) {
-      (void)cudaGetLastError();
-      n = 1;
-    }
-    each.store(n, std::memory_order_relaxed);
-  }
-  return (int64_t)n * ctx->sm_count;
-}
-
 // How the token axis is cut: by sequences where they are of equal length and fill at least half of the device (the edges' pass is
 // about half of the work again), else into spans of whole tiles, as many as the device holds at a time: one CTA more takes as long
 // as twice as many.  Each span costs a CTA's beginning and end and leaves sums of its own, dim x state values, which is more than
@@ -1431,7 +1416,7 @@ template <typename T> static void cut(Args<T>& a, int64_t across, int64_t full) 
 // whether a span may begin inside a sequence
 template <typename T> static bool joined(const Args<T>& a) { return a.spans > 1 && (a.rows.offsets || a.span % a.rows.each != 0); }
 
-template <typename T> struct Carve {
+struct Carve {
   char* at;
   size_t used = 0;
   template <typename U> U* take(int64_t n) {
@@ -1442,18 +1427,18 @@ template <typename T> struct Carve {
 };
 // `rows`: CTAs whose sums of dB and dC there is room for
 template <typename T> static size_t carve(Args<T>& a, bool backward, int rows, void* ws) {
-  Carve<T> c{(char*)ws};
+  Carve c{(char*)ws};
   const int64_t states = (int64_t)a.dim * a.state;
   if (joined(a)) {
-    a.edge = c.template take<T>((a.spans + 1) * states);
-    a.sum = c.template take<T>((int64_t)a.spans * a.dim);
-    a.passes = c.template take<int>(a.spans);
+    a.edge = c.take<T>((a.spans + 1) * states);
+    a.sum = c.take<T>((int64_t)a.spans * a.dim);
+    a.passes = c.take<int>(a.spans);
   }
   if (backward) {
-    a.part_A = c.template take<T>(a.spans * states);
-    a.part_D = c.template take<T>((int64_t)a.spans * a.dim);
-    a.part_bias = c.template take<T>((int64_t)a.spans * a.dim);
-    if (rows) a.part_BC = c.template take<T>((int64_t)rows * a.rows.tokens * a.groups * 2 * a.state);
+    a.part_A = c.take<T>(a.spans * states);
+    a.part_D = c.take<T>((int64_t)a.spans * a.dim);
+    a.part_bias = c.take<T>((int64_t)a.spans * a.dim);
+    if (rows) a.part_BC = c.take<T>((int64_t)rows * a.rows.tokens * a.groups * 2 * a.state);
   }
   return c.used;
 }
@@ -1504,7 +1489,7 @@ template <typename T, int L, int S, int FL, int FS> static prad_status launch(pr
   constexpr int edge_bytes = (int)sizeof(Edges<T, L, S>);
   if (!st) st = backward ? allow_smem<backward_edges_kernel<T, L, S>>(ctx, edge_bytes) : allow_smem<forward_kernel<T, FL, FS, true>>(ctx, bytes);
   if (st) return st;
-  cut(a, across, backward ? resident<backward_kernel<T, L, S>>(ctx, (int)sizeof(Shared)) : resident<forward_kernel<T, FL, FS, false>>(ctx, bytes));
+  cut(a, across, backward ? resident<backward_kernel<T, L, S>>(ctx, THREADS, (int)sizeof(Shared)) : resident<forward_kernel<T, FL, FS, false>>(ctx, THREADS, bytes));
   st = ensure_workspace(ctx, carve(a, backward, rows, nullptr));
   if (st) return st;
   carve(a, backward, rows, ctx->ws);
