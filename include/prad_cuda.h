@@ -570,9 +570,10 @@ prad_status prad_causal_conv_step(prad_ctx* ctx, prad_dtype dt, const void* x, i
  *   dt = delta + delta_bias[d], softplus of it if delta_softplus;  h_n <- exp(dt * A[d][n]) * h_n + dt * u * B[group][n];
  *   r = sum_n C[group][n] * h_n + D[d] * u;  y = r, or r * swish(z) with a z.
  * u, delta, z, y: [tokens x dim]; A: [dim x state]; B, C: [tokens x groups * state]; D, delta_bias: [dim]; h0, h_last: [sequences
- * x dim * state].  z, D, delta_bias and h0 may be NULL (none, 0, 0, 0), h_last as well.  `saved` (prad_selective_scan_saved_bytes,
- * by the scan's sizes alone: all states of every eighth token) keeps what the backward needs; NULL where none follows.  The backward does not differentiate h_last; of its
- * results dA, dD, ddelta_bias and dh0 may be NULL, and dz where there is no z. */
+ * x dim * state].  A counts as no lower than the type's lowest value (-inf forgets everything).  z, D, delta_bias and h0 may be NULL
+ * (none, 0, 0, 0), h_last as well.  `saved` (prad_selective_scan_saved_bytes, by the scan's sizes alone: all states of every eighth
+ * token) keeps what the backward needs; NULL where none follows.  The backward does not differentiate h_last; of its results dA, dD,
+ * ddelta_bias and dh0 may be NULL, and dz where there is no z. */
 typedef struct {
   int64_t tokens;
   int32_t sequences, dim, state, groups, delta_softplus;

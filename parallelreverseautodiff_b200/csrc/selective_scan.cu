@@ -41,8 +41,8 @@ constexpr int THREADS = 128;
 template <typename T, int L> constexpr int tile() { return sizeof(T) == 8 || L == 2 ? 16 : 32; }
 // spans are multiples of this many tokens, and two of them at least
 template <typename T> constexpr int span_unit() { return sizeof(T) == 8 ? 16 : 32; }
-// Tokens per checkpoint, and TT of the main backward pass: with 8 shared memory leaves room for three CTAs (16384 tokens of 1024 floats
-// with 16 states: 470 us when this was chosen; with 16, half of the checkpoints and two CTAs, 518).
+// Tokens per checkpoint, and TT of the main backward pass: with 8 shared memory leaves room for three CTAs, with 16 there are half of
+// the checkpoints and two CTAs (the pass took 518 us for 470 when this was chosen, with later steps 446).
 constexpr int POINT = 8;
 constexpr int MAX_STATE = 128;
 
